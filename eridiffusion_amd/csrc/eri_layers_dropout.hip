@@ -1,0 +1,56 @@
+/*
+ * Dropout of include/eri_layers.h: y = keep ? x / share : 0, the mask drawn from Philox4x32-10 where it is needed.
+ */
+#include "eri_layers_device.h"
+
+namespace eri_layers {
+namespace {
+
+constexpr uint32_t kThreads = 256;
+
+struct DropoutArgs {
+    const void *x;
+    void *y;
+    uint64_t cols, vectors; // vectors: of a row
+    uint32_t rows;
+    uint64_t x_stride, y_stride;
+    Drop drop;
+};
+
+template <typename T> __global__ __launch_bounds__(kThreads) void dropout_kernel(const DropoutArgs a) {
+    const uint64_t offset = drop_offset(a.drop);
+    for (uint32_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
+        const T *x = (const T *)a.x + row * a.x_stride;
+        T *y = (T *)a.y + row * a.y_stride;
+        for (uint64_t v = (uint64_t)blockIdx.x * kThreads + threadIdx.x; v < a.vectors; v += (uint64_t)gridDim.x * kThreads) {
+            const uint64_t col = v * 8, left = a.cols - col;
+            const uint32_t n = left < 8 ? (uint32_t)left : 8u;
+            Raw<T> r;
+            load8(r, x + col, 0, n);
+            const u32x4 bits = draw8(row * a.cols + col, a.drop, offset);
+            float out[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) out[e] = dropped(r.get(e), bits, e, a.drop);
+            store8(y + col, 0, n, out);
+        }
+    }
+}
+
+} // namespace
+
+int launch_dropout(const EriDropout &e, const Drop &d, uint32_t compute_units, void *stream) {
+    DropoutArgs a = {e.x, e.y, e.cols, 0, (uint32_t)e.rows, e.x_stride, e.y_stride, d};
+    if (e.x_stride == e.cols && e.y_stride == e.cols) { // no gaps: one long row
+        a.cols = e.rows * e.cols;
+        a.rows = 1;
+    }
+    a.vectors = (a.cols + 7) / 8;
+    const uint64_t x = (a.vectors + kThreads - 1) / kThreads, most = (uint64_t)compute_units * 64;
+    const dim3 grid((uint32_t)(x < most ? x : most), a.rows < 65535 ? a.rows : 65535);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (e.dtype_tag == ERI_DTYPE_F32) hipLaunchKernelGGL(dropout_kernel<float>, grid, dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL(dropout_kernel<bf16>, grid, dim3(kThreads), 0, s, a);
+    return (int)hipGetLastError();
+}
+
+} // namespace eri_layers

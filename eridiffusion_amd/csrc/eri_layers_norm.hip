@@ -1,0 +1,208 @@
+/*
+ * Residual addition and root-mean-square norm of include/eri_layers.h, forward.
+ */
+#include "eri_layers_device.h"
+
+namespace eri_layers {
+namespace {
+
+constexpr float kF8Max = 448.0f;
+constexpr uint32_t rows_of(uint32_t tpr) { return tpr < 256 ? 256 / tpr : 1; } // of a workgroup
+
+struct NormArgs {
+    const void *x, *residual, *weight;
+    void *y, *h;
+    float *rstd, *scales;
+    uint32_t rows, cols;
+    uint64_t x_stride, residual_stride, y_stride, h_stride;
+    float eps;
+    uint32_t weight_f32, y_dtype, group, groups;
+    Drop drop;
+};
+
+__device__ __forceinline__ void store8_f8(uint8_t *row, uint32_t col, uint32_t cols, const float (&v)[8]) {
+    uint32_t w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        int p = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
+        w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], p, true);
+    }
+    if (col + 8 <= cols) *(u32x2_at1 *)(row + col) = u32x2{w[0], w[1]};
+    else
+#pragma unroll
+        for (uint32_t e = 0; e < 7; ++e)
+            if (col + e < cols) row[col + e] = (uint8_t)(w[e / 4] >> (8 * (e & 3)));
+}
+
+/* h of elements col .. col+7 of a row, zero past its end. */
+template <typename TX, typename TR, bool RES, bool DROP>
+__device__ __forceinline__ void sum8(float (&h)[8], const Raw<TX> &x, const Raw<TR> &r, uint64_t first, const Drop &d, uint64_t offset) {
+    u32x4 bits = {0, 0, 0, 0};
+    if (DROP) bits = draw8(first, d, offset);
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) {
+        h[e] = x.get(e);
+        if (DROP) h[e] = dropped(h[e], bits, e, d);
+        if (RES) h[e] += r.get(e);
+    }
+}
+
+template <typename TX, typename TR, bool RES> __device__ __forceinline__ void store_h(const NormArgs &a, uint32_t row, uint32_t col, const float (&h)[8]) {
+    if (RES) store8((TR *)a.h + row * a.h_stride, col, a.cols, h);
+    else store8((TX *)a.h + row * a.h_stride, col, a.cols, h);
+}
+
+__device__ __forceinline__ void weigh(float (&v)[8], const NormArgs &a, uint32_t col, float rstd) {
+    float w[8];
+    if (a.weight) load8_of(w, a.weight, a.weight_f32, col, a.cols);
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) v[e] = a.weight ? v[e] * rstd * w[e] : v[e] * rstd;
+}
+
+/* y / scale as 8-bit floats; `most` is the largest |y| of the group */
+__device__ __forceinline__ void store_scaled(const NormArgs &a, uint32_t row, uint32_t col, const float (&v)[8], float most) {
+    const float inv = most > 0.0f ? kF8Max / most : 1.0f;
+    float q[8];
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) q[e] = v[e] * inv;
+    store8_f8((uint8_t *)a.y + row * a.y_stride, col, a.cols, q);
+}
+__device__ __forceinline__ float scale_of(float most) { return most > 0.0f ? most / kF8Max : 1.0f; }
+__device__ __forceinline__ float most_of(const float (&v)[8]) {
+    float m = 0.0f;
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) m = fmaxf(m, fabsf(v[e]));
+    return m;
+}
+
+/* A row to TPR threads, NV vectors of eight elements in the registers of each. */
+template <typename TX, typename TR, bool RES, bool DROP, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const NormArgs a) {
+    constexpr int kWaves = TPR / kWave;
+    __shared__ float slots[2][kWaves < 2 ? 1 : kWaves];
+    const uint32_t row = blockIdx.x * rows_of(TPR) + threadIdx.x / TPR, t = threadIdx.x % TPR;
+    if (row >= a.rows) return; // a whole wave, and only where a row is one wave's
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    Raw<TX> x[NV];
+    Raw<TR> r[NV];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) load8(x[k], (const TX *)a.x + row * a.x_stride, (k * TPR + t) * 8, a.cols);
+    if (RES)
+#pragma unroll
+        for (int k = 0; k < NV; ++k) load8(r[k], (const TR *)a.residual + row * a.residual_stride, (k * TPR + t) * 8, a.cols);
+    float h[NV][8], sum = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const uint32_t col = (k * TPR + t) * 8;
+        sum8<TX, TR, RES, DROP>(h[k], x[k], r[k], (uint64_t)row * a.cols + col, a.drop, offset);
+        if (a.h) store_h<TX, TR, RES>(a, row, col, h[k]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(h[k][e], h[k][e], sum);
+    }
+    const float rstd = 1.0f / sqrtf(group_sum<kWaves>(sum, slots[0]) / (float)a.cols + a.eps);
+    if (a.rstd && t == 0) a.rstd[row] = rstd;
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        const uint32_t col = (k * TPR + t) * 8;
+        weigh(h[k], a, col, rstd);
+        if (a.y_dtype == ERI_DTYPE_BF16) store8((bf16 *)a.y + row * a.y_stride, col, a.cols, h[k]);
+        else if (a.y_dtype == ERI_DTYPE_F32) store8((float *)a.y + row * a.y_stride, col, a.cols, h[k]);
+        else if (a.group) {
+            const float m = row16_max(most_of(h[k])); // 16 lanes hold 128 columns
+            store_scaled(a, row, col, h[k], m);
+            if (t % 16 == 0 && col < a.cols) a.scales[(uint64_t)row * a.groups + col / 128] = scale_of(m);
+        } else most = fmaxf(most, most_of(h[k]));
+    }
+    if (a.y_dtype == ERI_DTYPE_F8E4M3 && !a.group) {
+        most = group_max<kWaves>(most, slots[1]);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) store_scaled(a, row, (k * TPR + t) * 8, h[k], most);
+        if (t == 0) a.scales[row] = scale_of(most);
+    }
+}
+
+/* Rows too long for registers: read again for each of the passes.  h and y are written in the last one only, each
+ * element by the thread that has just read it, so that they may replace the residual and x. */
+template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a) {
+    __shared__ float slots[2][16];
+    const uint32_t row = blockIdx.x;
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    auto value = [&](float (&h)[8], uint32_t col) {
+        Raw<TX> x;
+        Raw<TR> r;
+        load8(x, (const TX *)a.x + row * a.x_stride, col, a.cols);
+        if (RES) load8(r, (const TR *)a.residual + row * a.residual_stride, col, a.cols);
+        sum8<TX, TR, RES, DROP>(h, x, r, (uint64_t)row * a.cols + col, a.drop, offset);
+    };
+    float sum = 0.0f;
+    for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
+        float h[8];
+        value(h, col);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(h[e], h[e], sum);
+    }
+    const float rstd = 1.0f / sqrtf(group_sum<16>(sum, slots[0]) / (float)a.cols + a.eps);
+    float most = 0.0f;
+    if (a.y_dtype == ERI_DTYPE_F8E4M3 && !a.group) {
+        for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
+            float h[8];
+            value(h, col);
+            weigh(h, a, col, rstd);
+            most = fmaxf(most, most_of(h));
+        }
+        most = group_max<16>(most, slots[1]);
+        if (threadIdx.x == 0) a.scales[row] = scale_of(most);
+    }
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+    // all lanes stay together to the last column: 16 of them share a group's maximum
+    for (uint32_t at = 0; at < a.cols; at += 8192) {
+        const uint32_t col = at + threadIdx.x * 8;
+        float h[8];
+        value(h, col);
+        if (a.h) store_h<TX, TR, RES>(a, row, col, h);
+        weigh(h, a, col, rstd);
+        if (a.y_dtype == ERI_DTYPE_BF16) store8((bf16 *)a.y + row * a.y_stride, col, a.cols, h);
+        else if (a.y_dtype == ERI_DTYPE_F32) store8((float *)a.y + row * a.y_stride, col, a.cols, h);
+        else if (a.group) {
+            const float m = row16_max(most_of(h));
+            store_scaled(a, row, col, h, m);
+            if (threadIdx.x % 16 == 0 && col < a.cols) a.scales[(uint64_t)row * a.groups + col / 128] = scale_of(m);
+        } else store_scaled(a, row, col, h, most);
+    }
+}
+
+template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormArgs &a, uint32_t compute_units, hipStream_t s) {
+#define ERI_NORM(TPR, NV) \
+    hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV>), dim3((a.rows + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+    if (a.cols <= 512) ERI_NORM(64, 1);
+    else if (a.cols <= 1024) ERI_NORM(64, 2);
+    else if (a.cols <= 2048) ERI_NORM(64, 4);
+    else if (a.cols <= 4096) ERI_NORM(256, 2);
+    else if (a.cols <= 8192) ERI_NORM(256, 4);
+    else if (a.cols <= 16384) ERI_NORM(1024, 2);
+    else if (a.cols <= 32768) ERI_NORM(1024, 4);
+    else hipLaunchKernelGGL((rms_norm_long_kernel<TX, TR, RES, DROP>), dim3(a.rows), dim3(1024), 0, s, a);
+#undef ERI_NORM
+}
+
+template <typename TX> void launch_of(const NormArgs &a, bool res, bool res_f32, uint32_t compute_units, hipStream_t s) {
+    const bool drop = a.drop.below != 0;
+    if (!res) drop ? launch<TX, TX, false, true>(a, compute_units, s) : launch<TX, TX, false, false>(a, compute_units, s);
+    else if (res_f32) drop ? launch<TX, float, true, true>(a, compute_units, s) : launch<TX, float, true, false>(a, compute_units, s);
+    else drop ? launch<TX, bf16, true, true>(a, compute_units, s) : launch<TX, bf16, true, false>(a, compute_units, s);
+}
+
+} // namespace
+
+int launch_rms_norm(const EriRmsNorm &e, const Drop &d, uint32_t compute_units, void *stream) {
+    const NormArgs a = {e.x, e.residual, e.weight, e.y, e.h, e.rstd, e.scales, (uint32_t)e.rows, (uint32_t)e.cols,
+                        e.x_stride, e.residual_stride, e.y_stride, e.h_stride, e.eps, e.weight_dtype == ERI_DTYPE_F32, (uint32_t)e.y_dtype,
+                        (uint32_t)e.scale_group, e.scale_group ? (uint32_t)((e.cols + 127) / 128) : 1u, d};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (e.x_dtype == ERI_DTYPE_F32) launch_of<float>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, compute_units, s);
+    else launch_of<bf16>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, compute_units, s);
+    return (int)hipGetLastError();
+}
+
+} // namespace eri_layers

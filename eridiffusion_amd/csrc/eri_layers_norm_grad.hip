@@ -1,0 +1,234 @@
+/*
+ * Gradient of the residual addition and root-mean-square norm of include/eri_layers.h.
+ */
+#include "eri_layers_device.h"
+
+namespace eri_layers {
+namespace {
+
+struct NormGradArgs {
+    const void *grad, *h, *weight, *grad_h;
+    const float *rstd;
+    void *grad_x, *grad_residual;
+    float *partial; // per workgroup a row of grad_weight's sums, padded floats apart; NULL: not wanted
+    uint32_t rows, cols, padded;
+    uint64_t grad_stride, h_stride, grad_h_stride, grad_x_stride, grad_residual_stride;
+    uint32_t weight_f32, x_f32;
+    Drop drop;
+};
+
+constexpr uint32_t kRowsOf(int tpr) { return tpr < 256 ? 256 / tpr : 1; }
+
+template <typename TR, bool DROP>
+__device__ __forceinline__ void store_grads(const NormGradArgs &a, uint32_t row, uint32_t col, float (&dh)[8], uint64_t offset) {
+    if (a.grad_residual) store8((TR *)a.grad_residual + row * a.grad_residual_stride, col, a.cols, dh);
+    if (!a.grad_x) return;
+    if (DROP) {
+        const u32x4 bits = draw8((uint64_t)row * a.cols + col, a.drop, offset);
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) dh[e] = dropped(dh[e], bits, e, a.drop);
+    }
+    if (a.x_f32) store8((float *)a.grad_x + row * a.grad_x_stride, col, a.cols, dh);
+    else store8((bf16 *)a.grad_x + row * a.grad_x_stride, col, a.cols, dh);
+}
+
+/* A row at a time to TPR threads, which keep the weight and their columns' sums of grad_weight in registers. */
+template <typename TG, typename TR, bool DROP, int TPR, int NV>
+__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(const NormGradArgs a) {
+    constexpr int kWaves = TPR / kWave;
+    __shared__ float slots[2][kWaves < 2 ? 1 : kWaves];
+    __shared__ float joined[TPR < 256 ? TPR * NV * 8 : 1];
+    const uint32_t t = threadIdx.x % TPR;
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    float w[NV][8], acc[NV][8];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+        if (a.weight) load8_of(w[k], a.weight, a.weight_f32, (k * TPR + t) * 8, a.cols);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            acc[k][e] = 0.0f;
+            if (!a.weight) w[k][e] = 1.0f;
+        }
+    }
+    uint32_t turn = 0;
+    for (uint32_t row = blockIdx.x * kRowsOf(TPR) + threadIdx.x / TPR; row < a.rows; row += gridDim.x * kRowsOf(TPR), turn ^= 1) {
+        Raw<TG> g[NV];
+        Raw<TR> h[NV], r[NV];
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            load8(g[k], (const TG *)a.grad + row * a.grad_stride, (k * TPR + t) * 8, a.cols);
+            load8(h[k], (const TR *)a.h + row * a.h_stride, (k * TPR + t) * 8, a.cols);
+        }
+        if (a.grad_h)
+#pragma unroll
+            for (int k = 0; k < NV; ++k) load8(r[k], (const TR *)a.grad_h + row * a.grad_h_stride, (k * TPR + t) * 8, a.cols);
+        else
+#pragma unroll
+            for (int k = 0; k < NV; ++k) r[k].clear();
+        const float rstd = a.rstd[row];
+        float c = 0.0f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                const float gh = g[k].get(e) * h[k].get(e);
+                c = fmaf(gh, w[k][e], c);
+                acc[k][e] = fmaf(gh, rstd, acc[k][e]);
+            }
+        c = group_sum<kWaves>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float dh[8];
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) dh[e] = fmaf(g[k].get(e) * w[k][e], rstd, fmaf(-h[k].get(e), c, r[k].get(e)));
+            store_grads<TR, DROP>(a, row, (k * TPR + t) * 8, dh, offset);
+        }
+    }
+    if (!a.partial) return;
+    if (TPR < 256) { // the waves' sums, one after the other
+        for (uint32_t turn = 0; turn < kRowsOf(TPR); ++turn) {
+            if (threadIdx.x / TPR == turn)
+#pragma unroll
+                for (int k = 0; k < NV; ++k)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float *j = joined + (k * 8 + e) * TPR + t;
+                        *j = acc[k][e] += turn ? *j : 0.0f;
+                    }
+            __syncthreads();
+        }
+        if (threadIdx.x / TPR != kRowsOf(TPR) - 1) return;
+    }
+    float *out = a.partial + (uint64_t)blockIdx.x * a.padded;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) store8(out, (k * TPR + t) * 8, a.padded, acc[k]);
+}
+
+/* Rows too long for registers: read twice, and the sums of grad_weight kept in the workgroup's row of partial. */
+template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(const NormGradArgs a) {
+    __shared__ float slots[2][16];
+    const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
+    float *out = a.partial ? a.partial + (uint64_t)blockIdx.x * a.padded : nullptr;
+    uint32_t turn = 0;
+    for (uint32_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+        const float rstd = a.rstd[row];
+        float c = 0.0f;
+        for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
+            Raw<TG> g;
+            Raw<TR> h;
+            float w[8], gh[8];
+            load8(g, (const TG *)a.grad + row * a.grad_stride, col, a.cols);
+            load8(h, (const TR *)a.h + row * a.h_stride, col, a.cols);
+            if (a.weight) load8_of(w, a.weight, a.weight_f32, col, a.cols);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) {
+                gh[e] = g.get(e) * h.get(e);
+                c = fmaf(gh[e], a.weight ? w[e] : 1.0f, c);
+            }
+            if (out) {
+                float old[8];
+                load8_of(old, out, true, col, a.padded);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) old[e] = row == blockIdx.x ? gh[e] * rstd : fmaf(gh[e], rstd, old[e]);
+                store8(out, col, a.padded, old);
+            }
+        }
+        c = group_sum<16>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
+        for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
+            Raw<TG> g;
+            Raw<TR> h, r;
+            float w[8], dh[8];
+            load8(g, (const TG *)a.grad + row * a.grad_stride, col, a.cols);
+            load8(h, (const TR *)a.h + row * a.h_stride, col, a.cols);
+            if (a.grad_h) load8(r, (const TR *)a.grad_h + row * a.grad_h_stride, col, a.cols);
+            else r.clear();
+            if (a.weight) load8_of(w, a.weight, a.weight_f32, col, a.cols);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) dh[e] = fmaf(a.weight ? g.get(e) * w[e] : g.get(e), rstd, fmaf(-h.get(e), c, r.get(e)));
+            store_grads<TR, DROP>(a, row, col, dh, offset);
+        }
+    }
+}
+
+/* grad_weight out of the workgroups' sums: 64 columns to a workgroup, 64 groups of rows, joined in their order. */
+__global__ __launch_bounds__(1024) void rms_norm_grad_weight_kernel(const float *partial, uint32_t n, uint32_t padded, void *out, uint32_t cols, uint32_t out_f32) {
+    __shared__ float sums[64][64];
+    const uint32_t quad = threadIdx.x % 16, part = threadIdx.x / 16, col = blockIdx.x * 64 + quad * 4;
+    float s[4] = {0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t r = part; r < n; r += 64) {
+        const float4 v = *(const float4 *)(partial + (uint64_t)r * padded + col);
+        s[0] += v.x, s[1] += v.y, s[2] += v.z, s[3] += v.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[part][quad * 4 + e] = s[e];
+    __syncthreads();
+    const uint32_t c = blockIdx.x * 64 + threadIdx.x;
+    if (threadIdx.x >= 64 || c >= cols) return;
+    float total = 0.0f;
+    for (uint32_t p = 0; p < 64; ++p) total += sums[p][threadIdx.x];
+    if (out_f32) ((float *)out)[c] = total;
+    else store_one((bf16 *)out + c, total);
+}
+
+/* Threads to a row, and how many workgroups the rows are dealt to. */
+struct Shape {
+    int tpr, nv; // nv 0: rows too long for registers
+    uint32_t groups;
+};
+Shape shape_of(uint64_t rows, uint64_t cols, uint32_t compute_units) {
+    Shape s = cols <= 512 ? Shape{64, 1, 0} : cols <= 1024 ? Shape{64, 2, 0} : cols <= 2048 ? Shape{256, 1, 0} : cols <= 4096 ? Shape{256, 2, 0} :
+              cols <= 8192 ? Shape{256, 4, 0} : cols <= 16384 ? Shape{1024, 2, 0} : cols <= 32768 ? Shape{1024, 4, 0} : Shape{1024, 0, 0};
+    const uint64_t all = (rows + kRowsOf(s.tpr) - 1) / kRowsOf(s.tpr), most = (uint64_t)compute_units * (s.tpr == 1024 ? 1 : 4);
+    s.groups = (uint32_t)(all < most ? all : most);
+    return s;
+}
+uint64_t padded_of(uint64_t cols) { return (cols + 63) / 64 * 64; }
+
+template <typename TG, typename TR, bool DROP> void launch(const NormGradArgs &a, const Shape &shape, hipStream_t s) {
+#define ERI_NORM_GRAD(TPR, NV) \
+    if (shape.tpr == TPR && shape.nv == NV) \
+    hipLaunchKernelGGL((rms_norm_grad_kernel<TG, TR, DROP, TPR, NV>), dim3(shape.groups), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+    ERI_NORM_GRAD(64, 1);
+    ERI_NORM_GRAD(64, 2);
+    ERI_NORM_GRAD(256, 1);
+    ERI_NORM_GRAD(256, 2);
+    ERI_NORM_GRAD(256, 4);
+    ERI_NORM_GRAD(1024, 2);
+    ERI_NORM_GRAD(1024, 4);
+#undef ERI_NORM_GRAD
+    if (shape.nv == 0) hipLaunchKernelGGL((rms_norm_grad_long_kernel<TG, TR, DROP>), dim3(shape.groups), dim3(1024), 0, s, a);
+}
+
+template <typename TG> void launch_of(const NormGradArgs &a, bool h_f32, const Shape &shape, hipStream_t s) {
+    if (h_f32) a.drop.below ? launch<TG, float, true>(a, shape, s) : launch<TG, float, false>(a, shape, s);
+    else a.drop.below ? launch<TG, bf16, true>(a, shape, s) : launch<TG, bf16, false>(a, shape, s);
+}
+
+} // namespace
+
+uint64_t rms_norm_grad_workspace(uint64_t rows, uint64_t cols, uint32_t compute_units) {
+    return shape_of(rows, cols, compute_units).groups * padded_of(cols) * sizeof(float);
+}
+
+int launch_rms_norm_grad(const EriRmsNormGrad &e, const Drop &d, uint32_t compute_units, void *stream) {
+    const Shape shape = shape_of(e.rows, e.cols, compute_units);
+    const uint32_t padded = (uint32_t)padded_of(e.cols);
+    float *partial = e.grad_weight ? (float *)e.workspace : nullptr;
+    const NormGradArgs a = {e.grad, e.h, e.weight, e.grad_h, e.rstd, e.grad_x, e.grad_residual, partial, (uint32_t)e.rows, (uint32_t)e.cols, padded,
+                            e.grad_stride, e.h_stride, e.grad_h_stride, e.grad_x_stride, e.grad_residual_stride, e.weight_dtype == ERI_DTYPE_F32,
+                            e.x_dtype == ERI_DTYPE_F32, d};
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (e.rows) {
+        if (e.grad_dtype == ERI_DTYPE_F32) launch_of<float>(a, e.h_dtype == ERI_DTYPE_F32, shape, s);
+        else launch_of<bf16>(a, e.h_dtype == ERI_DTYPE_F32, shape, s);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return (int)err;
+    }
+    if (e.grad_weight)
+        hipLaunchKernelGGL(rms_norm_grad_weight_kernel, dim3(padded / 64), dim3(1024), 0, s, partial, shape.groups, padded, e.grad_weight,
+                           (uint32_t)e.cols, (uint32_t)(e.grad_weight_dtype == ERI_DTYPE_F32));
+    return (int)hipGetLastError();
+}
+
+} // namespace eri_layers

@@ -42,6 +42,11 @@ fn main() {
         ("eri_adam8_step_plain.hip", "step_plain_f32", "-DERI_PLAIN_LAYOUT=0", true),
         ("eri_optim8_api.cpp", "api", "", true),
         ("eri_adam8bit_host.cpp", "host", "", false),
+        ("eri_layers_api.cpp", "layers_api", "", true),
+        ("eri_layers_dropout.hip", "layers_dropout", "", true),
+        ("eri_layers_norm.hip", "layers_norm", "", true),
+        ("eri_layers_norm_grad.hip", "layers_norm_grad", "", true),
+        ("eri_layers_embedding.hip", "layers_embedding", "", true),
     ] {
         let obj = out.join(format!("{obj_name}.o"));
         let mut cmd = Command::new(&hipcc);
@@ -67,7 +72,7 @@ fn main() {
     println!("cargo:rustc-link-search=native=/opt/rocm/lib");
     println!("cargo:rustc-link-lib=dylib=amdhip64");
     println!("cargo:rustc-link-lib=dylib=stdc++");
-    for h in ["eri_adam8_device.h", "eri_adam8_inline.h", "eri_dynamic_maps.inc"] {
+    for h in ["eri_adam8_device.h", "eri_adam8_inline.h", "eri_dynamic_maps.inc", "eri_layers_device.h"] {
         println!("cargo:rerun-if-changed=csrc/{h}");
     }
 }
