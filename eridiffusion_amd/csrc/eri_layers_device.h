@@ -190,14 +190,11 @@ __device__ __forceinline__ u32x4 draw8(uint64_t first, const Drop &d, uint64_t o
     const uint32_t s = (uint32_t)first & 7u;
     if (s == 0) return w;
     const u32x4 n = philox((first >> 3) + 1, offset, d.seed);
-    uint32_t v[8] = {w[0], w[1], w[2], w[3], n[0], n[1], n[2], n[3]};
-#pragma unroll
-    for (int k = 0; k < 6; ++k) v[k] = s & 4 ? v[k + 2] : v[k];
-#pragma unroll
-    for (int k = 0; k < 5; ++k) v[k] = s & 2 ? v[k + 1] : v[k];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] = s & 1 ? (v[k] >> 16) | (v[k + 1] << 16) : v[k];
-    return u32x4{v[0], v[1], v[2], v[3]};
+    const bool by4 = s & 4, by2 = s & 2;
+    const uint32_t b0 = by4 ? w[2] : w[0], b1 = by4 ? w[3] : w[1], b2 = by4 ? n[0] : w[2], b3 = by4 ? n[1] : w[3], b4 = by4 ? n[2] : n[0], b5 = by4 ? n[3] : n[1];
+    const uint32_t c0 = by2 ? b1 : b0, c1 = by2 ? b2 : b1, c2 = by2 ? b3 : b2, c3 = by2 ? b4 : b3, c4 = by2 ? b5 : b4;
+    if (!(s & 1)) return u32x4{c0, c1, c2, c3};
+    return u32x4{c0 >> 16 | c1 << 16, c1 >> 16 | c2 << 16, c2 >> 16 | c3 << 16, c3 >> 16 | c4 << 16};
 }
 
 __device__ __forceinline__ uint64_t drop_offset(const Drop &d) { return d.offset + (d.offset_ptr ? *d.offset_ptr : 0); }
