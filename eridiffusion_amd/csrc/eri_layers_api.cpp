@@ -108,7 +108,7 @@ int eri_embedding(const EriEmbedding *args, void *stream) {
 int eri_embedding_grad_workspace(uint64_t tokens, uint64_t vocab, uint64_t dim, uint64_t *bytes) {
     constexpr const char *kCall = "eri_embedding_grad_workspace";
     ERI_NEED(bytes, ERI_ERR_NULL, "bytes is NULL");
-    if (int rc = ids_ok("", 0, 0, vocab, dim, kCall)) return rc;
+    if (int rc = ids_ok(nullptr, 0, 0, vocab, dim, kCall)) return rc;
     ERI_NEED(tokens <= kCountMost, ERI_ERR_TOO_LARGE, "more than 2^31 - 1 tokens");
     *bytes = eri_layers::embedding_grad_workspace(tokens, vocab, dim);
     return 0;

@@ -70,53 +70,53 @@ template <typename T> void launch_lookup_of(const LookupArgs &a, uint32_t comput
 // ---------------------------------------------------------------------------------------------
 
 /*
- * Ids are dealt to K = 2^shift buckets by their low bits, a workgroup to a bucket.  It reads all ids twice, in order:
- * the first time it counts its own ones, each wave for its share of the tokens; the second time it writes the tokens of
- * each of its ids, in ascending order, to its part of `order`.  Where that part begins, it has counted too, as the
- * number of tokens in the buckets before it: no workgroup waits for another.  Then it writes its rows of the gradient:
- * zeros where no token names the row, the sum of up to kFew rows of grad.  Rows with more tokens go to a second kernel,
- * which spreads each over many workgroups.
+ * Sorting: ids are dealt to K = 2^shift buckets by their low bits, a workgroup to a bucket.  It reads all ids twice, in
+ * order: the first time it counts its own ones, each wave for its share of the tokens; the second time it writes the
+ * tokens of each of its ids, in ascending order, to its part of the sorted list.  Where that part begins, it has counted
+ * too, as the number of tokens in the buckets before it: no workgroup waits for another.  Between the two it writes the
+ * rows that no token names: stores that nothing waits for.
+ *
+ * Summing: the runs of equal ids in the sorted list are cut into pieces of kPiece tokens, and a wave sums the pieces that
+ * begin in its kStep places of the list, for L*8 columns: its loads go ahead through the list whatever the
+ * lengths of the runs, and a wave has at most kStep + kPiece - 1 tokens.  A run of one piece is written as it ends; the pieces
+ * of longer ones are left in the workspace and summed in their order by a third kernel.
  */
 constexpr uint32_t kWaves = 16;       // of a bucket's workgroup
 constexpr uint32_t kLocalMost = 1024; // ids of a bucket
-constexpr uint32_t kFew = 64;
+constexpr uint32_t kPiece = 64;
+constexpr uint32_t kStep = 16;
+constexpr uint32_t kAhead = 8;        // rows whose loads are under way together
 
-struct Heavy { // a row with more than kFew tokens
-    uint32_t id, start, count, unused;
+struct Place { // of the sorted list
+    uint32_t token, id;
+    uint32_t at, run; // place within the run of tokens with that id, and the run's length
 };
 
 struct GradArgs {
     Ids ids;
     const void *grad;
     void *out;
-    uint32_t *order;  // tokens numbers
-    Heavy *heavy;     // bucket b's from place heavy_first[b] on
-    uint32_t *heavy_first, *heavy_count; // one per bucket
-    uint32_t tokens, vocab, dim, shift, locals;
+    Place *sorted;    // tokens places, of which the first *used are set
+    uint32_t *used;
+    float *partial;   // sums of pieces, padded floats each
+    uint32_t tokens, vocab, dim, shift, locals, padded, tiles;
     uint64_t grad_stride, out_stride;
     int64_t padding_id;
     float scale;
-    uint32_t accumulate;
+    uint32_t accumulate, out_bytes, lanes; // lanes to a row of zeros
     __device__ __forceinline__ bool counts(int64_t id) const { return (uint64_t)id < vocab && id != padding_id; }
 };
 
-template <typename TO> __device__ __forceinline__ void finish8(const GradArgs &a, uint32_t id, uint32_t col, float (&v)[8]) {
-    TO *row = (TO *)a.out + id * a.out_stride;
-    Raw<TO> old;
-    if (a.accumulate) load8(old, row, col, a.dim);
-    else old.clear();
-#pragma unroll
-    for (uint32_t e = 0; e < 8; ++e) v[e] = v[e] * a.scale + old.get(e);
-    store8(row, col, a.dim, v);
-}
+/* Where the sum of the piece at place `start` goes, of a run with several.  The pieces of a run begin kPiece apart, and the
+ * next such run begins more than kPiece behind this one's beginning: of those that begin within one kPiece of
+ * places, one at most is a run's first and one at most is not. */
+__device__ __forceinline__ uint64_t slot_of(uint32_t start, bool first) { return 2 * (uint64_t)(start / kPiece) + first; }
 
-template <typename TG, typename TO, int L> __global__ __launch_bounds__(1024) void embedding_grad_kernel(const GradArgs a) {
+__global__ __launch_bounds__(1024) void embedding_sort_kernel(const GradArgs a) {
     extern __shared__ uint32_t counts[]; // kWaves x locals: first counts, then where the wave's next token of that id goes
-    __shared__ uint32_t starts[kLocalMost], lengths[kLocalMost], part[kWaves], before[kWaves], n_heavy;
+    __shared__ uint32_t starts[kLocalMost], lengths[kLocalMost], part[kWaves], before[kWaves];
     const uint32_t bucket = blockIdx.x, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, mask = (1u << a.shift) - 1;
-    if (bucket >= a.vocab) return;
     for (uint32_t i = threadIdx.x; i < kWaves * a.locals; i += 1024) counts[i] = 0;
-    if (threadIdx.x == 0) n_heavy = 0;
     __syncthreads();
 
     // count
@@ -126,10 +126,10 @@ template <typename TG, typename TO, int L> __global__ __launch_bounds__(1024) vo
 #pragma unroll 4
     for (uint32_t t = from + lane; t < to; t += kWave) {
         const int64_t id = a.ids[t];
-        if (!a.counts(id)) continue;
+        const bool use = a.counts(id);
         const uint32_t b = (uint32_t)id & mask;
-        if (b == bucket) atomicAdd(&mine[(uint32_t)id >> a.shift], 1u);
-        lower += b < bucket;
+        if (use && b == bucket) atomicAdd(&mine[(uint32_t)id >> a.shift], 1u);
+        lower += use && b < bucket;
     }
     for (int d = 1; d < 64; d *= 2) lower += __shfl_xor(lower, d);
     if (lane == 0) before[wave] = lower;
@@ -147,8 +147,10 @@ template <typename TG, typename TO, int L> __global__ __launch_bounds__(1024) vo
     }
     if (lane == 63) part[wave] = upto;
     __syncthreads();
-    uint32_t start = base + upto - total;
+    uint32_t start = base + upto - total, all_mine = 0;
     for (uint32_t w = 0; w < wave; ++w) start += part[w];
+    for (uint32_t w = 0; w < kWaves; ++w) all_mine += part[w];
+    if (bucket == gridDim.x - 1 && threadIdx.x == 0) *a.used = base + all_mine;
     if (threadIdx.x < a.locals) {
         starts[threadIdx.x] = start;
         lengths[threadIdx.x] = total;
@@ -161,7 +163,22 @@ template <typename TG, typename TO, int L> __global__ __launch_bounds__(1024) vo
     }
     __syncthreads();
 
-    // order: each wave for its share; of several tokens in one step, an id at a time
+    // rows without a token
+    if (!a.accumulate)
+        for (uint32_t local = threadIdx.x / a.lanes; local < a.locals; local += 1024 / a.lanes) {
+            const uint32_t id = local << a.shift | bucket;
+            if (id >= a.vocab || lengths[local]) continue;
+            char *row = (char *)a.out + id * a.out_stride * a.out_bytes;
+            const uint64_t bytes = (uint64_t)a.dim * a.out_bytes;
+            for (uint64_t at = threadIdx.x % a.lanes * 16ull; at < bytes; at += a.lanes * 16ull) {
+                if (at + 16 <= bytes) *(u32x4_at2 *)(row + at) = u32x4{0, 0, 0, 0};
+                else
+                    for (uint64_t b = at; b < bytes; b += 2) *(uint16_t *)(row + b) = 0;
+            }
+        }
+
+    // the list: each wave for its share; of several tokens in one step, an id at a time
+    if (all_mine == 0) return;
     for (uint32_t at = from; at < to; at += kWave) {
         const int64_t id = at + lane < to ? a.ids[at + lane] : -1;
         const bool own = a.counts(id) && ((uint32_t)id & mask) == bucket;
@@ -173,67 +190,86 @@ template <typename TG, typename TO, int L> __global__ __launch_bounds__(1024) vo
             uint32_t place = 0;
             if (lane == 0) place = atomicAdd(&mine[local], (uint32_t)__popcll(all));
             place = (uint32_t)__builtin_amdgcn_readfirstlane((int)place);
-            if (same) a.order[place + (uint32_t)__popcll(all & ((1ull << lane) - 1))] = at + lane;
+            if (same) {
+                place += (uint32_t)__popcll(all & ((1ull << lane) - 1));
+                a.sorted[place] = Place{at + lane, (uint32_t)id, place - starts[local], lengths[local]};
+            }
             left &= ~all;
         }
     }
-    __syncthreads();
+}
 
-    // rows: L lanes to each
-    const uint32_t sub = lane % L;
-    for (uint32_t local = threadIdx.x / L; local < a.locals; local += 1024 / L) {
-        const uint32_t id = local << a.shift | bucket, n = lengths[local], begin = starts[local];
-        if (id >= a.vocab || (n == 0 && a.accumulate)) continue;
-        if (n > kFew) {
-            if (sub == 0) a.heavy[base / (kFew + 1) + atomicAdd(&n_heavy, 1u)] = Heavy{id, begin, n, 0};
-            continue;
-        }
-        for (uint32_t col = sub * 8; col < a.dim; col += L * 8) {
-            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
-            for (uint32_t j = 0; j < n; ++j) {
-                Raw<TG> g;
-                load8(g, (const TG *)a.grad + a.order[begin + j] * a.grad_stride, col, a.dim);
+template <typename TO> __device__ __forceinline__ void finish8(const GradArgs &a, uint32_t id, uint32_t col, const float (&sum)[8]) {
+    TO *row = (TO *)a.out + id * a.out_stride;
+    Raw<TO> old;
+    if (a.accumulate) load8(old, row, col, a.dim);
+    else old.clear();
+    float v[8];
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) v[e] += g.get(e);
-            }
-            finish8<TO>(a, id, col, v);
+    for (uint32_t e = 0; e < 8; ++e) v[e] = sum[e] * a.scale + old.get(e);
+    store8(row, col, a.dim, v);
+}
+
+template <typename TG, typename TO, int L> __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const GradArgs a, const Place *__restrict__ sorted) {
+    const uint32_t used = *a.used;
+    uint32_t group = blockIdx.x * (kThreads / L) + threadIdx.x / L; // L lanes: a step of the list and a tile of columns
+    if (L == kWave) group = (uint32_t)__builtin_amdgcn_readfirstlane((int)group);
+    const uint32_t step = group / a.tiles, col = (group - step * a.tiles) * (L * 8) + threadIdx.x % L * 8;
+    const uint32_t begin = step * kStep;
+    if (begin >= used) return;
+    uint32_t end = begin + kStep < used ? begin + kStep : used;
+    // pieces that begin here: from the first one's beginning to the last one's end
+    const Place head = sorted[begin], tail = sorted[end - 1];
+    auto rest = [](const Place &p) { // from p to its piece's end
+        const uint32_t in = p.at % kPiece, left = p.run - p.at;
+        return kPiece - in < left ? kPiece - in : left;
+    };
+    const uint32_t first = head.at % kPiece ? begin + rest(head) : begin;
+    if (first >= end) return;
+    end = end - 1 + rest(tail);
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (uint32_t at = first; at < end; at += kAhead) {
+        Place p[kAhead];
+        Raw<TG> g[kAhead];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) p[k] = sorted[at + k < end ? at + k : end - 1];
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) load8(g[k], (const TG *)a.grad + p[k].token * a.grad_stride, col, a.dim);
+#pragma unroll
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            if (at + k >= end) break;
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) v[e] += g[k].get(e);
+            if (p[k].at % kPiece != kPiece - 1 && p[k].at + 1 != p[k].run) continue;
+            if (p[k].run <= kPiece) finish8<TO>(a, p[k].id, col, v);
+            else store8(a.partial + slot_of(at + k - p[k].at % kPiece, p[k].at < kPiece) * a.padded, col, a.padded, v);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) v[e] = 0.0f;
         }
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        a.heavy_first[bucket] = base / (kFew + 1);
-        a.heavy_count[bucket] = n_heavy;
     }
 }
 
-/* The rows with many tokens: 64 columns of one to a workgroup, eight lanes to a token's part of them. */
-constexpr uint32_t kHeavyThreads = 512;
-template <typename TG, typename TO> __global__ __launch_bounds__(kHeavyThreads) void embedding_grad_heavy_kernel(const GradArgs a, uint32_t buckets) {
-    __shared__ float sums[kHeavyThreads / 8][64];
-    const uint32_t group = threadIdx.x / 8, in = threadIdx.x % 8 * 8, col = blockIdx.x * 64 + in;
-    for (uint32_t bucket = blockIdx.y; bucket < buckets; bucket += gridDim.y)
-    for (uint32_t i = 0, n = a.heavy_count[bucket], first = a.heavy_first[bucket]; i < n; ++i) {
-        const Heavy h = a.heavy[first + i];
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 4
-        for (uint32_t j = group; j < h.count; j += kHeavyThreads / 8) {
-            Raw<TG> g;
-            load8(g, (const TG *)a.grad + a.order[h.start + j] * a.grad_stride, col, a.dim);
+/* Runs of several pieces: a wave looks for the one that begins in its kPiece places, and sums its pieces for 512 columns. */
+template <typename TO> __global__ __launch_bounds__(kThreads) void embedding_join_kernel(const GradArgs a, uint32_t tiles) {
+    static_assert(kPiece == kWave, "a lane to a place");
+    const uint32_t used = *a.used, group = blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    const uint32_t step = group / tiles, col = (group - step * tiles) * 512 + lane * 8, at = step * kPiece + lane;
+    Place p = {0, 0, 1, 0};
+    if (at < used) p = a.sorted[at];
+    const uint64_t found = __ballot(p.at == 0 && p.run > kPiece);
+    if (!found) return;
+    const int from = __builtin_ctzll(found);
+    const uint32_t run = (uint32_t)__builtin_amdgcn_readlane((int)p.run, from), id = (uint32_t)__builtin_amdgcn_readlane((int)p.id, from);
+    const uint32_t start = step * kPiece + from;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 8
+    for (uint32_t done = 0; done < run; done += kPiece) {
+        Raw<float> s;
+        load8(s, (const float *)a.partial + slot_of(start + done, done == 0) * a.padded, col, a.padded);
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) v[e] += g.get(e);
-        }
-        __syncthreads();
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) sums[group][in + e] = v[e];
-        __syncthreads();
-        if (threadIdx.x < 8) {
-            for (uint32_t p = 1; p < kHeavyThreads / 8; ++p)
-#pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) v[e] += sums[p][in + e];
-            finish8<TO>(a, h.id, col, v);
-        }
+        for (uint32_t e = 0; e < 8; ++e) v[e] += s.get(e);
     }
+    finish8<TO>(a, id, col, v);
 }
 
 uint32_t shift_of(uint64_t vocab) {
@@ -241,29 +277,27 @@ uint32_t shift_of(uint64_t vocab) {
     while (((vocab + (1ull << shift) - 1) >> shift) > kLocalMost) ++shift;
     return shift;
 }
+uint64_t padded_of(uint64_t dim) { return (dim + 7) / 8 * 8; }
 
-/* The workspace: order, heavy, heavy_first, heavy_count, each at a multiple of 16 bytes. */
-struct Workspace {
-    uint64_t heavy, first, count, bytes;
-    Workspace(uint64_t tokens, uint64_t vocab) {
-        heavy = (tokens * 4 + 15) / 16 * 16;
-        first = heavy + (tokens / (kFew + 1)) * sizeof(Heavy);
-        count = first + (4ull << shift_of(vocab));
-        bytes = count + (4ull << shift_of(vocab));
-    }
-};
+/* The workspace: the number of places, the places, the sums of pieces; 16 bytes and multiples of them. */
+constexpr uint64_t kHead = 16;
+uint64_t partial_at(uint64_t tokens) { return kHead + tokens * sizeof(Place); }
+uint64_t partial_bytes(uint64_t tokens, uint64_t dim) { return tokens > kPiece ? 2 * (tokens / kPiece + 1) * padded_of(dim) * sizeof(float) : 0; }
 
-template <typename TG, typename TO> void launch_grad(const GradArgs &a, hipStream_t s) {
-    const uint32_t buckets = 1u << a.shift, lds = kWaves * a.locals * 4;
-    const uint32_t grid = buckets < a.vocab ? buckets : a.vocab;
-#define ERI_EMB_GRAD(L) hipLaunchKernelGGL((embedding_grad_kernel<TG, TO, L>), dim3(grid), dim3(1024), lds, s, a)
-    if (a.dim <= 64) ERI_EMB_GRAD(8);
-    else if (a.dim <= 128) ERI_EMB_GRAD(16);
-    else if (a.dim <= 256) ERI_EMB_GRAD(32);
-    else ERI_EMB_GRAD(64);
-#undef ERI_EMB_GRAD
-    if (a.tokens > kFew)
-        hipLaunchKernelGGL((embedding_grad_heavy_kernel<TG, TO>), dim3((a.dim + 63) / 64, grid < 32768 ? grid : 32768), dim3(kHeavyThreads), 0, s, a, grid);
+template <typename TG, typename TO, int L> void launch_sum(GradArgs a, hipStream_t s) {
+    a.tiles = (a.dim + L * 8 - 1) / (L * 8);
+    const uint64_t groups = (uint64_t)((a.tokens + kStep - 1) / kStep) * a.tiles;
+    hipLaunchKernelGGL((embedding_sum_kernel<TG, TO, L>), dim3((uint32_t)((groups + kThreads / L - 1) / (kThreads / L))), dim3(kThreads), 0, s, a, a.sorted);
+}
+template <typename TG, typename TO> void launch_sums(const GradArgs &a, hipStream_t s) {
+    if (a.dim <= 64) launch_sum<TG, TO, 8>(a, s);
+    else if (a.dim <= 128) launch_sum<TG, TO, 16>(a, s);
+    else if (a.dim <= 256) launch_sum<TG, TO, 32>(a, s);
+    else launch_sum<TG, TO, 64>(a, s);
+    if (a.tokens <= kPiece) return;
+    const uint32_t tiles = (a.dim + 511) / 512;
+    const uint64_t groups = (uint64_t)((a.tokens + kPiece - 1) / kPiece) * tiles;
+    hipLaunchKernelGGL(embedding_join_kernel<TO>, dim3((uint32_t)((groups + 3) / 4)), dim3(kThreads), 0, s, a, tiles);
 }
 
 } // namespace
@@ -277,19 +311,23 @@ int launch_embedding(const EriEmbedding &e, uint32_t compute_units, void *stream
     return (int)hipGetLastError();
 }
 
-uint64_t embedding_grad_workspace(uint64_t tokens, uint64_t vocab, uint64_t) { return Workspace(tokens, vocab).bytes; }
+uint64_t embedding_grad_workspace(uint64_t tokens, uint64_t, uint64_t dim) { return partial_at(tokens) + partial_bytes(tokens, dim); }
 
 int launch_embedding_grad(const EriEmbeddingGrad &e, uint32_t, void *stream) {
-    const Workspace w(e.tokens, e.vocab);
     char *ws = static_cast<char *>(e.workspace);
-    GradArgs a = {{e.ids, (uint32_t)e.ids_64}, e.grad, e.out, (uint32_t *)ws, (Heavy *)(ws + w.heavy), (uint32_t *)(ws + w.first),
-                  (uint32_t *)(ws + w.count), (uint32_t)e.tokens, (uint32_t)e.vocab, (uint32_t)e.dim, shift_of(e.vocab), 0,
-                  e.grad_stride, e.out_stride, e.padding_id, e.scale, (uint32_t)(e.accumulate != 0)};
-    a.locals = (a.vocab + (1u << a.shift) - 1) >> a.shift;
+    GradArgs a = {{e.ids, (uint32_t)e.ids_64}, e.grad, e.out, (Place *)(ws + kHead), (uint32_t *)ws, (float *)(ws + partial_at(e.tokens)),
+                  (uint32_t)e.tokens, (uint32_t)e.vocab, (uint32_t)e.dim, shift_of(e.vocab), 0, (uint32_t)padded_of(e.dim), 0,
+                  e.grad_stride, e.out_stride, e.padding_id, e.scale, (uint32_t)(e.accumulate != 0), e.out_dtype == ERI_DTYPE_F32 ? 4u : 2u, 1};
+    const uint32_t buckets = 1u << a.shift;
+    a.locals = (a.vocab + buckets - 1) >> a.shift;
+    while (a.lanes < kWave && a.lanes * 16ull < (uint64_t)a.dim * a.out_bytes) a.lanes *= 2;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(embedding_sort_kernel, dim3(buckets < a.vocab ? buckets : a.vocab), dim3(1024), kWaves * a.locals * 4, s, a);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess || a.tokens == 0) return (int)err;
     const bool g32 = e.grad_dtype == ERI_DTYPE_F32, o32 = e.out_dtype == ERI_DTYPE_F32;
-    if (g32) o32 ? launch_grad<float, float>(a, s) : launch_grad<float, bf16>(a, s);
-    else o32 ? launch_grad<bf16, float>(a, s) : launch_grad<bf16, bf16>(a, s);
+    if (g32) o32 ? launch_sums<float, float>(a, s) : launch_sums<float, bf16>(a, s);
+    else o32 ? launch_sums<bf16, float>(a, s) : launch_sums<bf16, bf16>(a, s);
     return (int)hipGetLastError();
 }
 
