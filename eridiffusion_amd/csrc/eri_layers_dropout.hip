@@ -17,21 +17,21 @@ struct DropoutArgs {
     Drop drop;
 };
 
-template <typename T> __global__ __launch_bounds__(kThreads) void dropout_kernel(const DropoutArgs a) {
+template <typename T, bool SHORT> __global__ __launch_bounds__(kThreads) void dropout_kernel(const DropoutArgs a) {
     const uint64_t offset = drop_offset(a.drop);
     for (uint32_t row = blockIdx.y; row < a.rows; row += gridDim.y) {
         const T *x = (const T *)a.x + row * a.x_stride;
         T *y = (T *)a.y + row * a.y_stride;
         for (uint64_t v = (uint64_t)blockIdx.x * kThreads + threadIdx.x; v < a.vectors; v += (uint64_t)gridDim.x * kThreads) {
-            const uint64_t col = v * 8, left = a.cols - col;
-            const uint32_t n = left < 8 ? (uint32_t)left : 8u;
+            const uint64_t col = v * 8;
             Raw<T> r;
-            load8(r, x + col, 0, n);
+            load8<SHORT>(r, x, col, a.cols);
             const u32x4 bits = draw8(row * a.cols + col, a.drop, offset);
+            settle8<SHORT>(r, col, a.cols);
             float out[8];
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) out[e] = dropped(r.get(e), bits, e, a.drop);
-            store8(y + col, 0, n, out);
+            store8(y, col, a.cols, out);
         }
     }
 }
@@ -48,8 +48,10 @@ int launch_dropout(const EriDropout &e, const Drop &d, uint32_t compute_units, v
     const uint64_t x = (a.vectors + kThreads - 1) / kThreads, most = (uint64_t)compute_units * 64;
     const dim3 grid((uint32_t)(x < most ? x : most), a.rows < 65535 ? a.rows : 65535);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (e.dtype_tag == ERI_DTYPE_F32) hipLaunchKernelGGL(dropout_kernel<float>, grid, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL(dropout_kernel<bf16>, grid, dim3(kThreads), 0, s, a);
+    const bool f32 = e.dtype_tag == ERI_DTYPE_F32, is_short = a.cols < 8;
+    void (*const kernel)(const DropoutArgs) = f32 ? is_short ? dropout_kernel<float, true> : dropout_kernel<float, false>
+                                                  : is_short ? dropout_kernel<bf16, true> : dropout_kernel<bf16, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);
     return (int)hipGetLastError();
 }
 

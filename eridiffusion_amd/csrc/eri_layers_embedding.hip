@@ -24,42 +24,43 @@ struct LookupArgs {
 };
 
 /* L lanes to a row, U rows at a time in each thread's registers. */
-template <typename T, int L, int U> __global__ __launch_bounds__(kThreads) void embedding_kernel(const LookupArgs a) {
+template <typename T, int L, int U, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_kernel(const LookupArgs a) {
     constexpr uint32_t kRows = kThreads / L;
     const uint32_t first = blockIdx.x * kRows * U + threadIdx.x / L, lane = threadIdx.x % L;
     const T *row[U];
+    bool real[U]; // the table's first row stands in for ids outside it
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t t = first + u * kRows;
         const int64_t id = t < a.tokens ? a.ids[t] : -1;
-        row[u] = (uint64_t)id < a.vocab ? (const T *)a.table + id * a.table_stride : nullptr;
+        real[u] = (uint64_t)id < a.vocab;
+        row[u] = (const T *)a.table + (real[u] ? id * a.table_stride : 0);
     }
     for (uint32_t col = lane * 8; col < a.dim; col += L * 8) {
         Raw<T> r[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (row[u]) load8(r[u], row[u], col, a.dim);
-            else r[u].clear();
-        }
+        for (int u = 0; u < U; ++u) load8<SHORT>(r[u], row[u], col, a.dim);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t t = first + u * kRows;
+            settle8<SHORT>(r[u], col, a.dim);
             float v[8];
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) v[e] = row[u] ? r[u].get(e) * a.scale : 0.0f;
+            for (uint32_t e = 0; e < 8; ++e) v[e] = real[u] ? r[u].get(e) * a.scale : 0.0f;
             if (t < a.tokens) store8((T *)a.out + t * a.out_stride, col, a.dim, v);
         }
     }
 }
 
-template <typename T, int L> void launch_lookup(const LookupArgs &a, uint32_t compute_units, hipStream_t s) {
+template <typename T, int L, bool SHORT = false> void launch_lookup(const LookupArgs &a, uint32_t compute_units, hipStream_t s) {
     constexpr uint32_t kRows = kThreads / L;
-    if (a.tokens / (kRows * 4) >= compute_units * 4) // four rows a thread where that still fills the chip
-        hipLaunchKernelGGL((embedding_kernel<T, L, 4>), dim3((a.tokens + kRows * 4 - 1) / (kRows * 4)), dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((embedding_kernel<T, L, 1>), dim3((a.tokens + kRows - 1) / kRows), dim3(kThreads), 0, s, a);
+    if (!SHORT && a.tokens / (kRows * 4) >= compute_units * 4) // four rows a thread where that still fills the chip
+        hipLaunchKernelGGL((embedding_kernel<T, L, 4, false>), dim3((a.tokens + kRows * 4 - 1) / (kRows * 4)), dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((embedding_kernel<T, L, 1, SHORT>), dim3((a.tokens + kRows - 1) / kRows), dim3(kThreads), 0, s, a);
 }
 template <typename T> void launch_lookup_of(const LookupArgs &a, uint32_t compute_units, hipStream_t s) {
-    if (a.dim <= 64) launch_lookup<T, 8>(a, compute_units, s);
+    if (a.dim < 8) launch_lookup<T, 8, true>(a, compute_units, s);
+    else if (a.dim <= 64) launch_lookup<T, 8>(a, compute_units, s);
     else if (a.dim <= 256) launch_lookup<T, 32>(a, compute_units, s);
     else if (a.dim <= 1024) launch_lookup<T, 128>(a, compute_units, s);
     else launch_lookup<T, 256>(a, compute_units, s);
@@ -83,9 +84,8 @@ template <typename T> void launch_lookup_of(const LookupArgs &a, uint32_t comput
  */
 constexpr uint32_t kWaves = 16;       // of a bucket's workgroup
 constexpr uint32_t kLocalMost = 1024; // ids of a bucket
-constexpr uint32_t kPiece = 64;
+constexpr uint32_t kPiece = 32;
 constexpr uint32_t kStep = 16;
-constexpr uint32_t kAhead = 8;        // rows whose loads are under way together
 
 struct Place { // of the sorted list
     uint32_t token, id;
@@ -199,63 +199,111 @@ __global__ __launch_bounds__(1024) void embedding_sort_kernel(const GradArgs a) 
     }
 }
 
-template <typename TO> __device__ __forceinline__ void finish8(const GradArgs &a, uint32_t id, uint32_t col, const float (&sum)[8]) {
+template <bool SHORT, typename TO> __device__ __forceinline__ void finish8(const GradArgs &a, uint32_t id, uint32_t col, const float (&sum)[8]) {
     TO *row = (TO *)a.out + id * a.out_stride;
     Raw<TO> old;
-    if (a.accumulate) load8(old, row, col, a.dim);
-    else old.clear();
+    if (a.accumulate) {
+        load8<SHORT>(old, row, col, a.dim);
+        settle8<SHORT>(old, col, a.dim);
+    } else old.clear();
     float v[8];
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) v[e] = sum[e] * a.scale + old.get(e);
     store8(row, col, a.dim, v);
 }
 
-template <typename TG, typename TO, int L> __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const GradArgs a, const Place *__restrict__ sorted) {
+/* L lanes to a step of the list and a tile of L*8 columns.  The places of the step and of what its last piece reaches beyond it
+ * come in one trip to memory, then the rows, a set of them on its way while another is added up. */
+template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const GradArgs a) {
+    static_assert(kStep + kPiece <= kWave, "a lane to a place");
+    __shared__ Place list[L == kWave ? 1 : kThreads / L][kStep + kPiece];
+    uint32_t team = threadIdx.x / L;
+    if (L == kWave) team = (uint32_t)__builtin_amdgcn_readfirstlane((int)team);
+    const uint32_t group = blockIdx.x * (kThreads / L) + team, lane = threadIdx.x % L;
+    const uint32_t step = group / a.tiles, col = (group - step * a.tiles) * (L * 8) + lane * 8, begin = step * kStep;
+    Place held = {0, 0, 0, 0}; // of a whole wave each lane keeps a place
+    if (L == kWave) {
+        if (lane < kStep + kPiece && begin + lane < a.tokens) held = a.sorted[begin + lane];
+    } else
+        for (uint32_t i = lane; i < kStep + kPiece; i += L)
+            if (begin + i < a.tokens) list[team][i] = a.sorted[begin + i];
     const uint32_t used = *a.used;
-    uint32_t group = blockIdx.x * (kThreads / L) + threadIdx.x / L; // L lanes: a step of the list and a tile of columns
-    if (L == kWave) group = (uint32_t)__builtin_amdgcn_readfirstlane((int)group);
-    const uint32_t step = group / a.tiles, col = (group - step * a.tiles) * (L * 8) + threadIdx.x % L * 8;
-    const uint32_t begin = step * kStep;
+    __syncthreads();
     if (begin >= used) return;
-    uint32_t end = begin + kStep < used ? begin + kStep : used;
-    // pieces that begin here: from the first one's beginning to the last one's end
-    const Place head = sorted[begin], tail = sorted[end - 1];
+    // pieces that begin here: from the first one's beginning to the last one's end, counted from `begin`
+    const uint32_t here = used - begin < kStep ? used - begin : kStep;
+    auto place = [&](uint32_t i) {
+        if (L != kWave) return list[team][i];
+        auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
+        return Place{of(held.token), of(held.id), of(held.at), of(held.run)};
+    };
     auto rest = [](const Place &p) { // from p to its piece's end
         const uint32_t in = p.at % kPiece, left = p.run - p.at;
         return kPiece - in < left ? kPiece - in : left;
     };
-    const uint32_t first = head.at % kPiece ? begin + rest(head) : begin;
-    if (first >= end) return;
-    end = end - 1 + rest(tail);
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    for (uint32_t at = first; at < end; at += kAhead) {
-        Place p[kAhead];
-        Raw<TG> g[kAhead];
+    const Place head = place(0);
+    const uint32_t first = head.at % kPiece ? rest(head) : 0;
+    if (first >= here) return;
+    const uint32_t end = here - 1 + rest(place(here - 1));
+    auto ends = [](const Place &p) { return p.at % kPiece == kPiece - 1 || p.at + 1 == p.run; };
+    // Rows on their way: as many as the registers of two such sets hold.  No load of a set hangs on a condition (the last row stands
+    // in for those past the end): with a known number under way, a wait for the first of them leaves the others alone.
+    constexpr uint32_t kAhead = sizeof(TG) + (ACC ? sizeof(TO) : 0) <= 4 ? 8 : 4;
+    struct Ahead {
+        Raw<TG> grad[kAhead];
+        Raw<TO> old[ACC ? kAhead : 1];
+    };
+    auto fetch = [&](Ahead &f, uint32_t at) {
 #pragma unroll
-        for (uint32_t k = 0; k < kAhead; ++k) p[k] = sorted[at + k < end ? at + k : end - 1];
-#pragma unroll
-        for (uint32_t k = 0; k < kAhead; ++k) load8(g[k], (const TG *)a.grad + p[k].token * a.grad_stride, col, a.dim);
+        for (uint32_t k = 0; k < kAhead; ++k) {
+            const Place p = place(at + k < end ? at + k : end - 1);
+            load8<SHORT>(f.grad[k], (const TG *)a.grad + p.token * a.grad_stride, col, a.dim);
+            if (ACC) load8<SHORT>(f.old[k], (const TO *)a.out + p.id * a.out_stride, col, a.dim);
+        }
+    };
+    // Sums are shifted into place at their end where a row ends inside the vector: adding up commutes with it.
+    Raw<float> v;
+    v.clear();
+    auto add = [&](Ahead &f, uint32_t at) {
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; ++k) {
             if (at + k >= end) break;
+            const Place p = place(at + k);
+            float sum[8];
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) v[e] += g[k].get(e);
-            if (p[k].at % kPiece != kPiece - 1 && p[k].at + 1 != p[k].run) continue;
-            if (p[k].run <= kPiece) finish8<TO>(a, p[k].id, col, v);
-            else store8(a.partial + slot_of(at + k - p[k].at % kPiece, p[k].at < kPiece) * a.padded, col, a.padded, v);
+            for (uint32_t e = 0; e < 8; ++e) {
+                sum[e] = v.get(e) + f.grad[k].get(e);
+                v.set(e, sum[e]);
+            }
+            if (!ends(p)) continue;
+            const bool whole = p.run <= kPiece;
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) v[e] = 0.0f;
+            for (uint32_t e = 0; e < 8; ++e) v.set(e, whole ? sum[e] * a.scale + (ACC ? f.old[k].get(e) : 0.0f) : sum[e]);
+            settle8<SHORT>(v, col, a.dim);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) sum[e] = v.get(e);
+            if (whole) store8((TO *)a.out + p.id * a.out_stride, col, a.dim, sum);
+            else store8(a.partial + slot_of(begin + at + k - p.at % kPiece, p.at < kPiece) * a.padded, col, a.padded, sum);
+            v.clear();
         }
+    };
+    Ahead one, two;
+    fetch(one, first);
+    for (uint32_t at = first; at < end; at += 2 * kAhead) {
+        fetch(two, at + kAhead);
+        add(one, at);
+        fetch(one, at + 2 * kAhead);
+        add(two, at + kAhead);
     }
 }
 
 /* Runs of several pieces: a wave looks for the one that begins in its kPiece places, and sums its pieces for 512 columns. */
-template <typename TO> __global__ __launch_bounds__(kThreads) void embedding_join_kernel(const GradArgs a, uint32_t tiles) {
-    static_assert(kPiece == kWave, "a lane to a place");
+template <typename TO, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_join_kernel(const GradArgs a) {
+    static_assert(kPiece <= kWave, "a lane to a place");
     const uint32_t used = *a.used, group = blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const uint32_t step = group / tiles, col = (group - step * tiles) * 512 + lane * 8, at = step * kPiece + lane;
+    const uint32_t step = group / a.tiles, col = (group - step * a.tiles) * 512 + lane * 8, at = step * kPiece + lane;
     Place p = {0, 0, 1, 0};
-    if (at < used) p = a.sorted[at];
+    if (lane < kPiece && at < used) p = a.sorted[at];
     const uint64_t found = __ballot(p.at == 0 && p.run > kPiece);
     if (!found) return;
     const int from = __builtin_ctzll(found);
@@ -265,11 +313,12 @@ template <typename TO> __global__ __launch_bounds__(kThreads) void embedding_joi
 #pragma unroll 8
     for (uint32_t done = 0; done < run; done += kPiece) {
         Raw<float> s;
-        load8(s, (const float *)a.partial + slot_of(start + done, done == 0) * a.padded, col, a.padded);
+        load8<false>(s, (const float *)a.partial + slot_of(start + done, done == 0) * a.padded, col, a.padded);
+        settle8<false>(s, col, a.padded);
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) v[e] += s.get(e);
     }
-    finish8<TO>(a, id, col, v);
+    finish8<SHORT, TO>(a, id, col, v);
 }
 
 uint32_t shift_of(uint64_t vocab) {
@@ -284,20 +333,23 @@ constexpr uint64_t kHead = 16;
 uint64_t partial_at(uint64_t tokens) { return kHead + tokens * sizeof(Place); }
 uint64_t partial_bytes(uint64_t tokens, uint64_t dim) { return tokens > kPiece ? 2 * (tokens / kPiece + 1) * padded_of(dim) * sizeof(float) : 0; }
 
-template <typename TG, typename TO, int L> void launch_sum(GradArgs a, hipStream_t s) {
+template <typename TG, typename TO, int L, bool SHORT = false> void launch_sum(GradArgs a, hipStream_t s) {
     a.tiles = (a.dim + L * 8 - 1) / (L * 8);
-    const uint64_t groups = (uint64_t)((a.tokens + kStep - 1) / kStep) * a.tiles;
-    hipLaunchKernelGGL((embedding_sum_kernel<TG, TO, L>), dim3((uint32_t)((groups + kThreads / L - 1) / (kThreads / L))), dim3(kThreads), 0, s, a, a.sorted);
+    uint64_t groups = (uint64_t)((a.tokens + kStep - 1) / kStep) * a.tiles;
+    const dim3 grid((uint32_t)((groups + kThreads / L - 1) / (kThreads / L)));
+    if (a.accumulate) hipLaunchKernelGGL((embedding_sum_kernel<TG, TO, L, true, SHORT>), grid, dim3(kThreads), 0, s, a);
+    else hipLaunchKernelGGL((embedding_sum_kernel<TG, TO, L, false, SHORT>), grid, dim3(kThreads), 0, s, a);
+    if (a.tokens <= kPiece) return;
+    a.tiles = (a.dim + 511) / 512;
+    groups = (uint64_t)((a.tokens + kPiece - 1) / kPiece) * a.tiles;
+    hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT>), dim3((uint32_t)((groups + 3) / 4)), dim3(kThreads), 0, s, a);
 }
 template <typename TG, typename TO> void launch_sums(const GradArgs &a, hipStream_t s) {
-    if (a.dim <= 64) launch_sum<TG, TO, 8>(a, s);
+    if (a.dim < 8) launch_sum<TG, TO, 8, true>(a, s);
+    else if (a.dim <= 64) launch_sum<TG, TO, 8>(a, s);
     else if (a.dim <= 128) launch_sum<TG, TO, 16>(a, s);
     else if (a.dim <= 256) launch_sum<TG, TO, 32>(a, s);
     else launch_sum<TG, TO, 64>(a, s);
-    if (a.tokens <= kPiece) return;
-    const uint32_t tiles = (a.dim + 511) / 512;
-    const uint64_t groups = (uint64_t)((a.tokens + kPiece - 1) / kPiece) * tiles;
-    hipLaunchKernelGGL(embedding_join_kernel<TO>, dim3((uint32_t)((groups + 3) / 4)), dim3(kThreads), 0, s, a, tiles);
 }
 
 } // namespace

@@ -27,18 +27,32 @@ __device__ __forceinline__ void store8_f8(uint8_t *row, uint32_t col, uint32_t c
         int p = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k], v[4 * k + 1], 0, false);
         w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * k + 2], v[4 * k + 3], p, true);
     }
-    if (col + 8 <= cols) *(u32x2_at1 *)(row + col) = u32x2{w[0], w[1]};
-    else
-#pragma unroll
-        for (uint32_t e = 0; e < 7; ++e)
-            if (col + e < cols) row[col + e] = (uint8_t)(w[e / 4] >> (8 * (e & 3)));
+    if (col >= cols) return;
+    row += col;
+    const uint32_t n = cols - col;
+    if (n >= 8) {
+        *(u32x2_at1 *)row = u32x2{w[0], w[1]};
+        return;
+    }
+    if (n & 4) {
+        *(u32_at1 *)row = w[0];
+        row += 4, w[0] = w[1];
+    }
+    if (n & 2) {
+        *(u16_at1 *)row = (uint16_t)w[0];
+        row += 2, w[0] >>= 16;
+    }
+    if (n & 1) *row = (uint8_t)w[0];
 }
 
 /* h of elements col .. col+7 of a row, zero past its end. */
-template <typename TX, typename TR, bool RES, bool DROP>
-__device__ __forceinline__ void sum8(float (&h)[8], const Raw<TX> &x, const Raw<TR> &r, uint64_t first, const Drop &d, uint64_t offset) {
+template <bool SHORT, typename TX, typename TR, bool RES, bool DROP>
+__device__ __forceinline__ void sum8(float (&h)[8], Raw<TX> &x, Raw<TR> &r, uint32_t row, uint32_t col, uint32_t cols, const Drop &d, uint64_t offset) {
+    const uint64_t first = (uint64_t)row * cols + col;
     u32x4 bits = {0, 0, 0, 0};
     if (DROP) bits = draw8(first, d, offset);
+    settle8<SHORT>(x, col, cols);
+    if (RES) settle8<SHORT>(r, col, cols);
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) {
         h[e] = x.get(e);
@@ -52,9 +66,9 @@ template <typename TX, typename TR, bool RES> __device__ __forceinline__ void st
     else store8((TX *)a.h + row * a.h_stride, col, a.cols, h);
 }
 
-__device__ __forceinline__ void weigh(float (&v)[8], const NormArgs &a, uint32_t col, float rstd) {
+template <bool SHORT> __device__ __forceinline__ void weigh(float (&v)[8], const NormArgs &a, uint32_t col, float rstd) {
     float w[8];
-    if (a.weight) load8_of(w, a.weight, a.weight_f32, col, a.cols);
+    if (a.weight) load8_of<SHORT>(w, a.weight, a.weight_f32, col, a.cols);
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) v[e] = a.weight ? v[e] * rstd * w[e] : v[e] * rstd;
 }
@@ -76,7 +90,7 @@ __device__ __forceinline__ float most_of(const float (&v)[8]) {
 }
 
 /* A row to TPR threads, NV vectors of eight elements in the registers of each. */
-template <typename TX, typename TR, bool RES, bool DROP, int TPR, int NV>
+template <typename TX, typename TR, bool RES, bool DROP, int TPR, int NV, bool SHORT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const NormArgs a) {
     constexpr int kWaves = TPR / kWave;
     __shared__ float slots[2][kWaves < 2 ? 1 : kWaves];
@@ -86,15 +100,15 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
     Raw<TX> x[NV];
     Raw<TR> r[NV];
 #pragma unroll
-    for (int k = 0; k < NV; ++k) load8(x[k], (const TX *)a.x + row * a.x_stride, (k * TPR + t) * 8, a.cols);
+    for (int k = 0; k < NV; ++k) load8<SHORT>(x[k], (const TX *)a.x + row * a.x_stride, (k * TPR + t) * 8, a.cols);
     if (RES)
 #pragma unroll
-        for (int k = 0; k < NV; ++k) load8(r[k], (const TR *)a.residual + row * a.residual_stride, (k * TPR + t) * 8, a.cols);
+        for (int k = 0; k < NV; ++k) load8<SHORT>(r[k], (const TR *)a.residual + row * a.residual_stride, (k * TPR + t) * 8, a.cols);
     float h[NV][8], sum = 0.0f;
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const uint32_t col = (k * TPR + t) * 8;
-        sum8<TX, TR, RES, DROP>(h[k], x[k], r[k], (uint64_t)row * a.cols + col, a.drop, offset);
+        sum8<SHORT, TX, TR, RES, DROP>(h[k], x[k], r[k], row, col, a.cols, a.drop, offset);
         if (a.h) store_h<TX, TR, RES>(a, row, col, h[k]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(h[k][e], h[k][e], sum);
@@ -105,7 +119,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
         const uint32_t col = (k * TPR + t) * 8;
-        weigh(h[k], a, col, rstd);
+        weigh<SHORT>(h[k], a, col, rstd);
         if (a.y_dtype == ERI_DTYPE_BF16) store8((bf16 *)a.y + row * a.y_stride, col, a.cols, h[k]);
         else if (a.y_dtype == ERI_DTYPE_F32) store8((float *)a.y + row * a.y_stride, col, a.cols, h[k]);
         else if (a.group) {
@@ -131,9 +145,9 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
     auto value = [&](float (&h)[8], uint32_t col) {
         Raw<TX> x;
         Raw<TR> r;
-        load8(x, (const TX *)a.x + row * a.x_stride, col, a.cols);
-        if (RES) load8(r, (const TR *)a.residual + row * a.residual_stride, col, a.cols);
-        sum8<TX, TR, RES, DROP>(h, x, r, (uint64_t)row * a.cols + col, a.drop, offset);
+        load8<false>(x, (const TX *)a.x + row * a.x_stride, col, a.cols);
+        if (RES) load8<false>(r, (const TR *)a.residual + row * a.residual_stride, col, a.cols);
+        sum8<false, TX, TR, RES, DROP>(h, x, r, row, col, a.cols, a.drop, offset);
     };
     float sum = 0.0f;
     for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
@@ -148,7 +162,7 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
         for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
             float h[8];
             value(h, col);
-            weigh(h, a, col, rstd);
+            weigh<false>(h, a, col, rstd);
             most = fmaxf(most, most_of(h));
         }
         most = group_max<16>(most, slots[1]);
@@ -161,7 +175,7 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
         float h[8];
         value(h, col);
         if (a.h) store_h<TX, TR, RES>(a, row, col, h);
-        weigh(h, a, col, rstd);
+        weigh<false>(h, a, col, rstd);
         if (a.y_dtype == ERI_DTYPE_BF16) store8((bf16 *)a.y + row * a.y_stride, col, a.cols, h);
         else if (a.y_dtype == ERI_DTYPE_F32) store8((float *)a.y + row * a.y_stride, col, a.cols, h);
         else if (a.group) {
@@ -173,15 +187,16 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
 }
 
 template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormArgs &a, uint32_t compute_units, hipStream_t s) {
-#define ERI_NORM(TPR, NV) \
-    hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV>), dim3((a.rows + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
-    if (a.cols <= 512) ERI_NORM(64, 1);
-    else if (a.cols <= 1024) ERI_NORM(64, 2);
-    else if (a.cols <= 2048) ERI_NORM(64, 4);
-    else if (a.cols <= 4096) ERI_NORM(256, 2);
-    else if (a.cols <= 8192) ERI_NORM(256, 4);
-    else if (a.cols <= 16384) ERI_NORM(1024, 2);
-    else if (a.cols <= 32768) ERI_NORM(1024, 4);
+#define ERI_NORM(TPR, NV, SHORT) \
+    hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV, SHORT>), dim3((a.rows + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+    if (a.cols < 8) ERI_NORM(64, 1, true);
+    else if (a.cols <= 512) ERI_NORM(64, 1, false);
+    else if (a.cols <= 1024) ERI_NORM(64, 2, false);
+    else if (a.cols <= 2048) ERI_NORM(64, 4, false);
+    else if (a.cols <= 4096) ERI_NORM(256, 2, false);
+    else if (a.cols <= 8192) ERI_NORM(256, 4, false);
+    else if (a.cols <= 16384) ERI_NORM(1024, 2, false);
+    else if (a.cols <= 32768) ERI_NORM(1024, 4, false);
     else hipLaunchKernelGGL((rms_norm_long_kernel<TX, TR, RES, DROP>), dim3(a.rows), dim3(1024), 0, s, a);
 #undef ERI_NORM
 }

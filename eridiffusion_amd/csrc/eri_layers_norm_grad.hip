@@ -33,7 +33,7 @@ __device__ __forceinline__ void store_grads(const NormGradArgs &a, uint32_t row,
 }
 
 /* A row at a time to TPR threads, which keep the weight and their columns' sums of grad_weight in registers. */
-template <typename TG, typename TR, bool DROP, int TPR, int NV>
+template <typename TG, typename TR, bool DROP, int TPR, int NV, bool SHORT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(const NormGradArgs a) {
     constexpr int kWaves = TPR / kWave;
     __shared__ float slots[2][kWaves < 2 ? 1 : kWaves];
@@ -43,7 +43,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(co
     float w[NV][8], acc[NV][8];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
-        if (a.weight) load8_of(w[k], a.weight, a.weight_f32, (k * TPR + t) * 8, a.cols);
+        if (a.weight) load8_of<SHORT>(w[k], a.weight, a.weight_f32, (k * TPR + t) * 8, a.cols);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             acc[k][e] = 0.0f;
@@ -56,25 +56,29 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(co
         Raw<TR> h[NV], r[NV];
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            load8(g[k], (const TG *)a.grad + row * a.grad_stride, (k * TPR + t) * 8, a.cols);
-            load8(h[k], (const TR *)a.h + row * a.h_stride, (k * TPR + t) * 8, a.cols);
+            load8<SHORT>(g[k], (const TG *)a.grad + row * a.grad_stride, (k * TPR + t) * 8, a.cols);
+            load8<SHORT>(h[k], (const TR *)a.h + row * a.h_stride, (k * TPR + t) * 8, a.cols);
         }
         if (a.grad_h)
 #pragma unroll
-            for (int k = 0; k < NV; ++k) load8(r[k], (const TR *)a.grad_h + row * a.grad_h_stride, (k * TPR + t) * 8, a.cols);
+            for (int k = 0; k < NV; ++k) load8<SHORT>(r[k], (const TR *)a.grad_h + row * a.grad_h_stride, (k * TPR + t) * 8, a.cols);
         else
 #pragma unroll
             for (int k = 0; k < NV; ++k) r[k].clear();
         const float rstd = a.rstd[row];
         float c = 0.0f;
 #pragma unroll
-        for (int k = 0; k < NV; ++k)
+        for (int k = 0; k < NV; ++k) {
+            settle8<SHORT>(g[k], (k * TPR + t) * 8, a.cols);
+            settle8<SHORT>(h[k], (k * TPR + t) * 8, a.cols);
+            settle8<SHORT>(r[k], (k * TPR + t) * 8, a.cols);
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) {
                 const float gh = g[k].get(e) * h[k].get(e);
                 c = fmaf(gh, w[k][e], c);
                 acc[k][e] = fmaf(gh, rstd, acc[k][e]);
             }
+        }
         c = group_sum<kWaves>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
@@ -117,9 +121,11 @@ template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024
             Raw<TG> g;
             Raw<TR> h;
             float w[8], gh[8];
-            load8(g, (const TG *)a.grad + row * a.grad_stride, col, a.cols);
-            load8(h, (const TR *)a.h + row * a.h_stride, col, a.cols);
-            if (a.weight) load8_of(w, a.weight, a.weight_f32, col, a.cols);
+            load8<false>(g, (const TG *)a.grad + row * a.grad_stride, col, a.cols);
+            load8<false>(h, (const TR *)a.h + row * a.h_stride, col, a.cols);
+            if (a.weight) load8_of<false>(w, a.weight, a.weight_f32, col, a.cols);
+            settle8<false>(g, col, a.cols);
+            settle8<false>(h, col, a.cols);
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) {
                 gh[e] = g.get(e) * h.get(e);
@@ -127,7 +133,7 @@ template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024
             }
             if (out) {
                 float old[8];
-                load8_of(old, out, true, col, a.padded);
+                load8_of<false>(old, out, true, col, a.padded);
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) old[e] = row == blockIdx.x ? gh[e] * rstd : fmaf(gh[e], rstd, old[e]);
                 store8(out, col, a.padded, old);
@@ -138,11 +144,14 @@ template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024
             Raw<TG> g;
             Raw<TR> h, r;
             float w[8], dh[8];
-            load8(g, (const TG *)a.grad + row * a.grad_stride, col, a.cols);
-            load8(h, (const TR *)a.h + row * a.h_stride, col, a.cols);
-            if (a.grad_h) load8(r, (const TR *)a.grad_h + row * a.grad_h_stride, col, a.cols);
+            load8<false>(g, (const TG *)a.grad + row * a.grad_stride, col, a.cols);
+            load8<false>(h, (const TR *)a.h + row * a.h_stride, col, a.cols);
+            if (a.grad_h) load8<false>(r, (const TR *)a.grad_h + row * a.grad_h_stride, col, a.cols);
             else r.clear();
-            if (a.weight) load8_of(w, a.weight, a.weight_f32, col, a.cols);
+            if (a.weight) load8_of<false>(w, a.weight, a.weight_f32, col, a.cols);
+            settle8<false>(g, col, a.cols);
+            settle8<false>(h, col, a.cols);
+            settle8<false>(r, col, a.cols);
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) dh[e] = fmaf(a.weight ? g.get(e) * w[e] : g.get(e), rstd, fmaf(-h.get(e), c, r.get(e)));
             store_grads<TR, DROP>(a, row, col, dh, offset);
@@ -168,7 +177,7 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_weight_kernel(const float 
     float total = 0.0f;
     for (uint32_t p = 0; p < 64; ++p) total += sums[p][threadIdx.x];
     if (out_f32) ((float *)out)[c] = total;
-    else store_one((bf16 *)out + c, total);
+    else ((bf16 *)out)[c].bits = (uint16_t)bf16_pair(total, 0.0f);
 }
 
 /* Threads to a row, and how many workgroups the rows are dealt to. */
@@ -186,16 +195,17 @@ Shape shape_of(uint64_t rows, uint64_t cols, uint32_t compute_units) {
 uint64_t padded_of(uint64_t cols) { return (cols + 63) / 64 * 64; }
 
 template <typename TG, typename TR, bool DROP> void launch(const NormGradArgs &a, const Shape &shape, hipStream_t s) {
-#define ERI_NORM_GRAD(TPR, NV) \
-    if (shape.tpr == TPR && shape.nv == NV) \
-    hipLaunchKernelGGL((rms_norm_grad_kernel<TG, TR, DROP, TPR, NV>), dim3(shape.groups), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
-    ERI_NORM_GRAD(64, 1);
-    ERI_NORM_GRAD(64, 2);
-    ERI_NORM_GRAD(256, 1);
-    ERI_NORM_GRAD(256, 2);
-    ERI_NORM_GRAD(256, 4);
-    ERI_NORM_GRAD(1024, 2);
-    ERI_NORM_GRAD(1024, 4);
+#define ERI_NORM_GRAD(TPR, NV, SHORT) \
+    if (shape.tpr == TPR && shape.nv == NV && SHORT == (a.cols < 8)) \
+    hipLaunchKernelGGL((rms_norm_grad_kernel<TG, TR, DROP, TPR, NV, SHORT>), dim3(shape.groups), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+    ERI_NORM_GRAD(64, 1, true);
+    ERI_NORM_GRAD(64, 1, false);
+    ERI_NORM_GRAD(64, 2, false);
+    ERI_NORM_GRAD(256, 1, false);
+    ERI_NORM_GRAD(256, 2, false);
+    ERI_NORM_GRAD(256, 4, false);
+    ERI_NORM_GRAD(1024, 2, false);
+    ERI_NORM_GRAD(1024, 4, false);
 #undef ERI_NORM_GRAD
     if (shape.nv == 0) hipLaunchKernelGGL((rms_norm_grad_long_kernel<TG, TR, DROP>), dim3(shape.groups), dim3(1024), 0, s, a);
 }
