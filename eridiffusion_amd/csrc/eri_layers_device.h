@@ -44,6 +44,7 @@ template <> struct Raw<bf16> {
     u32x4 a;
     __device__ __forceinline__ void clear() { a = u32x4{0, 0, 0, 0}; }
     __device__ __forceinline__ void load(const bf16 *p) { a = *(const u32x4_at2 *)p; }
+    __device__ __forceinline__ void load_once(const bf16 *p) { a = __builtin_nontemporal_load((const u32x4_at2 *)p); }
     __device__ __forceinline__ void load_some(const bf16 *p, uint32_t n) { // n < 8 elements
         clear();
 #pragma unroll
@@ -65,6 +66,10 @@ template <> struct Raw<float> {
         a = *(const u32x4_at4 *)p;
         b = *(const u32x4_at4 *)(p + 4);
     }
+    __device__ __forceinline__ void load_once(const float *p) {
+        a = __builtin_nontemporal_load((const u32x4_at4 *)p);
+        b = __builtin_nontemporal_load((const u32x4_at4 *)(p + 4));
+    }
     __device__ __forceinline__ void load_some(const float *p, uint32_t n) {
         clear();
 #pragma unroll
@@ -85,10 +90,11 @@ template <> struct Raw<float> {
  * when the values are wanted.  Where a row ends inside the vector, its last eight elements are loaded instead and shifted
  * into place later: all lanes take the same load, and nothing between two loads waits for the first.  With a branch for each
  * case in its place, the wave at the end of an odd row waited at every row (sums of a table's gradient of 1155 columns: 59 us, so 25).
- * SHORT is for rows of less than eight elements, which have kernels of their own. */
+ * SHORT is for rows of less than eight elements, which have kernels of their own; ONCE for rows that nobody reads again. */
 template <typename I> __device__ __forceinline__ I from_of(I col, I cols) { return col + 8 <= cols ? col : cols - 8; }
-template <bool SHORT, typename T, typename I> __device__ __forceinline__ void load8(Raw<T> &r, const T *row, I col, I cols) {
+template <bool SHORT, bool ONCE = false, typename T, typename I> __device__ __forceinline__ void load8(Raw<T> &r, const T *row, I col, I cols) {
     if (SHORT) r.load_some(row, col == 0 ? (uint32_t)cols : 0u);
+    else if (ONCE) r.load_once(row + from_of(col, cols));
     else r.load(row + from_of(col, cols));
 }
 template <typename I> __device__ __forceinline__ uint32_t past_of(I col, I cols) { // elements of the vector that lie past the row's end

@@ -77,15 +77,15 @@ template <typename T> void launch_lookup_of(const LookupArgs &a, uint32_t comput
  * too, as the number of tokens in the buckets before it: no workgroup waits for another.  Between the two it writes the
  * rows that no token names: stores that nothing waits for.
  *
- * Summing: the runs of equal ids in the sorted list are cut into pieces of kPiece tokens, and a wave sums the pieces that
- * begin in its kStep places of the list, for L*8 columns: its loads go ahead through the list whatever the
- * lengths of the runs, and a wave has at most kStep + kPiece - 1 tokens.  A run of one piece is written as it ends; the pieces
+ * Summing: the runs of equal ids in the sorted list are cut into pieces of 2^log_piece tokens, and a wave sums the pieces that
+ * begin in its step of half as many places, for L*8 columns: its loads go ahead through the list whatever the lengths of the
+ * runs, and a wave has at most a piece and a step less one of tokens.  A run of one piece is written as it ends; the pieces
  * of longer ones are left in the workspace and summed in their order by a third kernel.
  */
 constexpr uint32_t kWaves = 16;       // of a bucket's workgroup
 constexpr uint32_t kLocalMost = 1024; // ids of a bucket
-constexpr uint32_t kPiece = 32;
-constexpr uint32_t kStep = 16;
+constexpr uint32_t kLogPieceMost = 5;
+constexpr uint32_t kListMost = (1 << kLogPieceMost) * 3 / 2; // places that a step and the piece that it ends with take
 
 struct Place { // of the sorted list
     uint32_t token, id;
@@ -99,7 +99,7 @@ struct GradArgs {
     Place *sorted;    // tokens places, of which the first *used are set
     uint32_t *used;
     float *partial;   // sums of pieces, padded floats each
-    uint32_t tokens, vocab, dim, shift, locals, padded, tiles;
+    uint32_t tokens, vocab, dim, shift, locals, padded, tiles, log_piece;
     uint64_t grad_stride, out_stride;
     int64_t padding_id;
     float scale;
@@ -107,10 +107,10 @@ struct GradArgs {
     __device__ __forceinline__ bool counts(int64_t id) const { return (uint64_t)id < vocab && id != padding_id; }
 };
 
-/* Where the sum of the piece at place `start` goes, of a run with several.  The pieces of a run begin kPiece apart, and the
- * next such run begins more than kPiece behind this one's beginning: of those that begin within one kPiece of
- * places, one at most is a run's first and one at most is not. */
-__device__ __forceinline__ uint64_t slot_of(uint32_t start, bool first) { return 2 * (uint64_t)(start / kPiece) + first; }
+/* Where the sum of the piece at place `start` goes, of a run with several.  The pieces of a run begin one length of a piece
+ * apart, and the next such run begins more than that behind this one's beginning: of those that begin within one length
+ * of places, one at most is a run's first and one at most is not. */
+__device__ __forceinline__ uint64_t slot_of(uint32_t start, bool first, uint32_t log_piece) { return 2 * (uint64_t)(start >> log_piece) + first; }
 
 __global__ __launch_bounds__(1024) void embedding_sort_kernel(const GradArgs a) {
     extern __shared__ uint32_t counts[]; // kWaves x locals: first counts, then where the wave's next token of that id goes
@@ -179,22 +179,32 @@ __global__ __launch_bounds__(1024) void embedding_sort_kernel(const GradArgs a) 
 
     // the list: each wave for its share; of several tokens in one step, an id at a time
     if (all_mine == 0) return;
-    for (uint32_t at = from; at < to; at += kWave) {
-        const int64_t id = at + lane < to ? a.ids[at + lane] : -1;
-        const bool own = a.counts(id) && ((uint32_t)id & mask) == bucket;
-        uint64_t left = __ballot(own);
-        while (left) {
-            const uint32_t local = (uint32_t)__builtin_amdgcn_readlane((int)((uint32_t)id >> a.shift), __builtin_ctzll(left));
-            const bool same = own && ((uint32_t)id >> a.shift) == local;
-            const uint64_t all = __ballot(same);
-            uint32_t place = 0;
-            if (lane == 0) place = atomicAdd(&mine[local], (uint32_t)__popcll(all));
-            place = (uint32_t)__builtin_amdgcn_readfirstlane((int)place);
-            if (same) {
-                place += (uint32_t)__popcll(all & ((1ull << lane) - 1));
-                a.sorted[place] = Place{at + lane, (uint32_t)id, place - starts[local], lengths[local]};
+    constexpr uint32_t kIds = 4;
+    for (uint32_t four = from; four < to; four += kIds * kWave) {
+        int64_t ids[kIds];
+#pragma unroll
+        for (uint32_t k = 0; k < kIds; ++k) {
+            const uint32_t t = four + k * kWave + lane;
+            ids[k] = a.ids[t < to ? t : to - 1];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kIds; ++k) {
+            const uint32_t t = four + k * kWave + lane, local_of = (uint32_t)ids[k] >> a.shift;
+            const bool own = t < to && a.counts(ids[k]) && ((uint32_t)ids[k] & mask) == bucket;
+            uint64_t left = __ballot(own);
+            while (left) {
+                const uint32_t local = (uint32_t)__builtin_amdgcn_readlane((int)local_of, __builtin_ctzll(left));
+                const bool same = own && local_of == local;
+                const uint64_t all = __ballot(same);
+                uint32_t place = 0;
+                if (lane == 0) place = atomicAdd(&mine[local], (uint32_t)__popcll(all));
+                place = (uint32_t)__builtin_amdgcn_readfirstlane((int)place);
+                if (same) {
+                    place += (uint32_t)__popcll(all & ((1ull << lane) - 1));
+                    a.sorted[place] = Place{t, (uint32_t)ids[k], place - starts[local], lengths[local]};
+                }
+                left &= ~all;
             }
-            left &= ~all;
         }
     }
 }
@@ -215,37 +225,39 @@ template <bool SHORT, typename TO> __device__ __forceinline__ void finish8(const
 /* L lanes to a step of the list and a tile of L*8 columns.  The places of the step and of what its last piece reaches beyond it
  * come in one trip to memory, then the rows, a set of them on its way while another is added up. */
 template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const GradArgs a) {
-    static_assert(kStep + kPiece <= kWave, "a lane to a place");
-    __shared__ Place list[L == kWave ? 1 : kThreads / L][kStep + kPiece];
+    static_assert(kListMost <= kWave, "a lane to a place");
+    __shared__ Place list[L == kWave ? 1 : kThreads / L][kListMost];
+    const uint32_t piece = 1u << a.log_piece, step = piece / 2;
     uint32_t team = threadIdx.x / L;
     if (L == kWave) team = (uint32_t)__builtin_amdgcn_readfirstlane((int)team);
-    const uint32_t group = blockIdx.x * (kThreads / L) + team, lane = threadIdx.x % L;
-    const uint32_t step = group / a.tiles, col = (group - step * a.tiles) * (L * 8) + lane * 8, begin = step * kStep;
+    const uint32_t group = blockIdx.x * (kThreads / L) + team, lane = threadIdx.x % L, turn = group / a.tiles;
+    const uint32_t col = (group - turn * a.tiles) * (L * 8) + lane * 8, begin = turn * step;
     Place held = {0, 0, 0, 0}; // of a whole wave each lane keeps a place
     if (L == kWave) {
-        if (lane < kStep + kPiece && begin + lane < a.tokens) held = a.sorted[begin + lane];
+        if (lane < step + piece && begin + lane < a.tokens) held = a.sorted[begin + lane];
     } else
-        for (uint32_t i = lane; i < kStep + kPiece; i += L)
+        for (uint32_t i = lane; i < step + piece; i += L)
             if (begin + i < a.tokens) list[team][i] = a.sorted[begin + i];
     const uint32_t used = *a.used;
     __syncthreads();
     if (begin >= used) return;
     // pieces that begin here: from the first one's beginning to the last one's end, counted from `begin`
-    const uint32_t here = used - begin < kStep ? used - begin : kStep;
+    const uint32_t here = used - begin < step ? used - begin : step;
     auto place = [&](uint32_t i) {
         if (L != kWave) return list[team][i];
         auto of = [&](uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)i); };
         return Place{of(held.token), of(held.id), of(held.at), of(held.run)};
     };
-    auto rest = [](const Place &p) { // from p to its piece's end
-        const uint32_t in = p.at % kPiece, left = p.run - p.at;
-        return kPiece - in < left ? kPiece - in : left;
+    auto in = [&](const Place &p) { return p.at & (piece - 1); };
+    auto rest = [&](const Place &p) { // from p to its piece's end
+        const uint32_t left = p.run - p.at;
+        return piece - in(p) < left ? piece - in(p) : left;
     };
     const Place head = place(0);
-    const uint32_t first = head.at % kPiece ? rest(head) : 0;
+    const uint32_t first = in(head) ? rest(head) : 0;
     if (first >= here) return;
     const uint32_t end = here - 1 + rest(place(here - 1));
-    auto ends = [](const Place &p) { return p.at % kPiece == kPiece - 1 || p.at + 1 == p.run; };
+    auto ends = [&](const Place &p) { return in(p) == piece - 1 || p.at + 1 == p.run; };
     // Rows on their way: as many as the registers of two such sets hold.  No load of a set hangs on a condition (the last row stands
     // in for those past the end): with a known number under way, a wait for the first of them leaves the others alone.
     constexpr uint32_t kAhead = sizeof(TG) + (ACC ? sizeof(TO) : 0) <= 4 ? 8 : 4;
@@ -257,7 +269,7 @@ template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __la
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; ++k) {
             const Place p = place(at + k < end ? at + k : end - 1);
-            load8<SHORT>(f.grad[k], (const TG *)a.grad + p.token * a.grad_stride, col, a.dim);
+            load8<SHORT, true>(f.grad[k], (const TG *)a.grad + p.token * a.grad_stride, col, a.dim);
             if (ACC) load8<SHORT>(f.old[k], (const TO *)a.out + p.id * a.out_stride, col, a.dim);
         }
     };
@@ -276,14 +288,14 @@ template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __la
                 v.set(e, sum[e]);
             }
             if (!ends(p)) continue;
-            const bool whole = p.run <= kPiece;
+            const bool whole = p.run <= piece;
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) v.set(e, whole ? sum[e] * a.scale + (ACC ? f.old[k].get(e) : 0.0f) : sum[e]);
             settle8<SHORT>(v, col, a.dim);
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) sum[e] = v.get(e);
             if (whole) store8((TO *)a.out + p.id * a.out_stride, col, a.dim, sum);
-            else store8(a.partial + slot_of(begin + at + k - p.at % kPiece, p.at < kPiece) * a.padded, col, a.padded, sum);
+            else store8(a.partial + slot_of(begin + at + k - in(p), p.at < piece, a.log_piece) * a.padded, col, a.padded, sum);
             v.clear();
         }
     };
@@ -297,28 +309,57 @@ template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __la
     }
 }
 
-/* Runs of several pieces: a wave looks for the one that begins in its kPiece places, and sums its pieces for 512 columns. */
+/* Runs of several pieces: a wave looks for the one that begins in its places, as many as a piece is long, and sums its pieces
+ * for 512 columns.  The pieces of a long one are shared out among the four waves of the workgroup. */
 template <typename TO, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_join_kernel(const GradArgs a) {
-    static_assert(kPiece <= kWave, "a lane to a place");
-    const uint32_t used = *a.used, group = blockIdx.x * (kThreads / kWave) + threadIdx.x / kWave, lane = threadIdx.x % kWave;
-    const uint32_t step = group / a.tiles, col = (group - step * a.tiles) * 512 + lane * 8, at = step * kPiece + lane;
+    constexpr uint32_t kTeam = kThreads / kWave;
+    static_assert(kLogPieceMost <= 6, "a lane to a place");
+    __shared__ Place runs[kTeam]; // token: where it begins
+    __shared__ float sums[kTeam][512];
+    const uint32_t used = *a.used, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, tile = blockIdx.x % a.tiles;
+    const uint32_t begin = (blockIdx.x / a.tiles * kTeam + wave) << a.log_piece, piece = 1u << a.log_piece, col = tile * 512 + lane * 8;
     Place p = {0, 0, 1, 0};
-    if (lane < kPiece && at < used) p = a.sorted[at];
-    const uint64_t found = __ballot(p.at == 0 && p.run > kPiece);
-    if (!found) return;
-    const int from = __builtin_ctzll(found);
-    const uint32_t run = (uint32_t)__builtin_amdgcn_readlane((int)p.run, from), id = (uint32_t)__builtin_amdgcn_readlane((int)p.id, from);
-    const uint32_t start = step * kPiece + from;
-    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-#pragma unroll 8
-    for (uint32_t done = 0; done < run; done += kPiece) {
-        Raw<float> s;
-        load8<false>(s, (const float *)a.partial + slot_of(start + done, done == 0) * a.padded, col, a.padded);
-        settle8<false>(s, col, a.padded);
+    if (lane < piece && begin + lane < used) p = a.sorted[begin + lane];
+    const bool found = p.at == 0 && p.run > piece; // one lane at most
+    if (__ballot(found) == 0) p.run = 0;
+    if (found || (p.run == 0 && lane == 0)) runs[wave] = Place{begin + lane, p.id, 0, p.run};
+    __syncthreads();
+    auto sum = [&](float (&v)[8], const Place &r, uint32_t from, uint32_t to) { // pieces of a run
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) v[e] += s.get(e);
+        for (uint32_t e = 0; e < 8; ++e) v[e] = 0.0f;
+#pragma unroll 8
+        for (uint32_t k = from; k < to; ++k) {
+            Raw<float> s;
+            load8<false>(s, (const float *)a.partial + slot_of(r.token + (k << a.log_piece), k == 0, a.log_piece) * a.padded, col, a.padded);
+            settle8<false>(s, col, a.padded);
+#pragma unroll
+            for (uint32_t e = 0; e < 8; ++e) v[e] += s.get(e);
+        }
+    };
+    constexpr uint32_t kAlone = 8; // pieces that a wave sums by itself: they are all on their way at once
+    float v[8];
+    const Place own = runs[wave];
+    const uint32_t pieces = (own.run + piece - 1) >> a.log_piece;
+    if (own.run && pieces <= kAlone) {
+        sum(v, own, 0, pieces);
+        finish8<SHORT, TO>(a, own.id, col, v);
     }
-    finish8<SHORT, TO>(a, id, col, v);
+    for (uint32_t w = 0; w < kTeam; ++w) { // the same for all waves
+        const Place r = runs[w];
+        const uint32_t n = (r.run + piece - 1) >> a.log_piece, share = (n + kTeam - 1) / kTeam;
+        if (n <= kAlone) continue;
+        sum(v, r, share * wave < n ? share * wave : n, share * (wave + 1) < n ? share * (wave + 1) : n);
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) sums[wave][e * kWave + lane] = v[e];
+        __syncthreads();
+        if (wave == 0) {
+            for (uint32_t o = 1; o < kTeam; ++o)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) v[e] += sums[o][e * kWave + lane];
+            finish8<SHORT, TO>(a, r.id, col, v);
+        }
+        __syncthreads();
+    }
 }
 
 uint32_t shift_of(uint64_t vocab) {
@@ -328,27 +369,41 @@ uint32_t shift_of(uint64_t vocab) {
 }
 uint64_t padded_of(uint64_t dim) { return (dim + 7) / 8 * 8; }
 
+uint32_t lanes_of(uint64_t dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : dim <= 256 ? 32 : 64; } // to a row in the sums
+
+/* Short pieces where that is what it takes to have a wave for every SIMD. */
+uint32_t log_piece_of(uint64_t tokens, uint64_t dim) {
+    const uint64_t lanes = lanes_of(dim), tiles = (dim + lanes * 8 - 1) / (lanes * 8);
+    uint32_t log_piece = kLogPieceMost;
+    while (log_piece > 3 && (tokens >> (log_piece - 1)) * tiles * lanes < 2048 * kWave) --log_piece;
+    return log_piece;
+}
+
 /* The workspace: the number of places, the places, the sums of pieces; 16 bytes and multiples of them. */
 constexpr uint64_t kHead = 16;
 uint64_t partial_at(uint64_t tokens) { return kHead + tokens * sizeof(Place); }
-uint64_t partial_bytes(uint64_t tokens, uint64_t dim) { return tokens > kPiece ? 2 * (tokens / kPiece + 1) * padded_of(dim) * sizeof(float) : 0; }
+uint64_t partial_bytes(uint64_t tokens, uint64_t dim) {
+    const uint32_t log_piece = log_piece_of(tokens, dim);
+    return tokens >> log_piece ? 2 * ((tokens >> log_piece) + 1) * padded_of(dim) * sizeof(float) : 0;
+}
 
 template <typename TG, typename TO, int L, bool SHORT = false> void launch_sum(GradArgs a, hipStream_t s) {
     a.tiles = (a.dim + L * 8 - 1) / (L * 8);
-    uint64_t groups = (uint64_t)((a.tokens + kStep - 1) / kStep) * a.tiles;
+    const uint32_t piece = 1u << a.log_piece, step = piece / 2;
+    const uint64_t groups = (uint64_t)((a.tokens + step - 1) / step) * a.tiles;
     const dim3 grid((uint32_t)((groups + kThreads / L - 1) / (kThreads / L)));
     if (a.accumulate) hipLaunchKernelGGL((embedding_sum_kernel<TG, TO, L, true, SHORT>), grid, dim3(kThreads), 0, s, a);
     else hipLaunchKernelGGL((embedding_sum_kernel<TG, TO, L, false, SHORT>), grid, dim3(kThreads), 0, s, a);
-    if (a.tokens <= kPiece) return;
+    if (a.tokens <= piece) return;
     a.tiles = (a.dim + 511) / 512;
-    groups = (uint64_t)((a.tokens + kPiece - 1) / kPiece) * a.tiles;
-    hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT>), dim3((uint32_t)((groups + 3) / 4)), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT>), dim3((a.tokens + 4 * piece - 1) / (4 * piece) * a.tiles), dim3(kThreads), 0, s, a);
 }
 template <typename TG, typename TO> void launch_sums(const GradArgs &a, hipStream_t s) {
+    const uint32_t lanes = lanes_of(a.dim);
     if (a.dim < 8) launch_sum<TG, TO, 8, true>(a, s);
-    else if (a.dim <= 64) launch_sum<TG, TO, 8>(a, s);
-    else if (a.dim <= 128) launch_sum<TG, TO, 16>(a, s);
-    else if (a.dim <= 256) launch_sum<TG, TO, 32>(a, s);
+    else if (lanes == 8) launch_sum<TG, TO, 8>(a, s);
+    else if (lanes == 16) launch_sum<TG, TO, 16>(a, s);
+    else if (lanes == 32) launch_sum<TG, TO, 32>(a, s);
     else launch_sum<TG, TO, 64>(a, s);
 }
 
@@ -368,7 +423,7 @@ uint64_t embedding_grad_workspace(uint64_t tokens, uint64_t, uint64_t dim) { ret
 int launch_embedding_grad(const EriEmbeddingGrad &e, uint32_t, void *stream) {
     char *ws = static_cast<char *>(e.workspace);
     GradArgs a = {{e.ids, (uint32_t)e.ids_64}, e.grad, e.out, (Place *)(ws + kHead), (uint32_t *)ws, (float *)(ws + partial_at(e.tokens)),
-                  (uint32_t)e.tokens, (uint32_t)e.vocab, (uint32_t)e.dim, shift_of(e.vocab), 0, (uint32_t)padded_of(e.dim), 0,
+                  (uint32_t)e.tokens, (uint32_t)e.vocab, (uint32_t)e.dim, shift_of(e.vocab), 0, (uint32_t)padded_of(e.dim), 0, log_piece_of(e.tokens, e.dim),
                   e.grad_stride, e.out_stride, e.padding_id, e.scale, (uint32_t)(e.accumulate != 0), e.out_dtype == ERI_DTYPE_F32 ? 4u : 2u, 1};
     const uint32_t buckets = 1u << a.shift;
     a.locals = (a.vocab + buckets - 1) >> a.shift;
