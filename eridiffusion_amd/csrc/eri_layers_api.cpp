@@ -121,10 +121,11 @@ int eri_embedding_grad(const EriEmbeddingGrad *args, void *stream) {
     if (int rc = ids_ok(a.ids, a.ids_64, a.tokens, a.vocab, a.dim, kCall)) return rc;
     ERI_NEED(floating(a.grad_dtype) && floating(a.out_dtype), ERI_ERR_DTYPE, "unsupported dtype tag (F32=0 and BF16=2 are supported)");
     ERI_NEED(stride(&a.grad_stride, a.dim) && stride(&a.out_stride, a.dim), ERI_ERR_ARG, "a stride shorter than a row");
-    ERI_NEED((a.grad || a.tokens == 0) && a.out && a.workspace, ERI_ERR_NULL, "grad, out or workspace is NULL");
+    const uint64_t need = eri_layers::embedding_grad_workspace(a.tokens, a.vocab, a.dim);
+    ERI_NEED((a.grad || a.tokens == 0) && a.out && (a.workspace || need == 0), ERI_ERR_NULL, "grad, out or workspace is NULL");
     ERI_NEED(aligned(a.grad, size_of(a.grad_dtype)) && aligned(a.out, size_of(a.out_dtype)), ERI_ERR_ALIGN, "grad or out is not aligned to its elements");
     ERI_NEED(aligned(a.workspace, 16), ERI_ERR_ALIGN, "workspace is not 16-byte aligned");
-    ERI_NEED(a.workspace_bytes >= eri_layers::embedding_grad_workspace(a.tokens, a.vocab, a.dim), ERI_ERR_ARG, "workspace is too small");
+    ERI_NEED(a.workspace_bytes >= need, ERI_ERR_ARG, "workspace is too small");
     uint32_t cus;
     if (int rc = compute_units(&cus, kCall)) return rc;
     return done(eri_layers::launch_embedding_grad(a, cus, stream), kCall);

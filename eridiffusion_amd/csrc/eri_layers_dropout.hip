@@ -46,7 +46,8 @@ int launch_dropout(const EriDropout &e, const Drop &d, uint32_t compute_units, v
     }
     a.vectors = (a.cols + 7) / 8;
     const uint64_t x = (a.vectors + kThreads - 1) / kThreads, most = (uint64_t)compute_units * 64;
-    const dim3 grid((uint32_t)(x < most ? x : most), a.rows < 65535 ? a.rows : 65535);
+    const uint64_t across = x < most ? x : most, down = most / across; // of workgroups; the rest in turn
+    const dim3 grid((uint32_t)across, (uint32_t)(a.rows < down ? a.rows : down));
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool f32 = e.dtype_tag == ERI_DTYPE_F32, is_short = a.cols < 8;
     void (*const kernel)(const DropoutArgs) = f32 ? is_short ? dropout_kernel<float, true> : dropout_kernel<float, false>

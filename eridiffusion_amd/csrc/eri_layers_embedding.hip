@@ -362,10 +362,132 @@ template <typename TO, bool SHORT> __global__ __launch_bounds__(kThreads) void e
     }
 }
 
-uint32_t shift_of(uint64_t vocab) {
+/* A wave's zeros for SIZE bytes of a row of so many, an even number. */
+template <uint32_t SIZE> __device__ __forceinline__ void zeros(char *row, uint32_t tile, uint32_t lane, uint64_t bytes) {
+#pragma unroll
+    for (uint32_t part = 0; part < SIZE; part += kWave * 16) {
+        const uint64_t at = (uint64_t)tile * SIZE + part + lane * 16;
+        if (at + 16 <= bytes) *(u32x4_at2 *)(row + at) = u32x4{0, 0, 0, 0};
+        else
+            for (uint64_t b = at; b < bytes; b += 2) *(uint16_t *)(row + b) = 0;
+    }
+}
+
+/*
+ * Few tokens: one launch.  A workgroup has a bucket's rows and a tile of 512 columns; each finds its tokens among all of them by
+ * itself, writes its rows without a token, and sums the others: a row with up to kAloneFew tokens by one wave, one with more by
+ * all four, their parts joined in the waves' order.
+ */
+constexpr uint32_t kFewTokens = 1024;
+constexpr uint32_t kFewLocals = 64; // rows of a bucket
+constexpr uint32_t kAloneFew = 16;
+template <typename TG, typename TO, bool ACC, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_few_kernel(const GradArgs a) {
+    constexpr uint32_t kTeam = kThreads / kWave, kEach = kFewTokens / kThreads, kAhead = 8;
+    __shared__ uint32_t counts[kFewLocals], numbers[kEach * kTeam], list[kFewTokens]; // list: token << 16 | local, ascending
+    __shared__ float sums[kTeam][512];
+    const uint32_t bucket = blockIdx.x / a.tiles, tile = blockIdx.x - bucket * a.tiles, mask = (1u << a.shift) - 1;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / kWave)), lane = threadIdx.x % kWave, col = tile * 512 + lane * 8;
+    int64_t ids[kEach];
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+        const uint32_t t = k * kThreads + threadIdx.x;
+        ids[k] = k * kThreads < a.tokens ? a.ids[t < a.tokens ? t : a.tokens - 1] : -1;
+    }
+    if (threadIdx.x < kFewLocals) counts[threadIdx.x] = 0;
+    __syncthreads();
+    uint64_t owns[kEach];
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k) {
+        const bool own = k * kThreads + threadIdx.x < a.tokens && a.counts(ids[k]) && ((uint32_t)ids[k] & mask) == bucket;
+        if (own) atomicAdd(&counts[(uint32_t)ids[k] >> a.shift], 1u);
+        owns[k] = __ballot(own);
+        if (lane == 0) numbers[k * kTeam + wave] = (uint32_t)__popcll(owns[k]);
+    }
+    __syncthreads();
+    uint32_t m = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kEach; ++k)
+#pragma unroll
+        for (uint32_t w = 0; w < kTeam; ++w) {
+            if (w == wave && (owns[k] >> lane & 1))
+                list[m + (uint32_t)__popcll(owns[k] & ((1ull << lane) - 1))] = (k * kThreads + threadIdx.x) << 16 | (uint32_t)ids[k] >> a.shift;
+            m += numbers[k * kTeam + w];
+        }
+    const uint32_t length = lane < kFewLocals ? counts[lane] : 0; // of the row with the lane's number
+    const uint64_t exist = __ballot((lane << a.shift | bucket) < a.vocab && lane < a.locals);
+    __syncthreads();
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (!ACC)
+        for (uint64_t left = exist & ~__ballot(length != 0); left; left &= left - 1) {
+            const uint32_t local = (uint32_t)__builtin_ctzll(left);
+            if (local % kTeam == wave) zeros<512 * sizeof(TO)>((char *)a.out + (uint64_t)(local << a.shift | bucket) * a.out_stride * sizeof(TO), tile, lane, (uint64_t)a.dim * sizeof(TO));
+        }
+    // the tokens of a row, those whose number in it is `from` or `every` more and so on
+    auto sum = [&](uint32_t local, uint32_t from, uint32_t every) {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) v[e] = 0.0f;
+        uint32_t number = 0, n = 0, held = 0; // lane n of held: the n-th token that is under way
+        auto flush = [&]() {
+            Raw<TG> g[kAhead];
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; ++k)
+                load8<SHORT>(g[k], (const TG *)a.grad + (uint32_t)__builtin_amdgcn_readlane((int)held, (int)(k < n ? k : n - 1)) * a.grad_stride, col, a.dim);
+#pragma unroll
+            for (uint32_t k = 0; k < kAhead; ++k) {
+                if (k >= n) break;
+                settle8<SHORT>(g[k], col, a.dim);
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) v[e] += g[k].get(e);
+            }
+            n = 0;
+        };
+        for (uint32_t at = 0; at < m; at += kWave) {
+            const uint32_t entry = at + lane < m ? list[at + lane] : 0xffffu;
+            for (uint64_t left = __ballot((entry & 0xffffu) == local); left; left &= left - 1, ++number) {
+                if (number % every != from) continue;
+                const uint32_t token = (uint32_t)__builtin_amdgcn_readlane((int)(entry >> 16), __builtin_ctzll(left));
+                held = lane == n ? token : held;
+                if (++n == kAhead) flush();
+            }
+        }
+        if (n) flush();
+    };
+    uint32_t turn = 0;
+    for (uint64_t left = __ballot(length != 0 && length <= kAloneFew); left; left &= left - 1, ++turn) {
+        if (turn % kTeam != wave) continue;
+        const uint32_t local = (uint32_t)__builtin_ctzll(left);
+        sum(local, 0, 1);
+        finish8<SHORT, TO>(a, local << a.shift | bucket, col, v);
+    }
+    for (uint64_t left = __ballot(length > kAloneFew); left; left &= left - 1) { // the same for all waves
+        const uint32_t local = (uint32_t)__builtin_ctzll(left);
+        sum(local, wave, kTeam);
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) sums[wave][e * kWave + lane] = v[e];
+        __syncthreads();
+        if (wave == 0) {
+            for (uint32_t o = 1; o < kTeam; ++o)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) v[e] += sums[o][e * kWave + lane];
+            finish8<SHORT, TO>(a, local << a.shift | bucket, col, v);
+        }
+        __syncthreads();
+    }
+}
+
+uint32_t shift_of(uint64_t vocab, uint32_t most) { // for at most so many ids in a bucket
     uint32_t shift = 8;
-    while (((vocab + (1ull << shift) - 1) >> shift) > kLocalMost) ++shift;
+    while (((vocab + (1ull << shift) - 1) >> shift) > most) ++shift;
     return shift;
+}
+/* One launch instead of three for few tokens, as long as the table is not so large that writing its zeros decides: whole rows from
+ * fewer workgroups fill it faster then.  us, one launch | three, for 2, 300 and 1024 tokens:
+ *   1000 x 768 bf16      5.2 | 8.9     6.4 | 13.6   10.9 | 14.8
+ *   32000 x 2048 bf16    23.6 | 24.1   24.1 | 28.6  24.6 | 30.6
+ *   49408 x 768 fp32     25.3 | 26.3   25.7 | 31.4  26.1 | 32.9
+ *   44679 x 3630 fp32    182 | 142     182 | 148    183 | 150 */
+bool is_few(uint64_t tokens, uint64_t vocab, uint64_t dim) {
+    return tokens <= kFewTokens && vocab * dim <= 1u << 26 && ((dim + 511) / 512 << shift_of(vocab, kFewLocals)) <= 1u << 20;
 }
 uint64_t padded_of(uint64_t dim) { return (dim + 7) / 8 * 8; }
 
@@ -407,32 +529,55 @@ template <typename TG, typename TO> void launch_sums(const GradArgs &a, hipStrea
     else launch_sum<TG, TO, 64>(a, s);
 }
 
+template <typename TG, typename TO> void launch_few(const GradArgs &a, uint32_t buckets, hipStream_t s) {
+    void (*const kernel)(const GradArgs) =
+        a.dim < 8 ? a.accumulate ? embedding_few_kernel<TG, TO, true, true> : embedding_few_kernel<TG, TO, false, true>
+                  : a.accumulate ? embedding_few_kernel<TG, TO, true, false> : embedding_few_kernel<TG, TO, false, false>;
+    hipLaunchKernelGGL(kernel, dim3(buckets * a.tiles), dim3(kThreads), 0, s, a);
+}
+
 } // namespace
 
 int launch_embedding(const EriEmbedding &e, uint32_t compute_units, void *stream) {
-    const LookupArgs a = {{e.ids, (uint32_t)e.ids_64}, e.table, e.out, (uint32_t)e.tokens, (uint32_t)e.vocab, (uint32_t)e.dim,
-                          e.table_stride, e.out_stride, e.scale};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (e.dtype_tag == ERI_DTYPE_F32) launch_lookup_of<float>(a, compute_units, s);
-    else launch_lookup_of<bf16>(a, compute_units, s);
-    return (int)hipGetLastError();
+    const bool f32 = e.dtype_tag == ERI_DTYPE_F32;
+    constexpr uint64_t kMost = 1u << 22; // tokens of a launch
+    for (uint64_t at = 0; at < e.tokens; at += kMost) {
+        const LookupArgs a = {{(const char *)e.ids + at * (e.ids_64 ? 8 : 4), (uint32_t)e.ids_64}, e.table, (char *)e.out + at * e.out_stride * (f32 ? 4 : 2),
+                              (uint32_t)(e.tokens - at < kMost ? e.tokens - at : kMost), (uint32_t)e.vocab, (uint32_t)e.dim, e.table_stride, e.out_stride, e.scale};
+        if (f32) launch_lookup_of<float>(a, compute_units, s);
+        else launch_lookup_of<bf16>(a, compute_units, s);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return (int)err;
+    }
+    return 0;
 }
 
-uint64_t embedding_grad_workspace(uint64_t tokens, uint64_t, uint64_t dim) { return partial_at(tokens) + partial_bytes(tokens, dim); }
+uint64_t embedding_grad_workspace(uint64_t tokens, uint64_t vocab, uint64_t dim) {
+    return is_few(tokens, vocab, dim) ? 0 : partial_at(tokens) + partial_bytes(tokens, dim);
+}
 
 int launch_embedding_grad(const EriEmbeddingGrad &e, uint32_t, void *stream) {
     char *ws = static_cast<char *>(e.workspace);
+    const bool few = is_few(e.tokens, e.vocab, e.dim);
     GradArgs a = {{e.ids, (uint32_t)e.ids_64}, e.grad, e.out, (Place *)(ws + kHead), (uint32_t *)ws, (float *)(ws + partial_at(e.tokens)),
-                  (uint32_t)e.tokens, (uint32_t)e.vocab, (uint32_t)e.dim, shift_of(e.vocab), 0, (uint32_t)padded_of(e.dim), 0, log_piece_of(e.tokens, e.dim),
-                  e.grad_stride, e.out_stride, e.padding_id, e.scale, (uint32_t)(e.accumulate != 0), e.out_dtype == ERI_DTYPE_F32 ? 4u : 2u, 1};
-    const uint32_t buckets = 1u << a.shift;
-    a.locals = (a.vocab + buckets - 1) >> a.shift;
-    while (a.lanes < kWave && a.lanes * 16ull < (uint64_t)a.dim * a.out_bytes) a.lanes *= 2;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(embedding_sort_kernel, dim3(buckets < a.vocab ? buckets : a.vocab), dim3(1024), kWaves * a.locals * 4, s, a);
-    const hipError_t err = hipGetLastError();
-    if (err != hipSuccess || a.tokens == 0) return (int)err;
+                  (uint32_t)e.tokens, (uint32_t)e.vocab, (uint32_t)e.dim, shift_of(e.vocab, few ? kFewLocals : kLocalMost), 0, (uint32_t)padded_of(e.dim), 0,
+                  log_piece_of(e.tokens, e.dim), e.grad_stride, e.out_stride, e.padding_id, e.scale, (uint32_t)(e.accumulate != 0),
+                  e.out_dtype == ERI_DTYPE_F32 ? 4u : 2u, 1};
     const bool g32 = e.grad_dtype == ERI_DTYPE_F32, o32 = e.out_dtype == ERI_DTYPE_F32;
+    const uint32_t buckets = 1u << a.shift, used_buckets = buckets < a.vocab ? buckets : a.vocab;
+    a.locals = (a.vocab + buckets - 1) >> a.shift;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (few) {
+        a.tiles = (a.dim + 511) / 512;
+        if (g32) o32 ? launch_few<float, float>(a, used_buckets, s) : launch_few<float, bf16>(a, used_buckets, s);
+        else o32 ? launch_few<bf16, float>(a, used_buckets, s) : launch_few<bf16, bf16>(a, used_buckets, s);
+        return (int)hipGetLastError();
+    }
+    while (a.lanes < kWave && a.lanes * 16ull < (uint64_t)a.dim * a.out_bytes) a.lanes *= 2;
+    hipLaunchKernelGGL(embedding_sort_kernel, dim3(used_buckets), dim3(1024), kWaves * a.locals * 4, s, a);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return (int)err;
     if (g32) o32 ? launch_sums<float, float>(a, s) : launch_sums<float, bf16>(a, s);
     else o32 ? launch_sums<bf16, float>(a, s) : launch_sums<bf16, bf16>(a, s);
     return (int)hipGetLastError();

@@ -13,7 +13,7 @@ struct NormArgs {
     const void *x, *residual, *weight;
     void *y, *h;
     float *rstd, *scales;
-    uint32_t rows, cols;
+    uint32_t first, rows, cols; // rows first .. rows-1
     uint64_t x_stride, residual_stride, y_stride, h_stride;
     float eps;
     uint32_t weight_f32, y_dtype, group, groups;
@@ -94,7 +94,7 @@ template <typename TX, typename TR, bool RES, bool DROP, int TPR, int NV, bool S
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const NormArgs a) {
     constexpr int kWaves = TPR / kWave;
     __shared__ float slots[2][kWaves < 2 ? 1 : kWaves];
-    const uint32_t row = blockIdx.x * rows_of(TPR) + threadIdx.x / TPR, t = threadIdx.x % TPR;
+    const uint32_t row = a.first + blockIdx.x * rows_of(TPR) + threadIdx.x / TPR, t = threadIdx.x % TPR;
     if (row >= a.rows) return; // a whole wave, and only where a row is one wave's
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     Raw<TX> x[NV];
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
  * element by the thread that has just read it, so that they may replace the residual and x. */
 template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bounds__(1024) void rms_norm_long_kernel(const NormArgs a) {
     __shared__ float slots[2][16];
-    const uint32_t row = blockIdx.x;
+    const uint32_t row = a.first + blockIdx.x;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     auto value = [&](float (&h)[8], uint32_t col) {
         Raw<TX> x;
@@ -188,7 +188,7 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
 
 template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormArgs &a, uint32_t compute_units, hipStream_t s) {
 #define ERI_NORM(TPR, NV, SHORT) \
-    hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV, SHORT>), dim3((a.rows + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+    hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV, SHORT>), dim3((a.rows - a.first + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
     if (a.cols < 8) ERI_NORM(64, 1, true);
     else if (a.cols <= 512) ERI_NORM(64, 1, false);
     else if (a.cols <= 1024) ERI_NORM(64, 2, false);
@@ -197,7 +197,7 @@ template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormA
     else if (a.cols <= 8192) ERI_NORM(256, 4, false);
     else if (a.cols <= 16384) ERI_NORM(1024, 2, false);
     else if (a.cols <= 32768) ERI_NORM(1024, 4, false);
-    else hipLaunchKernelGGL((rms_norm_long_kernel<TX, TR, RES, DROP>), dim3(a.rows), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((rms_norm_long_kernel<TX, TR, RES, DROP>), dim3(a.rows - a.first), dim3(1024), 0, s, a);
 #undef ERI_NORM
 }
 
@@ -211,13 +211,19 @@ template <typename TX> void launch_of(const NormArgs &a, bool res, bool res_f32,
 } // namespace
 
 int launch_rms_norm(const EriRmsNorm &e, const Drop &d, uint32_t compute_units, void *stream) {
-    const NormArgs a = {e.x, e.residual, e.weight, e.y, e.h, e.rstd, e.scales, (uint32_t)e.rows, (uint32_t)e.cols,
-                        e.x_stride, e.residual_stride, e.y_stride, e.h_stride, e.eps, e.weight_dtype == ERI_DTYPE_F32, (uint32_t)e.y_dtype,
-                        (uint32_t)e.scale_group, e.scale_group ? (uint32_t)((e.cols + 127) / 128) : 1u, d};
+    NormArgs a = {e.x, e.residual, e.weight, e.y, e.h, e.rstd, e.scales, 0, 0, (uint32_t)e.cols,
+                  e.x_stride, e.residual_stride, e.y_stride, e.h_stride, e.eps, e.weight_dtype == ERI_DTYPE_F32, (uint32_t)e.y_dtype,
+                  (uint32_t)e.scale_group, e.scale_group ? (uint32_t)((e.cols + 127) / 128) : 1u, d};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (e.x_dtype == ERI_DTYPE_F32) launch_of<float>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, compute_units, s);
-    else launch_of<bf16>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, compute_units, s);
-    return (int)hipGetLastError();
+    constexpr uint32_t kMost = 1u << 21; // rows of a launch
+    for (a.first = 0; a.first < e.rows; a.first += kMost) {
+        a.rows = e.rows - a.first < kMost ? (uint32_t)e.rows : a.first + kMost;
+        if (e.x_dtype == ERI_DTYPE_F32) launch_of<float>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, compute_units, s);
+        else launch_of<bf16>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, compute_units, s);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return (int)err;
+    }
+    return 0;
 }
 
 } // namespace eri_layers

@@ -10,8 +10,9 @@ struct NormGradArgs {
     const void *grad, *h, *weight, *grad_h;
     const float *rstd;
     void *grad_x, *grad_residual;
-    float *partial; // per workgroup a row of grad_weight's sums, padded floats apart; NULL: not wanted
-    uint32_t rows, cols, padded;
+    float *partial;    // per workgroup a row of grad_weight's sums, padded floats apart; NULL: not wanted
+    void *grad_weight; // few rows: written by the workgroups behind the first row_groups; NULL otherwise
+    uint32_t rows, cols, padded, row_groups, grad_weight_f32;
     uint64_t grad_stride, h_stride, grad_h_stride, grad_x_stride, grad_residual_stride;
     uint32_t weight_f32, x_f32;
     Drop drop;
@@ -32,12 +33,42 @@ __device__ __forceinline__ void store_grads(const NormGradArgs &a, uint32_t row,
     else store8((bf16 *)a.grad_x + row * a.grad_x_stride, col, a.cols, dh);
 }
 
+/* grad_weight of 32 columns over all rows: four lanes to a row's part of them, the rest of the workgroup side by side, and their
+ * sums joined in their order. */
+template <typename TG, typename TR, bool SHORT, int THREADS> __device__ __forceinline__ void weight_of_columns(const NormGradArgs &a, uint32_t tile) {
+    __shared__ float sums[THREADS / 4][32];
+    const uint32_t part = threadIdx.x / 4, in = threadIdx.x % 4 * 8, col = tile * 32 + in;
+    float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll 4
+    for (uint32_t row = part; row < a.rows; row += THREADS / 4) {
+        Raw<TG> g;
+        Raw<TR> h;
+        load8<SHORT>(g, (const TG *)a.grad + row * a.grad_stride, col, a.cols);
+        load8<SHORT>(h, (const TR *)a.h + row * a.h_stride, col, a.cols);
+        const float rstd = a.rstd[row];
+        settle8<SHORT>(g, col, a.cols);
+        settle8<SHORT>(h, col, a.cols);
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) v[e] = fmaf(g.get(e) * h.get(e), rstd, v[e]);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 8; ++e) sums[part][in + e] = v[e];
+    __syncthreads();
+    const uint32_t c = tile * 32 + threadIdx.x;
+    if (threadIdx.x >= 32 || c >= a.cols) return;
+    float total = 0.0f;
+    for (uint32_t p = 0; p < THREADS / 4; ++p) total += sums[p][threadIdx.x];
+    if (a.grad_weight_f32) ((float *)a.grad_weight)[c] = total;
+    else ((bf16 *)a.grad_weight)[c].bits = (uint16_t)bf16_pair(total, 0.0f);
+}
+
 /* A row at a time to TPR threads, which keep the weight and their columns' sums of grad_weight in registers. */
 template <typename TG, typename TR, bool DROP, int TPR, int NV, bool SHORT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(const NormGradArgs a) {
     constexpr int kWaves = TPR / kWave;
     __shared__ float slots[2][kWaves < 2 ? 1 : kWaves];
     __shared__ float joined[TPR < 256 ? TPR * NV * 8 : 1];
+    if (blockIdx.x >= a.row_groups) return weight_of_columns<TG, TR, SHORT, TPR < 256 ? 256 : TPR>(a, blockIdx.x - a.row_groups);
     const uint32_t t = threadIdx.x % TPR;
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     float w[NV][8], acc[NV][8];
@@ -51,7 +82,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(co
         }
     }
     uint32_t turn = 0;
-    for (uint32_t row = blockIdx.x * kRowsOf(TPR) + threadIdx.x / TPR; row < a.rows; row += gridDim.x * kRowsOf(TPR), turn ^= 1) {
+    for (uint32_t row = blockIdx.x * kRowsOf(TPR) + threadIdx.x / TPR; row < a.rows; row += a.row_groups * kRowsOf(TPR), turn ^= 1) {
         Raw<TG> g[NV];
         Raw<TR> h[NV], r[NV];
 #pragma unroll
@@ -180,6 +211,16 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_weight_kernel(const float 
     else ((bf16 *)out)[c].bits = (uint16_t)bf16_pair(total, 0.0f);
 }
 
+/* Few rows: grad_weight comes out of the same launch, from workgroups that read grad and h once more, instead of a second one
+ * over the sums that the rows' workgroups leave.  us, one launch | two, at so many rows:
+ *   rows            128          512          768          1024         1536
+ *   256 bf16     5.8 | 9.0    5.8 | 9.1    6.0 | 9.0    5.9 | 9.1    6.1 | 9.3
+ *   1024 fp32    5.8 | 8.9    5.6 | 8.9    6.6 | 8.8    8.7 | 9.2   11.3 | 10.4
+ *   1281 bf16    5.5 | 9.0    6.1 | 8.9    8.4 | 9.4   10.5 | 9.6   14.7 | 10.6
+ *   4096 bf16    5.4 | 8.8    6.7 | 12.5   9.3 | 13.6  11.8 | 13.8  16.6 | 15.5
+ *   8192 fp32    5.8 | 10.5  17.6 | 20.1  28.6 | 26.1  34.0 | 31.4  48.3 | 42.2 */
+bool is_few(uint64_t rows, uint64_t cols) { return rows <= (cols <= 512 ? 1536 : 768); }
+
 /* Threads to a row, and how many workgroups the rows are dealt to. */
 struct Shape {
     int tpr, nv; // nv 0: rows too long for registers
@@ -188,16 +229,17 @@ struct Shape {
 Shape shape_of(uint64_t rows, uint64_t cols, uint32_t compute_units) {
     Shape s = cols <= 512 ? Shape{64, 1, 0} : cols <= 1024 ? Shape{64, 2, 0} : cols <= 2048 ? Shape{256, 1, 0} : cols <= 4096 ? Shape{256, 2, 0} :
               cols <= 8192 ? Shape{256, 4, 0} : cols <= 16384 ? Shape{1024, 2, 0} : cols <= 32768 ? Shape{1024, 4, 0} : Shape{1024, 0, 0};
-    const uint64_t all = (rows + kRowsOf(s.tpr) - 1) / kRowsOf(s.tpr), most = (uint64_t)compute_units * (s.tpr == 1024 ? 1 : 4);
+    const uint64_t all = (rows + kRowsOf(s.tpr) - 1) / kRowsOf(s.tpr), most = (uint64_t)compute_units * (s.tpr == 1024 ? 1 : 2); // more of them leave more sums to read again: with 4, 3-15 % slower
     s.groups = (uint32_t)(all < most ? all : most);
     return s;
 }
 uint64_t padded_of(uint64_t cols) { return (cols + 63) / 64 * 64; }
 
 template <typename TG, typename TR, bool DROP> void launch(const NormGradArgs &a, const Shape &shape, hipStream_t s) {
+    const uint32_t groups = shape.groups + (a.grad_weight ? a.padded / 32 : 0);
 #define ERI_NORM_GRAD(TPR, NV, SHORT) \
     if (shape.tpr == TPR && shape.nv == NV && SHORT == (a.cols < 8)) \
-    hipLaunchKernelGGL((rms_norm_grad_kernel<TG, TR, DROP, TPR, NV, SHORT>), dim3(shape.groups), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+    hipLaunchKernelGGL((rms_norm_grad_kernel<TG, TR, DROP, TPR, NV, SHORT>), dim3(groups), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
     ERI_NORM_GRAD(64, 1, true);
     ERI_NORM_GRAD(64, 1, false);
     ERI_NORM_GRAD(64, 2, false);
@@ -224,10 +266,13 @@ uint64_t rms_norm_grad_workspace(uint64_t rows, uint64_t cols, uint32_t compute_
 int launch_rms_norm_grad(const EriRmsNormGrad &e, const Drop &d, uint32_t compute_units, void *stream) {
     const Shape shape = shape_of(e.rows, e.cols, compute_units);
     const uint32_t padded = (uint32_t)padded_of(e.cols);
-    float *partial = e.grad_weight ? (float *)e.workspace : nullptr;
-    const NormGradArgs a = {e.grad, e.h, e.weight, e.grad_h, e.rstd, e.grad_x, e.grad_residual, partial, (uint32_t)e.rows, (uint32_t)e.cols, padded,
-                            e.grad_stride, e.h_stride, e.grad_h_stride, e.grad_x_stride, e.grad_residual_stride, e.weight_dtype == ERI_DTYPE_F32,
-                            e.x_dtype == ERI_DTYPE_F32, d};
+    // grad and h are read twice where that saves the second launch; not when one of them is being replaced
+    const bool replaces = (e.grad_x && (e.grad_x == e.grad || e.grad_x == e.h)) || (e.grad_residual && (e.grad_residual == e.grad || e.grad_residual == e.h));
+    const bool few = e.grad_weight && e.rows && is_few(e.rows, e.cols) && shape.nv && !replaces;
+    float *partial = e.grad_weight && !few ? (float *)e.workspace : nullptr;
+    const NormGradArgs a = {e.grad, e.h, e.weight, e.grad_h, e.rstd, e.grad_x, e.grad_residual, partial, few ? e.grad_weight : nullptr, (uint32_t)e.rows,
+                            (uint32_t)e.cols, padded, shape.groups, e.grad_weight_dtype == ERI_DTYPE_F32, e.grad_stride, e.h_stride, e.grad_h_stride, e.grad_x_stride,
+                            e.grad_residual_stride, e.weight_dtype == ERI_DTYPE_F32, e.x_dtype == ERI_DTYPE_F32, d};
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (e.rows) {
         if (e.grad_dtype == ERI_DTYPE_F32) launch_of<float>(a, e.h_dtype == ERI_DTYPE_F32, shape, s);
@@ -235,7 +280,7 @@ int launch_rms_norm_grad(const EriRmsNormGrad &e, const Drop &d, uint32_t comput
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return (int)err;
     }
-    if (e.grad_weight)
+    if (e.grad_weight && !few)
         hipLaunchKernelGGL(rms_norm_grad_weight_kernel, dim3(padded / 64), dim3(1024), 0, s, partial, shape.groups, padded, e.grad_weight,
                            (uint32_t)e.cols, (uint32_t)(e.grad_weight_dtype == ERI_DTYPE_F32));
     return (int)hipGetLastError();

@@ -71,7 +71,7 @@ def rms_norm(x: Tensor, weight: Optional[Tensor] = None, eps: float = 1e-6, *, r
     for each 128 columns of it with scale_group=128, so that y * scale is the norm's output.  h has the residual's dtype."""
     got = _layers_face.rms_norm(x, weight, eps, residual, p, seed, offset, dtype, scale_group)
     if got is not None:
-        return RmsNorm(*got)
+        return RmsNorm._make(got)
     if residual is None and p == 0:
         y, rstd = _RmsNorm.apply(x, weight, None, eps, 0.0, 0, 0, dtype)
         return RmsNorm(y, x, rstd, None)
@@ -85,7 +85,7 @@ def rms_norm_grad(grad: Tensor, h: Tensor, rstd: Tensor, weight: Optional[Tensor
     """Gradients of rms_norm's x, residual and weight (`needs`: which of them) from that of y, and grad_h, what reaches h
     besides the norm.  h and rstd are what rms_norm returned; dtype is x's (grad's by default), weight's gradient has weight's
     dtype.  The same inputs give the same bits."""
-    return RmsNormGrad(*_layers_face.rms_norm_grad(grad, h, rstd, weight, grad_h, p, seed, offset, dtype, needs))
+    return RmsNormGrad._make(_layers_face.rms_norm_grad(grad, h, rstd, weight, grad_h, p, seed, offset, dtype, needs))
 
 
 class _Embedding(torch.autograd.Function):

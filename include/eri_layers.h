@@ -52,7 +52,7 @@ typedef struct EriEmbeddingGrad {
     const void *ids;
     const void *grad; /* tokens rows of dim elements */
     void *out;        /* vocab rows of dim elements */
-    void *workspace;  /* 16-byte aligned, eri_embedding_grad_workspace() bytes */
+    void *workspace;  /* 16-byte aligned, eri_embedding_grad_workspace() bytes; few tokens need none */
     uint64_t workspace_bytes;
     uint64_t tokens, vocab, dim;
     uint64_t grad_stride, out_stride;

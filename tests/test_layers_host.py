@@ -103,9 +103,10 @@ def test_refusals_of_the_tables_gradient():
     need = C.c_uint64()
     fn = L.lib().eri_embedding_grad_workspace
     fn.restype, fn.argtypes = C.c_int, [C.c_uint64] * 3 + [C.c_void_p]
-    assert fn(4, 8, 16, C.byref(need)) == 0 and need.value > 0
+    assert fn(4, 8, 16, C.byref(need)) == 0 and need.value == 0  # few tokens need none
+    assert fn(4000, 8, 16, C.byref(need)) == 0 and need.value > 0
     assert fn(4, 8, 16, None) == NULL and fn(4, 0, 16, C.byref(need)) == EMPTY and fn(2 ** 31, 8, 16, C.byref(need)) == TOO_LARGE
-    base = dict(ids=0x1000, grad=0x2000, out=0x3000, workspace=0x4000, workspace_bytes=need.value, tokens=4, vocab=8, dim=16, padding_id=-1, ids_64=0,
+    base = dict(ids=0x1000, grad=0x2000, out=0x3000, workspace=0x4000, workspace_bytes=need.value, tokens=4000, vocab=8, dim=16, padding_id=-1, ids_64=0,
                 grad_dtype=BF16, out_dtype=F32, scale=1.0)
     assert _refused("eri_embedding_grad", None) == NULL
     for code, change in [(NULL, dict(ids=0)), (NULL, dict(grad=0)), (NULL, dict(out=0)), (NULL, dict(workspace=0)), (ALIGN, dict(ids=0x1002)),
