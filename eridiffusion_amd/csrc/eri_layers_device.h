@@ -187,28 +187,38 @@ __device__ __forceinline__ float wave_max(float v) { // of values >= 0
     return fmaxf(fmaxf(lane_of(v, 0), lane_of(v, 16)), fmaxf(lane_of(v, 32), lane_of(v, 48)));
 }
 
-/* Over the WAVES waves of a workgroup through `slots` (WAVES floats).  The caller alternates between two arrays of slots
- * from one call to the next: a wave that is a call ahead must not overwrite what a slower one still reads. */
-template <int WAVES> __device__ __forceinline__ float group_sum(float v, float *slots) {
+/* Over T threads that stand side by side: 16, 32, a wave, or the waves of a workgroup through `slots` (a float for each).  The caller
+ * alternates between two arrays of slots from one call to the next: a wave that is a call ahead must not overwrite
+ * what a slower one still reads. */
+template <int T> constexpr int kSlots = T > (int)kWave ? T / (int)kWave : 1;
+template <int T> __device__ __forceinline__ float sum_over(float v, float *slots) {
+    if (T == 16) return row16_sum(v);
+    if (T == 32) {
+        v = row16_sum(v);
+        return v + __shfl_xor(v, 16);
+    }
     v = wave_sum(v);
-    if (WAVES == 1) return v;
-    const uint32_t wave = threadIdx.x / kWave;
-    if (threadIdx.x % kWave == 0) slots[wave] = v;
+    if (T == kWave) return v;
+    if (threadIdx.x % kWave == 0) slots[threadIdx.x / kWave] = v;
     __syncthreads();
     float s = slots[0];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) s += slots[w];
+    for (int w = 1; w < kSlots<T>; ++w) s += slots[w];
     return s;
 }
-template <int WAVES> __device__ __forceinline__ float group_max(float v, float *slots) {
+template <int T> __device__ __forceinline__ float max_over(float v, float *slots) { // of values >= 0
+    if (T == 16) return row16_max(v);
+    if (T == 32) {
+        v = row16_max(v);
+        return fmaxf(v, __shfl_xor(v, 16));
+    }
     v = wave_max(v);
-    if (WAVES == 1) return v;
-    const uint32_t wave = threadIdx.x / kWave;
-    if (threadIdx.x % kWave == 0) slots[wave] = v;
+    if (T == kWave) return v;
+    if (threadIdx.x % kWave == 0) slots[threadIdx.x / kWave] = v;
     __syncthreads();
     float s = slots[0];
 #pragma unroll
-    for (int w = 1; w < WAVES; ++w) s = fmaxf(s, slots[w]);
+    for (int w = 1; w < kSlots<T>; ++w) s = fmaxf(s, slots[w]);
     return s;
 }
 

@@ -92,10 +92,9 @@ __device__ __forceinline__ float most_of(const float (&v)[8]) {
 /* A row to TPR threads, NV vectors of eight elements in the registers of each. */
 template <typename TX, typename TR, bool RES, bool DROP, int TPR, int NV, bool SHORT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const NormArgs a) {
-    constexpr int kWaves = TPR / kWave;
-    __shared__ float slots[2][kWaves < 2 ? 1 : kWaves];
+    __shared__ float slots[2][kSlots<TPR>];
     const uint32_t row = a.first + blockIdx.x * rows_of(TPR) + threadIdx.x / TPR, t = threadIdx.x % TPR;
-    if (row >= a.rows) return; // a whole wave, and only where a row is one wave's
+    if (row >= a.rows) return; // all threads of the row, and only where none of them waits for others
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
     Raw<TX> x[NV];
     Raw<TR> r[NV];
@@ -113,7 +112,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(h[k][e], h[k][e], sum);
     }
-    const float rstd = 1.0f / sqrtf(group_sum<kWaves>(sum, slots[0]) / (float)a.cols + a.eps);
+    const float rstd = 1.0f / sqrtf(sum_over<TPR>(sum, slots[0]) / (float)a.cols + a.eps);
     if (a.rstd && t == 0) a.rstd[row] = rstd;
     float most = 0.0f;
 #pragma unroll
@@ -129,7 +128,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const N
         } else most = fmaxf(most, most_of(h[k]));
     }
     if (a.y_dtype == ERI_DTYPE_F8E4M3 && !a.group) {
-        most = group_max<kWaves>(most, slots[1]);
+        most = max_over<TPR>(most, slots[1]);
 #pragma unroll
         for (int k = 0; k < NV; ++k) store_scaled(a, row, (k * TPR + t) * 8, h[k], most);
         if (t == 0) a.scales[row] = scale_of(most);
@@ -156,7 +155,7 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(h[e], h[e], sum);
     }
-    const float rstd = 1.0f / sqrtf(group_sum<16>(sum, slots[0]) / (float)a.cols + a.eps);
+    const float rstd = 1.0f / sqrtf(sum_over<1024>(sum, slots[0]) / (float)a.cols + a.eps);
     float most = 0.0f;
     if (a.y_dtype == ERI_DTYPE_F8E4M3 && !a.group) {
         for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
@@ -165,7 +164,7 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
             weigh<false>(h, a, col, rstd);
             most = fmaxf(most, most_of(h));
         }
-        most = group_max<16>(most, slots[1]);
+        most = max_over<1024>(most, slots[1]);
         if (threadIdx.x == 0) a.scales[row] = scale_of(most);
     }
     if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
@@ -189,7 +188,9 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
 template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormArgs &a, uint32_t compute_units, hipStream_t s) {
 #define ERI_NORM(TPR, NV, SHORT) \
     hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV, SHORT>), dim3((a.rows - a.first + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
-    if (a.cols < 8) ERI_NORM(64, 1, true);
+    if (a.cols < 8) ERI_NORM(16, 1, true);
+    else if (a.cols <= 128) ERI_NORM(16, 1, false);
+    else if (a.cols <= 256) ERI_NORM(32, 1, false);
     else if (a.cols <= 512) ERI_NORM(64, 1, false);
     else if (a.cols <= 1024) ERI_NORM(64, 2, false);
     else if (a.cols <= 2048) ERI_NORM(64, 4, false);

@@ -65,8 +65,7 @@ template <typename TG, typename TR, bool SHORT, int THREADS> __device__ __forcei
 /* A row at a time to TPR threads, which keep the weight and their columns' sums of grad_weight in registers. */
 template <typename TG, typename TR, bool DROP, int TPR, int NV, bool SHORT>
 __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(const NormGradArgs a) {
-    constexpr int kWaves = TPR / kWave;
-    __shared__ float slots[2][kWaves < 2 ? 1 : kWaves];
+    __shared__ float slots[2][kSlots<TPR>];
     __shared__ float joined[TPR < 256 ? TPR * NV * 8 : 1];
     if (blockIdx.x >= a.row_groups) return weight_of_columns<TG, TR, SHORT, TPR < 256 ? 256 : TPR>(a, blockIdx.x - a.row_groups);
     const uint32_t t = threadIdx.x % TPR;
@@ -110,7 +109,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(co
                 acc[k][e] = fmaf(gh, rstd, acc[k][e]);
             }
         }
-        c = group_sum<kWaves>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
+        c = sum_over<TPR>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             float dh[8];
@@ -139,7 +138,8 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(co
     for (int k = 0; k < NV; ++k) store8(out, (k * TPR + t) * 8, a.padded, acc[k]);
 }
 
-/* Rows too long for registers: read twice, and the sums of grad_weight kept in the workgroup's row of partial. */
+/* Rows too long for registers (with 32 elements of four rows in each of 1024 threads the compiler spills 200 of them, and 4096 x 20000
+ * bf16 took 535 us; this takes 254): read twice, and the sums of grad_weight kept in the workgroup's row of partial. */
 template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(const NormGradArgs a) {
     __shared__ float slots[2][16];
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
@@ -170,7 +170,7 @@ template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024
                 store8(out, col, a.padded, old);
             }
         }
-        c = group_sum<16>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
+        c = sum_over<1024>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
         for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
             Raw<TG> g;
             Raw<TR> h, r;
@@ -227,8 +227,8 @@ struct Shape {
     uint32_t groups;
 };
 Shape shape_of(uint64_t rows, uint64_t cols, uint32_t compute_units) {
-    Shape s = cols <= 512 ? Shape{64, 1, 0} : cols <= 1024 ? Shape{64, 2, 0} : cols <= 2048 ? Shape{256, 1, 0} : cols <= 4096 ? Shape{256, 2, 0} :
-              cols <= 8192 ? Shape{256, 4, 0} : cols <= 16384 ? Shape{1024, 2, 0} : cols <= 32768 ? Shape{1024, 4, 0} : Shape{1024, 0, 0};
+    Shape s = cols <= 128 ? Shape{16, 1, 0} : cols <= 256 ? Shape{32, 1, 0} : cols <= 512 ? Shape{64, 1, 0} : cols <= 1024 ? Shape{64, 2, 0} : cols <= 2048 ? Shape{256, 1, 0} : cols <= 4096 ? Shape{256, 2, 0} :
+              cols <= 8192 ? Shape{256, 4, 0} : cols <= 16384 ? Shape{1024, 2, 0} : Shape{1024, 0, 0};
     const uint64_t all = (rows + kRowsOf(s.tpr) - 1) / kRowsOf(s.tpr), most = (uint64_t)compute_units * (s.tpr == 1024 ? 1 : 2); // more of them leave more sums to read again: with 4, 3-15 % slower
     s.groups = (uint32_t)(all < most ? all : most);
     return s;
@@ -240,14 +240,15 @@ template <typename TG, typename TR, bool DROP> void launch(const NormGradArgs &a
 #define ERI_NORM_GRAD(TPR, NV, SHORT) \
     if (shape.tpr == TPR && shape.nv == NV && SHORT == (a.cols < 8)) \
     hipLaunchKernelGGL((rms_norm_grad_kernel<TG, TR, DROP, TPR, NV, SHORT>), dim3(groups), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
-    ERI_NORM_GRAD(64, 1, true);
+    ERI_NORM_GRAD(16, 1, true);
+    ERI_NORM_GRAD(16, 1, false);
+    ERI_NORM_GRAD(32, 1, false);
     ERI_NORM_GRAD(64, 1, false);
     ERI_NORM_GRAD(64, 2, false);
     ERI_NORM_GRAD(256, 1, false);
     ERI_NORM_GRAD(256, 2, false);
     ERI_NORM_GRAD(256, 4, false);
     ERI_NORM_GRAD(1024, 2, false);
-    ERI_NORM_GRAD(1024, 4, false);
 #undef ERI_NORM_GRAD
     if (shape.nv == 0) hipLaunchKernelGGL((rms_norm_grad_long_kernel<TG, TR, DROP>), dim3(shape.groups), dim3(1024), 0, s, a);
 }
