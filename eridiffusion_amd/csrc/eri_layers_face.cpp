@@ -164,6 +164,16 @@ void *stream_of(const at::Tensor &t) {
     return s;
 }
 
+/* A given output, which is written in place: autograd has to know that its values change. */
+const at::Tensor &written(PyObject *o, const char *name, const at::Tensor &beside) {
+    const at::Tensor &t = floats(o, name, &beside);
+    ERI_VALUE(!records(t), std::string(name) + " requires a gradient itself");
+    return t;
+}
+void changed(const at::Tensor &t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 /* Ids are read as they lie, 32 or 64 bits each. */
 at::Tensor ids_of(PyObject *o) {
     const at::Tensor &t = tensor(o, "ids");
@@ -213,7 +223,7 @@ PyObject *embedding(PyObject *const *args) {
     Outputs made;
     made.guard.reset_device(weight.device());
     const auto shape = with_last(ids.sizes(), weight.size(1));
-    const Rows out(args[3] == Py_None ? made.empty(shape, weight.scalar_type(), weight) : floats(args[3], "out", &weight), "out");
+    const Rows out(args[3] == Py_None ? made.empty(shape, weight.scalar_type(), weight) : written(args[3], "out", weight), "out");
     ERI_VALUE(out.t.sizes() == at::IntArrayRef(shape) && out.t.scalar_type() == weight.scalar_type(), "out has another shape or dtype than the rows");
     a.ids = ids.const_data_ptr();
     a.table = table.t.const_data_ptr();
@@ -225,6 +235,7 @@ PyObject *embedding(PyObject *const *args) {
     a.out_stride = out.stride;
     a.ids_64 = ids.scalar_type() == at::kLong;
     a.dtype_tag = tag_of(weight.scalar_type());
+    changed(out.t);
     check(eri_embedding(&a, stream_of(weight)), "eri_embedding");
     return args[3] == Py_None ? wrapped(out.t) : Py_NewRef(args[3]);
 }
@@ -257,9 +268,8 @@ PyObject *embedding_grad(PyObject *const *args) {
     Outputs made;
     made.guard.reset_device(grad.device());
     const std::vector<int64_t> shape = {(int64_t)vocab, grad.size(-1)};
-    const Rows out(args[6] == Py_None ? made.empty(shape, dtype, grad) : floats(args[6], "out", &grad), "out");
+    const Rows out(args[6] == Py_None ? made.empty(shape, dtype, grad) : written(args[6], "out", grad), "out");
     ERI_VALUE(out.t.sizes() == at::IntArrayRef(shape) && (args[5] == Py_None || out.t.scalar_type() == dtype), "out has another shape or dtype than the gradient");
-    ERI_VALUE(!records(out.t), "out requires a gradient itself");
     const Rows rows(grad);
     check(eri_embedding_grad_workspace((uint64_t)ids.numel(), vocab, (uint64_t)grad.size(-1), &a.workspace_bytes), "eri_embedding_grad_workspace");
     const at::Tensor workspace = made.empty({(int64_t)a.workspace_bytes}, at::kByte, grad);
@@ -276,6 +286,7 @@ PyObject *embedding_grad(PyObject *const *args) {
     a.grad_dtype = tag_of(grad.scalar_type());
     a.out_dtype = tag_of(out.t.scalar_type());
     a.accumulate = accumulate;
+    changed(out.t);
     check(eri_embedding_grad(&a, stream_of(grad)), "eri_embedding_grad");
     return args[6] == Py_None ? wrapped(out.t) : Py_NewRef(args[6]);
 }
@@ -292,7 +303,7 @@ PyObject *dropout(PyObject *const *args) {
     const Rows x(given);
     Outputs made;
     made.guard.reset_device(given.device());
-    const Rows out(args[4] == Py_None ? made.empty(given.sizes(), given.scalar_type(), given) : floats(args[4], "out", &given), "out");
+    const Rows out(args[4] == Py_None ? made.empty(given.sizes(), given.scalar_type(), given) : written(args[4], "out", given), "out");
     ERI_VALUE(out.t.sizes() == given.sizes() && out.t.scalar_type() == given.scalar_type(), "out has another shape or dtype than x");
     a.x = x.t.const_data_ptr();
     a.y = out.t.data_ptr();
@@ -301,6 +312,7 @@ PyObject *dropout(PyObject *const *args) {
     a.x_stride = x.stride;
     a.y_stride = out.stride;
     a.dtype_tag = tag_of(given.scalar_type());
+    changed(out.t);
     check(eri_dropout(&a, stream_of(given)), "eri_dropout");
     return args[4] == Py_None ? wrapped(out.t) : Py_NewRef(args[4]);
 }

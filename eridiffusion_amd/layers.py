@@ -39,6 +39,8 @@ def embedding(ids: Tensor, weight: Tensor, scale: float = 1.0, *, out: Optional[
     """scale * weight[ids], of shape ids.shape + (dim,); a row of zeros for an id outside the table.
 
     Rows named padding_id are looked up like others, but get no gradient."""
+    if padding_id is not None and not 0 <= padding_id < weight.shape[0]:
+        raise ValueError("padding_id is no row of the table")
     rows = _layers_face.embedding(ids, weight, scale, out)
     return _Embedding.apply(ids, weight, scale, padding_id) if rows is None else rows
 

@@ -478,6 +478,53 @@ def test_autograd_takes_what_is_needed(layers):
         y.float().sum().backward()
 
 
+def test_outputs_that_are_given_count_as_changed(layers):
+    """A value that autograd has saved is not overwritten unnoticed, and a parameter is no output."""
+    x = _new(6, 40).cuda()
+    w = _new(40).cuda().requires_grad_()
+    loss = (x * w).sum()
+    layers.dropout(x, 0.5, 1, out=x)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    ids = torch.zeros(6, dtype=torch.long, device="cuda")
+    p = torch.nn.Parameter(x.clone())
+    for call in [lambda: layers.dropout(x, 0.5, 1, out=p), lambda: layers.embedding(ids, x, out=p), lambda: layers.embedding_grad(ids, x, 6, out=p),
+                 lambda: layers.embedding(ids, p, out=x), lambda: layers.dropout(p, 0.5, 1, out=x), lambda: layers.embedding(ids, x, padding_id=6)]:
+        with pytest.raises(ValueError):
+            call()
+    with torch.no_grad():
+        assert torch.equal(layers.dropout(x, 0.5, 1, out=p), layers.dropout(x, 0.5, 1))
+    with torch.inference_mode():
+        y = torch.zeros(6, 40, device="cuda")
+        assert torch.equal(layers.dropout(x, 0.5, 1, out=y), layers.dropout(x, 0.5, 1))
+
+
+def test_norm_and_its_gradient_past_32_bit_offsets(layers):
+    rows, cols = 2 ** 18 + 3, 16390  # 2^32 elements and more
+    x = torch.zeros(rows, cols, dtype=BF, device="cuda")
+    at = torch.tensor([0, 1, 2 ** 17, 2 ** 18 - 1, 2 ** 18 + 2])
+    some, w = _new(5, cols, dtype=BF), _new(cols, dtype=BF, std=0.3, mean=1.0)
+    x[at.cuda()] = some.cuda()
+    r = layers.rms_norm(x, w.cuda(), 1e-6, p=0.5, seed=3)
+    first = [int(i) * cols for i in at]
+    keep = []
+    for f in first:
+        words = of.philox(np.arange(f // 8, (f + cols) // 8 + 1, dtype=np.uint64), 3, 0)
+        bits = np.stack((words & np.uint64(0xFFFF), words >> np.uint64(16)), 2).reshape(-1)[f % 8:f % 8 + cols]
+        keep.append(torch.from_numpy(np.where(bits >= 32768, 2.0, 0.0)))
+    keep = torch.stack(keep)
+    h = some.double() * keep
+    rstd = 1 / torch.sqrt((h * h).mean(-1) + 1e-6)
+    y = h * rstd[:, None] * w.double()
+    _near(r.h[at.cuda()], h, U[BF] * h.abs())
+    _near(r.y[at.cuda()], y, U[BF] * y.abs() + U32 * (_depth(cols) + 8) * y.abs())
+    g = layers.rms_norm_grad(r.y, r.h, r.rstd, w.cuda(), p=0.5, seed=3, needs=(True, False, True))
+    y, h, q = r.y[at.cuda()].cpu(), r.h[at.cuda()].cpu(), r.rstd[at.cuda()].cpu()
+    _, dh, dw, size, size_w = of.rms_norm_grad(y, h, q, w)
+    _near(g.x[at.cuda()], dh * keep, U[BF] * (dh * keep).abs() + 2 * U32 * (_depth(cols) + 12) * size)
+    _near(g.weight, dw, U[BF] * dw.abs() + U32 * 800 * size_w)  # five rows' terms, and zeros, in sums of at most 513 + 130
+
+
 def test_on_another_stream(layers):
     """Work queued on a side stream, its inputs made there: the calls follow it."""
     s = torch.cuda.Stream()
@@ -527,3 +574,16 @@ def test_a_captured_training_pass_replays(layers):
         torch.cuda.synchronize()
         want, want_n = step()
         assert torch.equal(first, want) and torch.equal(second, want_n), k
+
+
+def test_the_example_learns():
+    import importlib.util
+    import os
+
+    from test_layers_host import ROOT
+    spec = importlib.util.spec_from_file_location("train_tokens", os.path.join(ROOT, "examples", "train_tokens.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    losses = example.train(steps=30, log=None)
+    assert abs(losses[0] - np.log(example.VOCAB)) < 1 and losses[-1] < 0.5 * losses[0] and all(np.isfinite(losses))
+    assert losses[0] == example.train(steps=1, log=None)[0]
