@@ -71,11 +71,11 @@ template <typename T> void launch_lookup_of(const LookupArgs &a, uint32_t comput
 // ---------------------------------------------------------------------------------------------
 
 /*
- * Sorting: ids are dealt to K = 2^shift buckets by their low bits, a workgroup to a bucket.  It reads all ids twice, in
- * order: the first time it counts its own ones, each wave for its share of the tokens; the second time it writes the
- * tokens of each of its ids, in ascending order, to its part of the sorted list.  Where that part begins, it has counted
- * too, as the number of tokens in the buckets before it: no workgroup waits for another.  Between the two it writes the
- * rows that no token names: stores that nothing waits for.
+ * Sorting: ids are dealt to K = 2^shift buckets by their low bits, a workgroup to a bucket.  It reads all ids, in order and
+ * each wave its share of them, counts its own ones and keeps their tokens; then it writes the tokens of each of its ids, in
+ * ascending order, to its part of the sorted list.  Where that part begins, it has counted too, as the number of tokens
+ * in the buckets before it: no workgroup waits for another.  Between the two it writes the rows that no token names:
+ * stores that nothing waits for.
  *
  * Summing: the runs of equal ids in the sorted list are cut into pieces of 2^log_piece tokens, and a wave sums the pieces that
  * begin in its step of half as many places, for L*8 columns: its loads go ahead through the list whatever the lengths of the
@@ -84,6 +84,7 @@ template <typename T> void launch_lookup_of(const LookupArgs &a, uint32_t comput
  */
 constexpr uint32_t kWaves = 16;       // of a bucket's workgroup
 constexpr uint32_t kLocalMost = 1024; // ids of a bucket
+constexpr uint32_t kOwnMost = 512;    // tokens of a bucket that a wave keeps from the first look to the second
 constexpr uint32_t kLogPieceMost = 5;
 constexpr uint32_t kListMost = (1 << kLogPieceMost) * 3 / 2; // places that a step and the piece that it ends with take
 
@@ -115,23 +116,37 @@ __device__ __forceinline__ uint64_t slot_of(uint32_t start, bool first, uint32_t
 __global__ __launch_bounds__(1024) void embedding_sort_kernel(const GradArgs a) {
     extern __shared__ uint32_t counts[]; // kWaves x locals: first counts, then where the wave's next token of that id goes
     __shared__ uint32_t starts[kLocalMost], lengths[kLocalMost], part[kWaves], before[kWaves];
+    __shared__ uint32_t own_token[kWaves][kOwnMost];
+    __shared__ uint16_t own_local[kWaves][kOwnMost];
     const uint32_t bucket = blockIdx.x, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, mask = (1u << a.shift) - 1;
     for (uint32_t i = threadIdx.x; i < kWaves * a.locals; i += 1024) counts[i] = 0;
     __syncthreads();
 
-    // count
+    // count, and keep the bucket's own tokens: the first kOwnMost that a wave finds in its share
     const uint32_t share = (a.tokens + kWaves * kWave - 1) / (kWaves * kWave) * kWave;
     const uint32_t from = wave * share, to = from + share < a.tokens ? from + share : a.tokens;
-    uint32_t *mine = counts + wave * a.locals, lower = 0;
-#pragma unroll 4
-    for (uint32_t t = from + lane; t < to; t += kWave) {
-        const int64_t id = a.ids[t];
-        const bool use = a.counts(id);
-        const uint32_t b = (uint32_t)id & mask;
-        if (use && b == bucket) atomicAdd(&mine[(uint32_t)id >> a.shift], 1u);
-        lower += use && b < bucket;
+    uint32_t *mine = counts + wave * a.locals, lower = 0, found = 0;
+    constexpr uint32_t kIds = 8; // of a lane, under way together
+    for (uint32_t set = from; set < to; set += kIds * kWave) {
+        int64_t ids[kIds];
+#pragma unroll
+        for (uint32_t k = 0; k < kIds; ++k) {
+            const uint32_t t = set + k * kWave + lane;
+            ids[k] = a.ids[t < to ? t : to - 1];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < kIds; ++k) {
+            const uint32_t t = set + k * kWave + lane, id = (uint32_t)ids[k], b = id & mask;
+            const bool use = t < to && a.counts(ids[k]), own = use && b == bucket;
+            lower += (uint32_t)__popcll(__ballot(use && b < bucket));
+            const uint64_t all = __ballot(own);
+            if (!all) continue;
+            const uint32_t n = found + (uint32_t)__popcll(all & ((1ull << lane) - 1));
+            if (own) atomicAdd(&mine[id >> a.shift], 1u);
+            if (own && n < kOwnMost) own_token[wave][n] = t, own_local[wave][n] = (uint16_t)(id >> a.shift);
+            found += (uint32_t)__popcll(all);
+        }
     }
-    for (int d = 1; d < 64; d *= 2) lower += __shfl_xor(lower, d);
     if (lane == 0) before[wave] = lower;
     __syncthreads();
 
@@ -179,32 +194,40 @@ __global__ __launch_bounds__(1024) void embedding_sort_kernel(const GradArgs a) 
 
     // the list: each wave for its share; of several tokens in one step, an id at a time
     if (all_mine == 0) return;
-    constexpr uint32_t kIds = 4;
-    for (uint32_t four = from; four < to; four += kIds * kWave) {
+    auto put = [&](bool own, uint32_t token, uint32_t local_of) {
+        const uint32_t start_of = starts[own ? local_of : 0], run_of = lengths[own ? local_of : 0];
+        for (uint64_t left = __ballot(own); left;) {
+            const uint32_t local = (uint32_t)__builtin_amdgcn_readlane((int)local_of, __builtin_ctzll(left));
+            const bool same = own && local_of == local;
+            const uint64_t all = __ballot(same);
+            uint32_t place = 0;
+            if (lane == 0) place = atomicAdd(&mine[local], (uint32_t)__popcll(all));
+            place = (uint32_t)__builtin_amdgcn_readfirstlane((int)place);
+            if (same) {
+                place += (uint32_t)__popcll(all & ((1ull << lane) - 1));
+                a.sorted[place] = Place{token, local << a.shift | bucket, place - start_of, run_of};
+            }
+            left &= ~all;
+        }
+    };
+    if (found <= kOwnMost) {
+        for (uint32_t at = 0; at < found; at += kWave) {
+            const bool own = at + lane < found;
+            put(own, own ? own_token[wave][at + lane] : 0, own ? own_local[wave][at + lane] : 0);
+        }
+        return;
+    }
+    for (uint32_t set = from; set < to; set += kIds * kWave) { // more than that: a second look
         int64_t ids[kIds];
 #pragma unroll
         for (uint32_t k = 0; k < kIds; ++k) {
-            const uint32_t t = four + k * kWave + lane;
+            const uint32_t t = set + k * kWave + lane;
             ids[k] = a.ids[t < to ? t : to - 1];
         }
-#pragma unroll
+#pragma unroll 1
         for (uint32_t k = 0; k < kIds; ++k) {
-            const uint32_t t = four + k * kWave + lane, local_of = (uint32_t)ids[k] >> a.shift;
-            const bool own = t < to && a.counts(ids[k]) && ((uint32_t)ids[k] & mask) == bucket;
-            uint64_t left = __ballot(own);
-            while (left) {
-                const uint32_t local = (uint32_t)__builtin_amdgcn_readlane((int)local_of, __builtin_ctzll(left));
-                const bool same = own && local_of == local;
-                const uint64_t all = __ballot(same);
-                uint32_t place = 0;
-                if (lane == 0) place = atomicAdd(&mine[local], (uint32_t)__popcll(all));
-                place = (uint32_t)__builtin_amdgcn_readfirstlane((int)place);
-                if (same) {
-                    place += (uint32_t)__popcll(all & ((1ull << lane) - 1));
-                    a.sorted[place] = Place{t, (uint32_t)ids[k], place - starts[local], lengths[local]};
-                }
-                left &= ~all;
-            }
+            const uint32_t t = set + k * kWave + lane;
+            put(t < to && a.counts(ids[k]) && ((uint32_t)ids[k] & mask) == bucket, t, (uint32_t)ids[k] >> a.shift);
         }
     }
 }
@@ -224,7 +247,7 @@ template <bool SHORT, typename TO> __device__ __forceinline__ void finish8(const
 
 /* L lanes to a step of the list and a tile of L*8 columns.  The places of the step and of what its last piece reaches beyond it
  * come in one trip to memory, then the rows, a set of them on its way while another is added up. */
-template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const GradArgs a) {
+template <typename TG, typename TO, int L, bool ACC, bool SHORT, bool ONCE> __global__ __launch_bounds__(kThreads) void embedding_sum_kernel(const GradArgs a) {
     static_assert(kListMost <= kWave, "a lane to a place");
     __shared__ Place list[L == kWave ? 1 : kThreads / L][kListMost];
     const uint32_t piece = 1u << a.log_piece, step = piece / 2;
@@ -260,7 +283,7 @@ template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __la
     auto ends = [&](const Place &p) { return in(p) == piece - 1 || p.at + 1 == p.run; };
     // Rows on their way: as many as the registers of two such sets hold.  No load of a set hangs on a condition (the last row stands
     // in for those past the end): with a known number under way, a wait for the first of them leaves the others alone.
-    constexpr uint32_t kAhead = sizeof(TG) + (ACC ? sizeof(TO) : 0) <= 4 ? 8 : 4;
+    constexpr uint32_t kAhead = sizeof(TG) + (ACC ? sizeof(TO) : 0) <= 4 ? 4 : 2;
     struct Ahead {
         Raw<TG> grad[kAhead];
         Raw<TO> old[ACC ? kAhead : 1];
@@ -269,7 +292,7 @@ template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __la
 #pragma unroll
         for (uint32_t k = 0; k < kAhead; ++k) {
             const Place p = place(at + k < end ? at + k : end - 1);
-            load8<SHORT, true>(f.grad[k], (const TG *)a.grad + p.token * a.grad_stride, col, a.dim);
+            load8<SHORT, ONCE>(f.grad[k], (const TG *)a.grad + p.token * a.grad_stride, col, a.dim);
             if (ACC) load8<SHORT>(f.old[k], (const TO *)a.out + p.id * a.out_stride, col, a.dim);
         }
     };
@@ -310,9 +333,8 @@ template <typename TG, typename TO, int L, bool ACC, bool SHORT> __global__ __la
 }
 
 /* Runs of several pieces: a wave looks for the one that begins in its places, as many as a piece is long, and sums its pieces
- * for 512 columns.  The pieces of a long one are shared out among the four waves of the workgroup. */
-template <typename TO, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_join_kernel(const GradArgs a) {
-    constexpr uint32_t kTeam = kThreads / kWave;
+ * for 512 columns.  The pieces of a long one are shared out among the waves of the workgroup. */
+template <typename TO, bool SHORT, uint32_t kTeam> __global__ __launch_bounds__(kTeam * kWave) void embedding_join_kernel(const GradArgs a) {
     static_assert(kLogPieceMost <= 6, "a lane to a place");
     __shared__ Place runs[kTeam]; // token: where it begins
     __shared__ float sums[kTeam][512];
@@ -327,7 +349,7 @@ template <typename TO, bool SHORT> __global__ __launch_bounds__(kThreads) void e
     auto sum = [&](float (&v)[8], const Place &r, uint32_t from, uint32_t to) { // pieces of a run
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) v[e] = 0.0f;
-#pragma unroll 8
+#pragma unroll 4
         for (uint32_t k = from; k < to; ++k) {
             Raw<float> s;
             load8<false>(s, (const float *)a.partial + slot_of(r.token + (k << a.log_piece), k == 0, a.log_piece) * a.padded, col, a.padded);
@@ -344,15 +366,16 @@ template <typename TO, bool SHORT> __global__ __launch_bounds__(kThreads) void e
         sum(v, own, 0, pieces);
         finish8<SHORT, TO>(a, own.id, col, v);
     }
-    for (uint32_t w = 0; w < kTeam; ++w) { // the same for all waves
-        const Place r = runs[w];
+    // the same for all waves: longer than that
+    for (uint64_t left = __ballot(lane < kTeam && runs[lane < kTeam ? lane : 0].run > kAlone << a.log_piece); left; left &= left - 1) {
+        const Place r = runs[__builtin_ctzll(left)];
         const uint32_t n = (r.run + piece - 1) >> a.log_piece, share = (n + kTeam - 1) / kTeam;
-        if (n <= kAlone) continue;
         sum(v, r, share * wave < n ? share * wave : n, share * (wave + 1) < n ? share * (wave + 1) : n);
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) sums[wave][e * kWave + lane] = v[e];
         __syncthreads();
         if (wave == 0) {
+#pragma unroll 3
             for (uint32_t o = 1; o < kTeam; ++o)
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) v[e] += sums[o][e * kWave + lane];
@@ -514,11 +537,21 @@ template <typename TG, typename TO, int L, bool SHORT = false> void launch_sum(G
     const uint32_t piece = 1u << a.log_piece, step = piece / 2;
     const uint64_t groups = (uint64_t)((a.tokens + step - 1) / step) * a.tiles;
     const dim3 grid((uint32_t)((groups + kThreads / L - 1) / (kThreads / L)));
-    if (a.accumulate) hipLaunchKernelGGL((embedding_sum_kernel<TG, TO, L, true, SHORT>), grid, dim3(kThreads), 0, s, a);
-    else hipLaunchKernelGGL((embedding_sum_kernel<TG, TO, L, false, SHORT>), grid, dim3(kThreads), 0, s, a);
+    // Rows of grad are read once.  Where they and the table are more than the last cache holds, they go past it, so that they do not
+    // push out the zeros that were just written: sums of 32768 x 4096 bf16 after 1 GB of zeros 117 -> 84 us.  Where they fit,
+    // they may still be in it from the kernel that made them: 16384 x 1024 fp32 63 us past it, 57 through it.
+    constexpr uint64_t kLastCache = 256u << 20;
+    const bool once = L == kWave && (uint64_t)a.tokens * a.dim * sizeof(TG) + (uint64_t)a.vocab * a.dim * sizeof(TO) > kLastCache;
+    void (*const kernel)(const GradArgs) =
+        a.accumulate ? once ? embedding_sum_kernel<TG, TO, L, true, SHORT, L == kWave> : embedding_sum_kernel<TG, TO, L, true, SHORT, false>
+                     : once ? embedding_sum_kernel<TG, TO, L, false, SHORT, L == kWave> : embedding_sum_kernel<TG, TO, L, false, SHORT, false>;
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);
     if (a.tokens <= piece) return;
     a.tiles = (a.dim + 511) / 512;
-    hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT>), dim3((a.tokens + 4 * piece - 1) / (4 * piece) * a.tiles), dim3(kThreads), 0, s, a);
+    const uint32_t team = a.tokens <= 8192 ? 4 : 16; // waves for a run: the longest ones grow with the list
+    const dim3 joins((a.tokens + team * piece - 1) / (team * piece) * a.tiles);
+    if (team == 4) hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT, 4>), joins, dim3(4 * kWave), 0, s, a);
+    else hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT, 16>), joins, dim3(16 * kWave), 0, s, a);
 }
 template <typename TG, typename TO> void launch_sums(const GradArgs &a, hipStream_t s) {
     const uint32_t lanes = lanes_of(a.dim);
