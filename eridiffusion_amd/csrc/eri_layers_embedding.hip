@@ -334,7 +334,8 @@ template <typename TG, typename TO, int L, bool ACC, bool SHORT, bool ONCE> __gl
 
 /* Runs of several pieces: a wave looks for the one that begins in its places, as many as a piece is long, and sums its pieces
  * for 512 columns.  The pieces of a long one are shared out among the waves of the workgroup. */
-template <typename TO, bool SHORT, uint32_t kTeam> __global__ __launch_bounds__(kTeam * kWave) void embedding_join_kernel(const GradArgs a) {
+constexpr uint32_t kTeam = 16;
+template <typename TO, bool SHORT> __global__ __launch_bounds__(kTeam * kWave) void embedding_join_kernel(const GradArgs a) {
     static_assert(kLogPieceMost <= 6, "a lane to a place");
     __shared__ Place runs[kTeam]; // token: where it begins
     __shared__ float sums[kTeam][512];
@@ -405,7 +406,7 @@ constexpr uint32_t kFewTokens = 1024;
 constexpr uint32_t kFewLocals = 64; // rows of a bucket
 constexpr uint32_t kAloneFew = 16;
 template <typename TG, typename TO, bool ACC, bool SHORT> __global__ __launch_bounds__(kThreads) void embedding_few_kernel(const GradArgs a) {
-    constexpr uint32_t kTeam = kThreads / kWave, kEach = kFewTokens / kThreads, kAhead = 8;
+    constexpr uint32_t kTeam = kThreads / kWave, kEach = kFewTokens / kThreads, kAhead = sizeof(TG) == 2 ? 16 : 8;
     __shared__ uint32_t counts[kFewLocals], numbers[kEach * kTeam], list[kFewTokens]; // list: token << 16 | local, ascending
     __shared__ float sums[kTeam][512];
     const uint32_t bucket = blockIdx.x / a.tiles, tile = blockIdx.x - bucket * a.tiles, mask = (1u << a.shift) - 1;
@@ -445,11 +446,11 @@ template <typename TG, typename TO, bool ACC, bool SHORT> __global__ __launch_bo
             const uint32_t local = (uint32_t)__builtin_ctzll(left);
             if (local % kTeam == wave) zeros<512 * sizeof(TO)>((char *)a.out + (uint64_t)(local << a.shift | bucket) * a.out_stride * sizeof(TO), tile, lane, (uint64_t)a.dim * sizeof(TO));
         }
-    // the tokens of a row, those whose number in it is `from` or `every` more and so on
-    auto sum = [&](uint32_t local, uint32_t from, uint32_t every) {
+    // the tokens of a row, from the parts `from`, from + every and so on of the list, each of so many entries
+    auto sum = [&](uint32_t local, uint32_t from, uint32_t every, uint32_t part) {
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) v[e] = 0.0f;
-        uint32_t number = 0, n = 0, held = 0; // lane n of held: the n-th token that is under way
+        uint32_t n = 0, held = 0; // lane n of held: the n-th token that is under way
         auto flush = [&]() {
             Raw<TG> g[kAhead];
 #pragma unroll
@@ -464,10 +465,9 @@ template <typename TG, typename TO, bool ACC, bool SHORT> __global__ __launch_bo
             }
             n = 0;
         };
-        for (uint32_t at = 0; at < m; at += kWave) {
-            const uint32_t entry = at + lane < m ? list[at + lane] : 0xffffu;
-            for (uint64_t left = __ballot((entry & 0xffffu) == local); left; left &= left - 1, ++number) {
-                if (number % every != from) continue;
+        for (uint32_t at = from * part; at < m; at += every * part) {
+            const uint32_t entry = lane < part && at + lane < m ? list[at + lane] : 0xffffu;
+            for (uint64_t left = __ballot((entry & 0xffffu) == local); left; left &= left - 1) {
                 const uint32_t token = (uint32_t)__builtin_amdgcn_readlane((int)(entry >> 16), __builtin_ctzll(left));
                 held = lane == n ? token : held;
                 if (++n == kAhead) flush();
@@ -479,12 +479,12 @@ template <typename TG, typename TO, bool ACC, bool SHORT> __global__ __launch_bo
     for (uint64_t left = __ballot(length != 0 && length <= kAloneFew); left; left &= left - 1, ++turn) {
         if (turn % kTeam != wave) continue;
         const uint32_t local = (uint32_t)__builtin_ctzll(left);
-        sum(local, 0, 1);
+        sum(local, 0, 1, kWave);
         finish8<SHORT, TO>(a, local << a.shift | bucket, col, v);
     }
     for (uint64_t left = __ballot(length > kAloneFew); left; left &= left - 1) { // the same for all waves
         const uint32_t local = (uint32_t)__builtin_ctzll(left);
-        sum(local, wave, kTeam);
+        sum(local, wave, kTeam, 16);
 #pragma unroll
         for (uint32_t e = 0; e < 8; ++e) sums[wave][e * kWave + lane] = v[e];
         __syncthreads();
@@ -548,10 +548,7 @@ template <typename TG, typename TO, int L, bool SHORT = false> void launch_sum(G
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);
     if (a.tokens <= piece) return;
     a.tiles = (a.dim + 511) / 512;
-    const uint32_t team = a.tokens <= 8192 ? 4 : 16; // waves for a run: the longest ones grow with the list
-    const dim3 joins((a.tokens + team * piece - 1) / (team * piece) * a.tiles);
-    if (team == 4) hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT, 4>), joins, dim3(4 * kWave), 0, s, a);
-    else hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT, 16>), joins, dim3(16 * kWave), 0, s, a);
+    hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT>), dim3((a.tokens + kTeam * piece - 1) / (kTeam * piece) * a.tiles), dim3(kTeam * kWave), 0, s, a);
 }
 template <typename TG, typename TO> void launch_sums(const GradArgs &a, hipStream_t s) {
     const uint32_t lanes = lanes_of(a.dim);
