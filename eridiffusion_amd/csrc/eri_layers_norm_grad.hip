@@ -1,5 +1,12 @@
 /*
- * Gradient of the residual addition and root-mean-square norm of include/eri_layers.h.
+ * Gradient of the residual addition and root-mean-square norm of include/eri_layers.h:
+ *     dh = dr + q dy w - h q^3 mean(dy w h),  dx = drop(dh),  dw = sum over rows of dy h q
+ *
+ * Bound by HBM: dy, h and dr are read once, dh and dx written once; the row waits in registers for its sum, and each thread keeps
+ * the weight and the sums of dw of its columns over all rows that its workgroup takes.  The workgroups' sums (two a compute
+ * unit) are joined by a second kernel in their order, so that the same inputs give the same bits; few rows do without it.
+ * 16384 x 4096 bf16 with dropout 131 us, 5.1 TB/s (a copy of that size runs at 5.2); 1025 x 1281 fp32 7.5 + 3.5 us.
+ * Tried: the next row's loads before this row's sum (level or 1-25 % slower: the registers cost waves), four workgroups a unit.
  */
 #include "eri_layers_device.h"
 
