@@ -14,6 +14,7 @@ namespace eri_layers {
 namespace {
 
 constexpr float kF8Max = 448.0f;
+constexpr float kLeast = 0x1p-100f; // a group whose largest |y| is below this is zeros: 448 / |y| would leave fp32 not far below
 constexpr uint32_t rows_of(uint32_t tpr) { return tpr < 256 ? 256 / tpr : 1; } // of a workgroup
 
 struct NormArgs {
@@ -82,13 +83,13 @@ template <bool SHORT> __device__ __forceinline__ void weigh(float (&v)[8], const
 
 /* y / scale as 8-bit floats; `most` is the largest |y| of the group */
 __device__ __forceinline__ void store_scaled(const NormArgs &a, uint32_t row, uint32_t col, const float (&v)[8], float most) {
-    const float inv = most > 0.0f ? kF8Max / most : 1.0f;
+    const float inv = most >= kLeast ? kF8Max / most : 1.0f;
     float q[8];
 #pragma unroll
     for (uint32_t e = 0; e < 8; ++e) q[e] = v[e] * inv;
     store8_f8((uint8_t *)a.y + row * a.y_stride, col, a.cols, q);
 }
-__device__ __forceinline__ float scale_of(float most) { return most > 0.0f ? most / kF8Max : 1.0f; }
+__device__ __forceinline__ float scale_of(float most) { return most >= kLeast ? most / kF8Max : 1.0f; }
 __device__ __forceinline__ float most_of(const float (&v)[8]) {
     float m = 0.0f;
 #pragma unroll

@@ -100,8 +100,8 @@ int eri_dropout(const EriDropout *args, void *stream);
  *     h = residual + dropout(x)           rstd = 1 / sqrt(mean of h^2 over the row + eps)
  *     y = h * rstd * weight               (from h before it is rounded to its dtype)
  * with y in F32, BF16, or F8E4M3 with scales: for each row (scale_group 0) or each 128 columns of a row (scale_group
- * 128, the last group of a row may be shorter) scale = max|y| / 448, or 1 where that is 0, and the 8-bit value is
- * y / scale rounded to nearest even.  NaN is left out of max|y| and stays NaN.
+ * 128, the last group of a row may be shorter) scale = max|y| / 448, or 1 where max|y| is below 2^-100, and the 8-bit
+ * value is y / scale rounded to nearest even.  NaN is left out of max|y| and stays NaN.
  * ------------------------------------------------------------------------------------------- */
 typedef struct EriRmsNorm {
     const void *x;        /* rows of cols elements */

@@ -65,7 +65,7 @@ def scales_of(y, group):
     """The scale of each group of columns, NaN left out of the largest magnitude."""
     parts = y.split(group or y.shape[-1], -1)
     most = torch.stack([torch.nan_to_num(q.abs(), 0.0, float("inf")).amax(-1) for q in parts], -1)
-    return torch.where(most > 0, most / F8_MAX, 1.0)
+    return torch.where(most >= 2.0 ** -100, most / F8_MAX, 1.0)
 
 
 def rms_norm_grad(grad, h, rstd, weight, grad_h=None, p=0.0, seed=0, offset=0):

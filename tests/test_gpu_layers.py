@@ -196,7 +196,7 @@ def test_refusals_on_the_device(layers):
 @pytest.mark.parametrize("dtype,out", [(BF, BF), (BF, F32), (F32, F32), (F32, BF)])
 @pytest.mark.parametrize("tokens,vocab,dim,common", [
     (0, 5, 8, 0), (1, 1, 1, 0), (64, 1, 24, 0), (65, 1, 24, 0), (500, 3, 7, 0), (300, 256, 64, 0), (300, 257, 65, 0.5), (2000, 700, 130, 0.2),
-    (4097, 1023, 257, 0.1), (5000, 40, 520, 0.6), (3000, 100, 1156, 1.0), (1000, 263000, 9, 0.1), (20000, 5000, 16, 0.3)])
+    (4097, 1023, 257, 0.1), (5000, 40, 520, 0.6), (3000, 100, 1156, 1.0), (2000, 262144, 8, 0.1), (1000, 263000, 9, 0.1), (20000, 5000, 16, 0.3)])
 def test_table_gradient(layers, dtype, out, tokens, vocab, dim, common):
     ids, grad = _ids(tokens, vocab, common=common), _new(tokens, dim, dtype=dtype)
     scale = np.float32(1.7).item()
@@ -327,6 +327,29 @@ def test_norm_of_zeros_infinities_and_nan(layers, cols):
     assert torch.equal(f8.scales.isnan().cpu(), torch.zeros_like(f8.scales.cpu(), dtype=torch.bool))
     z = layers.rms_norm(torch.zeros(2, cols, device="cuda"), eps=0.0)  # 0 * infinity
     assert bool(z.y.isnan().all()) and bool(z.rstd.isinf().all())
+
+
+@pytest.mark.parametrize("group", [0, 128])
+def test_eight_bits_of_very_small_values(layers, group):
+    """Where 448 / max|y| would leave float32 the group counts as zeros; just above, it is scaled like any other."""
+    x = torch.ones(4, 300)
+    x[0], x[1], x[2, 10:] = 1e-38, 2.0 ** -110, 0
+    w = torch.full((300,), 2.0 ** -95)
+    got = layers.rms_norm(x.cuda(), w.cuda(), 1.0, dtype=F8, scale_group=group)
+    y, _, _ = of.rms_norm(x, w, 1.0)
+    scales = of.scales_of(y, group)
+    _near(got.scales, scales, 16 * U32 * scales)
+    assert bool((got.scales[:2] == 1).all()) and bool((got.y[:2].float() == 0).all())
+    assert bool((got.y[3].float() == 448).all()) and not bool(got.y.float().isnan().any())
+
+
+def test_norm_of_a_single_row_without_other_dimensions(layers):
+    x, r, w = _new(40).cuda(), _new(40, seed=1).cuda(), _new(40, seed=2).cuda()
+    got, want = layers.rms_norm(x, w, residual=r), layers.rms_norm(x[None], w, residual=r[None])
+    assert got.rstd.shape == () and torch.equal(got.y, want.y[0]) and torch.equal(got.h, want.h[0]) and torch.equal(got.rstd, want.rstd[0])
+    assert layers.rms_norm(x, w, dtype=F8).scales.shape == (1,)
+    back, rows = layers.rms_norm_grad(x, got.h, got.rstd, w), layers.rms_norm_grad(x[None], want.h, want.rstd, w)
+    assert torch.equal(back.x, rows.x[0]) and torch.equal(back.weight, rows.weight)
 
 
 def test_norm_of_strided_shaped_and_empty_inputs(layers):
