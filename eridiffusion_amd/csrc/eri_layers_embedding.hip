@@ -599,7 +599,11 @@ uint64_t embedding_grad_workspace(uint64_t tokens, uint64_t vocab, uint64_t dim)
 
 int launch_embedding_grad(const EriEmbeddingGrad &e, uint32_t, void *stream) {
     char *ws = static_cast<char *>(e.workspace);
-    const bool few = is_few(e.tokens, e.vocab, e.dim);
+    // accumulating, there are no zeros to write: one launch as long as its workgroups, most of them with nothing to do, start faster than
+    // two more launches.  300 tokens, one | three: 128000 x 1024 (4096 workgroups) 9.4 | 12.9 us, 88138 x 1272 (6144) 12.6 | 13.6,
+    // 128000 x 2048 (8192) 15.6 | 13.7
+    const bool few = is_few(e.tokens, e.vocab, e.dim) ||
+                     (e.accumulate && e.tokens <= kFewTokens && ((e.dim + 511) / 512 << shift_of(e.vocab, kFewLocals)) <= 4096);
     GradArgs a = {{e.ids, (uint32_t)e.ids_64}, e.grad, e.out, (Place *)(ws + kHead), (uint32_t *)ws, (float *)(ws + partial_at(e.tokens)),
                   (uint32_t)e.tokens, (uint32_t)e.vocab, (uint32_t)e.dim, shift_of(e.vocab, few ? kFewLocals : kLocalMost), 0, (uint32_t)padded_of(e.dim), 0,
                   log_piece_of(e.tokens, e.dim), e.grad_stride, e.out_stride, e.padding_id, e.scale, (uint32_t)(e.accumulate != 0),

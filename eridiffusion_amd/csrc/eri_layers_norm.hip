@@ -3,8 +3,11 @@
  * y = h q w, in 8 bits scaled by each group's largest |y|.
  *
  * Bound by HBM: x and r are read once, h and y written once, and the row waits in registers for its sum.  16 threads to a row of up
- * to 128 columns (a group of the 8-bit output is 16 lanes then, as it is in every layout), 32 to 256, a wave to 2048 and no barrier
- * that far, then 256 and 1024 threads.  Narrow rows on whole waves ran at a third: 100000 x 128 bf16 28 us, now 11.
+ * to 128 columns (a group of the 8-bit output is 16 lanes then, as it is in every layout), 32 to 256, a wave to 1024 and no
+ * barrier that far, then as many threads as the row has vectors of eight, to two or four each in the longest.  Narrow rows on
+ * whole waves ran at a third: 100000 x 128 bf16 28 us, now 11.  Fewer threads with more of the row each, us for 8192 rows:
+ *   2048 bf16 64 threads 22.4, 256 21.2;   4096 bf16 64 50.9, 256 42.6, 512 42.2;   4096 fp32 64 109, 256 97.8, 512 93.4;
+ *   5120 bf16 256 62.8, 512 61.1, 1024 64.4;   8192 bf16 256 96.7, 512 94.6, 1024 91.4;   1000 bf16 128 12.4, 64 11.9
  * Dropout is drawn beside the loads and costs nothing: 16384 x 4096 bf16 with residual and dropout 95 us, 5.7 TB/s (a copy of that
  * size runs at 5.2); 8192 x 5120 to 8 bits 56-60 us, 4.9-5.3 TB/s; one row of 4096 2.8 us, a launch and two trips to memory.
  */
@@ -15,7 +18,7 @@ namespace {
 
 constexpr float kF8Max = 448.0f;
 constexpr float kLeast = 0x1p-100f; // a group whose largest |y| is below this is zeros: 448 / |y| would leave fp32 not far below
-constexpr uint32_t rows_of(uint32_t tpr) { return tpr < 256 ? 256 / tpr : 1; } // of a workgroup
+constexpr uint32_t rows_of(uint32_t tpr) { return tpr <= kWave ? 256 / tpr : 1; } // of a workgroup
 
 struct NormArgs {
     const void *x, *residual, *weight;
@@ -99,7 +102,7 @@ __device__ __forceinline__ float most_of(const float (&v)[8]) {
 
 /* A row to TPR threads, NV vectors of eight elements in the registers of each. */
 template <typename TX, typename TR, bool RES, bool DROP, int TPR, int NV, bool SHORT>
-__global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_kernel(const NormArgs a) {
+__global__ __launch_bounds__(TPR * rows_of(TPR)) void rms_norm_kernel(const NormArgs a) {
     __shared__ float slots[2][kSlots<TPR>];
     const uint32_t row = a.first + blockIdx.x * rows_of(TPR) + threadIdx.x / TPR, t = threadIdx.x % TPR;
     if (row >= a.rows) return; // all threads of the row, and only where none of them waits for others
@@ -195,15 +198,16 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
 
 template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormArgs &a, uint32_t compute_units, hipStream_t s) {
 #define ERI_NORM(TPR, NV, SHORT) \
-    hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV, SHORT>), dim3((a.rows - a.first + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR < 256 ? 256 : TPR), 0, s, a)
+    hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV, SHORT>), dim3((a.rows - a.first + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR * rows_of(TPR)), 0, s, a)
     if (a.cols < 8) ERI_NORM(16, 1, true);
     else if (a.cols <= 128) ERI_NORM(16, 1, false);
     else if (a.cols <= 256) ERI_NORM(32, 1, false);
     else if (a.cols <= 512) ERI_NORM(64, 1, false);
     else if (a.cols <= 1024) ERI_NORM(64, 2, false);
-    else if (a.cols <= 2048) ERI_NORM(64, 4, false);
-    else if (a.cols <= 4096) ERI_NORM(256, 2, false);
-    else if (a.cols <= 8192) ERI_NORM(256, 4, false);
+    else if (a.cols <= 2048) ERI_NORM(256, 1, false);
+    else if (a.cols <= 4096) ERI_NORM(512, 1, false);
+    else if (a.cols <= 6144) ERI_NORM(512, 2, false);
+    else if (a.cols <= 8192) ERI_NORM(1024, 1, false);
     else if (a.cols <= 16384) ERI_NORM(1024, 2, false);
     else if (a.cols <= 32768) ERI_NORM(1024, 4, false);
     else hipLaunchKernelGGL((rms_norm_long_kernel<TX, TR, RES, DROP>), dim3(a.rows - a.first), dim3(1024), 0, s, a);

@@ -228,14 +228,16 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_weight_kernel(const float 
  *   8192 fp32    5.8 | 10.5  17.6 | 20.1  28.6 | 26.1  34.0 | 31.4  48.3 | 42.2 */
 bool is_few(uint64_t rows, uint64_t cols) { return rows <= (cols <= 512 ? 1536 : 768); }
 
-/* Threads to a row, and how many workgroups the rows are dealt to. */
+/* Threads to a row, and how many workgroups the rows are dealt to.  512 threads to a row of 2049 to 8192 columns: with 256 and twice
+ * as much of it each, 2048 x 4096 bf16 took 18.2 us for 17.1, 2048 x 8192 30.1 for 28.0, 256 x 8192 7.6 for 6.8; with 1024 to a row of
+ * 8192 26.5, but 256 rows 9.4. */
 struct Shape {
     int tpr, nv; // nv 0: rows too long for registers
     uint32_t groups;
 };
 Shape shape_of(uint64_t rows, uint64_t cols, uint32_t compute_units) {
-    Shape s = cols <= 128 ? Shape{16, 1, 0} : cols <= 256 ? Shape{32, 1, 0} : cols <= 512 ? Shape{64, 1, 0} : cols <= 1024 ? Shape{64, 2, 0} : cols <= 2048 ? Shape{256, 1, 0} : cols <= 4096 ? Shape{256, 2, 0} :
-              cols <= 8192 ? Shape{256, 4, 0} : cols <= 16384 ? Shape{1024, 2, 0} : Shape{1024, 0, 0};
+    Shape s = cols <= 128 ? Shape{16, 1, 0} : cols <= 256 ? Shape{32, 1, 0} : cols <= 512 ? Shape{64, 1, 0} : cols <= 1024 ? Shape{64, 2, 0} : cols <= 2048 ? Shape{256, 1, 0} : cols <= 4096 ? Shape{512, 1, 0} :
+              cols <= 8192 ? Shape{512, 2, 0} : cols <= 16384 ? Shape{1024, 2, 0} : Shape{1024, 0, 0};
     const uint64_t all = (rows + kRowsOf(s.tpr) - 1) / kRowsOf(s.tpr), most = (uint64_t)compute_units * (s.tpr == 1024 ? 1 : 2); // more of them leave more sums to read again: with 4, 3-15 % slower
     s.groups = (uint32_t)(all < most ? all : most);
     return s;
@@ -253,8 +255,8 @@ template <typename TG, typename TR, bool DROP> void launch(const NormGradArgs &a
     ERI_NORM_GRAD(64, 1, false);
     ERI_NORM_GRAD(64, 2, false);
     ERI_NORM_GRAD(256, 1, false);
-    ERI_NORM_GRAD(256, 2, false);
-    ERI_NORM_GRAD(256, 4, false);
+    ERI_NORM_GRAD(512, 1, false);
+    ERI_NORM_GRAD(512, 2, false);
     ERI_NORM_GRAD(1024, 2, false);
 #undef ERI_NORM_GRAD
     if (shape.nv == 0) hipLaunchKernelGGL((rms_norm_grad_long_kernel<TG, TR, DROP>), dim3(shape.groups), dim3(1024), 0, s, a);
