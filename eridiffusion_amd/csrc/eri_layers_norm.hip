@@ -8,16 +8,17 @@
  * whole waves ran at a third: 100000 x 128 bf16 28 us, now 11.  Fewer threads with more of the row each, us for 8192 rows with a
  * residual:
  *   2048 bf16 64 threads 22.4, 256 21.2;   4096 bf16 64 50.9, 256 42.6, 512 42.2;   4096 fp32 64 109, 256 97.8, 512 93.4;
- *   5120 fp32 256 150, 512 144;   8192 bf16 256 96.7, 512 94.6, 1024 91.4;   1000 bf16 128 12.4, 64 11.9
- * Where the row moves fewer bytes there is less for many threads to wait on, and half the threads with twice the vectors win.  A
+ *   6144 fp32 256 150, 512 144;   8192 bf16 256 96.7, 512 94.6, 1024 91.4;   1000 bf16 128 12.4, 64 11.9
+ * Where a row moves fewer bytes, half the threads with twice the vectors win.  A
  * bf16 row of 4097 to 6144 columns: to 8 bits with a residual 256 threads 50.7, 512 57.5 (at 6144 columns 65.5 and 67.6), to bf16
- * with one 60.1 and 59.2 (2048 rows 14.1 and 15.5).  Up to 6 bytes an element, which is without a residual and not fp32 to fp32:
+ * with one 60.1 and 59.2 (2048 rows 14.1 and 15.5).  Without a residual, unless y is fp32:
  *   bf16 to 8 bits  2560 18.4, was 22.2;   4096 20.2, 23.1;   5120 30.0, 38.3;   8192 43.2, 51.9;   12288 64.1, 80.0
  *   bf16 to bf16    2560 16.4, was 19.6;   4096 21.5, 22.9;   5120 30.1, 35.6;   8192 44.7, 52.5;   12288 72.9, 80.4
  *   fp32 to bf16    2560 22.9, was 26.2;   4096 32.8, 32.5;   5120 41.6, 43.8;   8192 72.4, 76.2;   12288 105.9, 117.7
+ *   bf16 to fp32    2560 22.2, not so 22.8; 4096 37.3, 35.3; 5120 45.3, 47.7; 8192 76.8, 75.6;   2048 19.5, 18.1: not worth it
  * A row's layout, and so its rounding, does not depend on how many rows there are.
  * Dropout is drawn beside the loads and costs nothing: 16384 x 4096 bf16 with residual and dropout 91 us, 5.9 TB/s (a copy of that
- * size runs at 5.2); 8192 x 5120 to 8 bits 51 us, 5.8 TB/s; one row of 4096 2.2 us, a launch and two trips to memory.
+ * size runs at 5.2); 8192 x 5120 to 8 bits 51-57 us, 5.2-5.8 TB/s; one row of 4096 2.2 us, a launch and two trips to memory.
  */
 #include "eri_layers_device.h"
 
@@ -207,15 +208,14 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
 template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormArgs &a, uint32_t compute_units, hipStream_t s) {
 #define ERI_NORM(TPR, NV, SHORT) \
     hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV, SHORT>), dim3((a.rows - a.first + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR * rows_of(TPR)), 0, s, a)
-// a light row's layout, then the others'; only those that some call reaches are compiled
+// the layout of a row that moves few bytes, then the others'; only those that some call reaches are compiled
 #define ERI_NORM_EITHER(TPR, NV, TPR2, NV2) \
     do { \
         if constexpr (!kMayBeLight) ERI_NORM(TPR2, NV2, false); \
-        else if constexpr (sizeof(TX) == 2) ERI_NORM(TPR, NV, false); \
         else if (a.y_dtype != ERI_DTYPE_F32) ERI_NORM(TPR, NV, false); \
         else ERI_NORM(TPR2, NV2, false); \
     } while (0)
-    constexpr bool kMayBeLight = !RES; // and then all but fp32 to fp32 is
+    constexpr bool kMayBeLight = !RES; // and is unless y is fp32
     constexpr int kMiddle = RES && sizeof(TX) + sizeof(TR) == 4 ? 256 : 512; // threads to other rows of 4097 to 6144 columns
     if (a.cols < 8) ERI_NORM(16, 1, true);
     else if (a.cols <= 128) ERI_NORM(16, 1, false);
