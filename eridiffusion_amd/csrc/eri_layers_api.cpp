@@ -126,9 +126,7 @@ int eri_embedding_grad(const EriEmbeddingGrad *args, void *stream) {
     ERI_NEED(aligned(a.grad, size_of(a.grad_dtype)) && aligned(a.out, size_of(a.out_dtype)), ERI_ERR_ALIGN, "grad or out is not aligned to its elements");
     ERI_NEED(aligned(a.workspace, 16), ERI_ERR_ALIGN, "workspace is not 16-byte aligned");
     ERI_NEED(a.workspace_bytes >= need, ERI_ERR_ARG, "workspace is too small");
-    uint32_t cus;
-    if (int rc = compute_units(&cus, kCall)) return rc;
-    return done(eri_layers::launch_embedding_grad(a, cus, stream), kCall);
+    return done(eri_layers::launch_embedding_grad(a, stream), kCall);
 }
 
 int eri_dropout(const EriDropout *args, void *stream) {
@@ -170,9 +168,7 @@ int eri_rms_norm(const EriRmsNorm *args, void *stream) {
     ERI_NEED(aligned(a.x, size_of(a.x_dtype)) && aligned(a.y, size_of(a.y_dtype)) && aligned(a.h, size_of(h_dtype)) && aligned(a.rstd, 4) && aligned(a.scales, 4) &&
                  (!a.residual || aligned(a.residual, size_of(a.residual_dtype))) && (!a.weight || aligned(a.weight, size_of(a.weight_dtype))),
              ERI_ERR_ALIGN, "an address is not aligned to its elements");
-    uint32_t cus;
-    if (int rc = compute_units(&cus, kCall)) return rc;
-    return done(eri_layers::launch_rms_norm(a, d, cus, stream), kCall);
+    return done(eri_layers::launch_rms_norm(a, d, stream), kCall);
 }
 
 int eri_rms_norm_grad_workspace(uint64_t rows, uint64_t cols, uint64_t *bytes) {

@@ -272,10 +272,10 @@ __device__ __forceinline__ float dropped(float v, const u32x4 &bits, uint32_t e,
 /* Launchers, one file for each; `stream` is a hipStream_t and the result a hipError_t.  The arguments have been checked:
  * strides are set, rows and cols are not 0 where it is not said. */
 int launch_embedding(const EriEmbedding &a, uint32_t compute_units, void *stream);
-int launch_embedding_grad(const EriEmbeddingGrad &a, uint32_t compute_units, void *stream);
+int launch_embedding_grad(const EriEmbeddingGrad &a, void *stream);
 uint64_t embedding_grad_workspace(uint64_t tokens, uint64_t vocab, uint64_t dim);
 int launch_dropout(const EriDropout &a, const Drop &d, uint32_t compute_units, void *stream);
-int launch_rms_norm(const EriRmsNorm &a, const Drop &d, uint32_t compute_units, void *stream);
+int launch_rms_norm(const EriRmsNorm &a, const Drop &d, void *stream);
 int launch_rms_norm_grad(const EriRmsNormGrad &a, const Drop &d, uint32_t compute_units, void *stream); // rows may be 0
 uint64_t rms_norm_grad_workspace(uint64_t rows, uint64_t cols, uint32_t compute_units);
 

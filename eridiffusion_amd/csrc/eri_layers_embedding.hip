@@ -597,7 +597,7 @@ uint64_t embedding_grad_workspace(uint64_t tokens, uint64_t vocab, uint64_t dim)
     return is_few(tokens, vocab, dim) ? 0 : partial_at(tokens) + partial_bytes(tokens, dim);
 }
 
-int launch_embedding_grad(const EriEmbeddingGrad &e, uint32_t, void *stream) {
+int launch_embedding_grad(const EriEmbeddingGrad &e, void *stream) {
     char *ws = static_cast<char *>(e.workspace);
     // accumulating, there are no zeros to write: one launch as long as its workgroups, most of them with nothing to do, start faster than
     // two more launches.  300 tokens, one | three: 128000 x 1024 (4096 workgroups) 9.4 | 12.9 us, 88138 x 1272 (6144) 12.6 | 13.6,
@@ -621,7 +621,7 @@ int launch_embedding_grad(const EriEmbeddingGrad &e, uint32_t, void *stream) {
     while (a.lanes < kWave && a.lanes * 16ull < (uint64_t)a.dim * a.out_bytes) a.lanes *= 2;
     hipLaunchKernelGGL(embedding_sort_kernel, dim3(used_buckets), dim3(1024), kWaves * a.locals * 4, s, a);
     const hipError_t err = hipGetLastError();
-    if (err != hipSuccess) return (int)err;
+    if (err != hipSuccess || a.tokens == 0) return (int)err;
     if (g32) o32 ? launch_sums<float, float>(a, s) : launch_sums<float, bf16>(a, s);
     else o32 ? launch_sums<bf16, float>(a, s) : launch_sums<bf16, bf16>(a, s);
     return (int)hipGetLastError();

@@ -205,7 +205,7 @@ template <typename TX, typename TR, bool RES, bool DROP> __global__ __launch_bou
     }
 }
 
-template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormArgs &a, uint32_t compute_units, hipStream_t s) {
+template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormArgs &a, hipStream_t s) {
 #define ERI_NORM(TPR, NV, SHORT) \
     hipLaunchKernelGGL((rms_norm_kernel<TX, TR, RES, DROP, TPR, NV, SHORT>), dim3((a.rows - a.first + rows_of(TPR) - 1) / rows_of(TPR)), dim3(TPR * rows_of(TPR)), 0, s, a)
 // the layout of a row that moves few bytes, then the others'; only those that some call reaches are compiled
@@ -234,16 +234,16 @@ template <typename TX, typename TR, bool RES, bool DROP> void launch(const NormA
 #undef ERI_NORM
 }
 
-template <typename TX> void launch_of(const NormArgs &a, bool res, bool res_f32, uint32_t compute_units, hipStream_t s) {
+template <typename TX> void launch_of(const NormArgs &a, bool res, bool res_f32, hipStream_t s) {
     const bool drop = a.drop.below != 0;
-    if (!res) drop ? launch<TX, TX, false, true>(a, compute_units, s) : launch<TX, TX, false, false>(a, compute_units, s);
-    else if (res_f32) drop ? launch<TX, float, true, true>(a, compute_units, s) : launch<TX, float, true, false>(a, compute_units, s);
-    else drop ? launch<TX, bf16, true, true>(a, compute_units, s) : launch<TX, bf16, true, false>(a, compute_units, s);
+    if (!res) drop ? launch<TX, TX, false, true>(a, s) : launch<TX, TX, false, false>(a, s);
+    else if (res_f32) drop ? launch<TX, float, true, true>(a, s) : launch<TX, float, true, false>(a, s);
+    else drop ? launch<TX, bf16, true, true>(a, s) : launch<TX, bf16, true, false>(a, s);
 }
 
 } // namespace
 
-int launch_rms_norm(const EriRmsNorm &e, const Drop &d, uint32_t compute_units, void *stream) {
+int launch_rms_norm(const EriRmsNorm &e, const Drop &d, void *stream) {
     NormArgs a = {e.x, e.residual, e.weight, e.y, e.h, e.rstd, e.scales, 0, 0, (uint32_t)e.cols,
                   e.x_stride, e.residual_stride, e.y_stride, e.h_stride, e.eps, e.weight_dtype == ERI_DTYPE_F32, (uint32_t)e.y_dtype,
                   (uint32_t)e.scale_group, e.scale_group ? (uint32_t)((e.cols + 127) / 128) : 1u, d};
@@ -251,8 +251,8 @@ int launch_rms_norm(const EriRmsNorm &e, const Drop &d, uint32_t compute_units, 
     constexpr uint32_t kMost = 1u << 21; // rows of a launch
     for (a.first = 0; a.first < e.rows; a.first += kMost) {
         a.rows = e.rows - a.first < kMost ? (uint32_t)e.rows : a.first + kMost;
-        if (e.x_dtype == ERI_DTYPE_F32) launch_of<float>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, compute_units, s);
-        else launch_of<bf16>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, compute_units, s);
+        if (e.x_dtype == ERI_DTYPE_F32) launch_of<float>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, s);
+        else launch_of<bf16>(a, e.residual != nullptr, e.residual_dtype == ERI_DTYPE_F32, s);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return (int)err;
     }

@@ -242,6 +242,17 @@ def test_table_gradient_past_32_bit_offsets(layers):
     assert int((out != 0).any(1).sum()) == 3
 
 
+@pytest.mark.parametrize("vocab,dim", [(70000, 1000), (300000, 256)])
+def test_table_gradient_of_no_token(layers, vocab, dim):
+    """A large table, which takes the sort, with an empty batch: zeros, or what was there."""
+    ids, grad = torch.zeros(0, dtype=torch.long, device="cuda"), torch.zeros(0, dim, dtype=BF, device="cuda")
+    out = torch.full((vocab, dim), 3.0, dtype=BF, device="cuda")
+    layers.embedding_grad(ids, grad, vocab, out=out, accumulate=True)
+    assert bool((out == 3).all())
+    layers.embedding_grad(ids, grad, vocab, out=out)
+    assert bool((out == 0).all())
+
+
 # ---------------------------------------------------------------------------------------------------------------
 # norm
 # ---------------------------------------------------------------------------------------------------------------
