@@ -1,6 +1,8 @@
 /*
  * Gradient of the residual addition and root-mean-square norm of include/eri_layers.h:
  *     dh = dr + q dy w - h q^3 mean(dy w h),  dx = drop(dh),  dw = sum over rows of dy h q
+ * computed as c = q (q mean(dy w h)), dh = dr + q (dy w - h c): q^3 leaves fp32 for rows of 1e-13 and is lost for rows of 1e15, while
+ * q mean(dy w h) and h c are of the order of dy w whatever the rows' size.
  *
  * Bound by HBM: dy, h and dr are read once, dh and dx written once; the row waits in registers for its sum, and each thread keeps
  * the weight and the sums of dw of its columns over all rows that its workgroup takes.  The workgroups' sums (two a compute
@@ -116,12 +118,12 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(co
                 acc[k][e] = fmaf(gh, rstd, acc[k][e]);
             }
         }
-        c = sum_over<TPR>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
+        c = sum_over<TPR>(c, slots[turn]) * rstd / (float)a.cols * rstd;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             float dh[8];
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) dh[e] = fmaf(g[k].get(e) * w[k][e], rstd, fmaf(-h[k].get(e), c, r[k].get(e)));
+            for (uint32_t e = 0; e < 8; ++e) dh[e] = fmaf(fmaf(-h[k].get(e), c, g[k].get(e) * w[k][e]), rstd, r[k].get(e));
             store_grads<TR, DROP>(a, row, (k * TPR + t) * 8, dh, offset);
         }
     }
@@ -177,7 +179,7 @@ template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024
                 store8(out, col, a.padded, old);
             }
         }
-        c = sum_over<1024>(c, slots[turn]) / (float)a.cols * (rstd * rstd * rstd);
+        c = sum_over<1024>(c, slots[turn]) * rstd / (float)a.cols * rstd;
         for (uint32_t col = threadIdx.x * 8; col < a.cols; col += 8192) {
             Raw<TG> g;
             Raw<TR> h, r;
@@ -191,7 +193,7 @@ template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024
             settle8<false>(h, col, a.cols);
             settle8<false>(r, col, a.cols);
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e) dh[e] = fmaf(a.weight ? g.get(e) * w[e] : g.get(e), rstd, fmaf(-h.get(e), c, r.get(e)));
+            for (uint32_t e = 0; e < 8; ++e) dh[e] = fmaf(fmaf(-h.get(e), c, a.weight ? g.get(e) * w[e] : g.get(e)), rstd, r.get(e));
             store_grads<TR, DROP>(a, row, col, dh, offset);
         }
     }
