@@ -527,19 +527,27 @@ uint32_t lanes_of(uint64_t dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : dim <
 
 /* Short pieces where that is what it takes to have waves enough: 616 tokens of 768 took 7.9 us with pieces of 32, 4.7 with 8;
  * 32768 of 4096 84 with 32, 93 with 16, 124 with 8. */
+constexpr uint32_t kLogPieceLeast = 3;
+constexpr uint64_t kThreadsEnough = 2048 * kWave;
+uint64_t threads_of(uint64_t dim) { // to a row in the sums, all tiles together
+    const uint64_t lanes = lanes_of(dim);
+    return (dim + lanes * 8 - 1) / (lanes * 8) * lanes;
+}
 uint32_t log_piece_of(uint64_t tokens, uint64_t dim) {
-    const uint64_t lanes = lanes_of(dim), tiles = (dim + lanes * 8 - 1) / (lanes * 8);
     uint32_t log_piece = kLogPieceMost;
-    while (log_piece > 3 && (tokens >> (log_piece - 1)) * tiles * lanes < 2048 * kWave) --log_piece;
+    while (log_piece > kLogPieceLeast && (tokens >> (log_piece - 1)) * threads_of(dim) < kThreadsEnough) --log_piece;
     return log_piece;
 }
 
 /* The workspace: the number of places, the places, the sums of pieces; 16 bytes and multiples of them. */
 constexpr uint64_t kHead = 16;
 uint64_t partial_at(uint64_t tokens) { return kHead + tokens * sizeof(Place); }
+/* For any number of tokens up to this one, so that a workspace that was made for the largest batch does for all.  Fewer tokens may be
+ * cut into more pieces, shorter ones: at most as many as need the last threads that are wanted. */
 uint64_t partial_bytes(uint64_t tokens, uint64_t dim) {
-    const uint32_t log_piece = log_piece_of(tokens, dim);
-    return tokens >> log_piece ? 2 * ((tokens >> log_piece) + 1) * padded_of(dim) * sizeof(float) : 0;
+    const uint64_t own = tokens >> log_piece_of(tokens, dim), shortest = tokens >> kLogPieceLeast, wanted = (kThreadsEnough - 1) / threads_of(dim);
+    const uint64_t fewer = shortest < wanted ? shortest : wanted, pieces = own > fewer ? own : fewer;
+    return pieces ? 2 * (pieces + 1) * padded_of(dim) * sizeof(float) : 0;
 }
 
 template <typename TG, typename TO, int L, bool SHORT = false> void launch_sum(GradArgs a, hipStream_t s) {

@@ -45,7 +45,8 @@ int eri_embedding(const EriEmbedding *args, void *stream);
 /* ---------------------------------------------------------------------------------------------
  * The table's gradient: out[v] = scale * (sum of grad[t] over the tokens t with ids[t] = v), all rows of out written,
  * rows that no token names with zeros.  accumulate: the sum is added to what out holds, and rows without a token are
- * not touched.  Tokens whose id is padding_id or lies outside [0, vocab) add nothing.  Sums are F32 in an order that
+ * not touched.  Tokens whose id is padding_id or lies outside [0, vocab) add nothing.  The workspace that some tokens need does
+ * for fewer tokens of the same table too.  Sums are F32 in an order that
  * the sizes alone decide: the same inputs give the same bits.
  * ------------------------------------------------------------------------------------------- */
 typedef struct EriEmbeddingGrad {
@@ -125,7 +126,8 @@ int eri_rms_norm(const EriRmsNorm *args, void *stream);
  *     dh = grad_h + rstd * (grad * weight) - h * rstd^3 * mean(grad * weight * h)
  *     grad_residual = dh     grad_x = dropout(dh)     grad_weight = sum over rows of grad * h * rstd
  * Any of the three outputs may be NULL.  Sums are F32; grad_weight's order is decided by the sizes and the device's
- * number of compute units: the same inputs give the same bits. */
+ * number of compute units: the same inputs give the same bits.  The workspace that some rows need does for fewer rows of the
+ * same length too. */
 typedef struct EriRmsNormGrad {
     const void *grad;
     const void *h;

@@ -116,6 +116,19 @@ def test_refusals_of_the_tables_gradient():
         assert _refused("eri_embedding_grad", _with(EmbeddingGrad, base, **change)) == code, change
 
 
+@pytest.mark.parametrize("dim", [1, 7, 40, 64, 100, 256, 257, 768, 1155, 4096, 20000])
+def test_the_tables_gradients_workspace_does_for_fewer_tokens(dim):
+    """Whoever makes it for the largest batch has enough for a shorter last one."""
+    fn, need, most = L.lib().eri_embedding_grad_workspace, C.c_uint64(), 0
+    fn.restype, fn.argtypes = C.c_int, [C.c_uint64] * 3 + [C.c_void_p]
+    for vocab in (8, 49408):
+        most = 0
+        for tokens in sorted({t for k in range(24) for t in range(max(0, 2 ** k - 40), 2 ** k + 41)} | set(range(0, 40000, 7)) | {9000, 2 ** 31 - 1}):
+            assert fn(tokens, vocab, dim, C.byref(need)) == 0
+            assert need.value >= most, (tokens, need.value, most)
+            most = need.value
+
+
 def test_refusals_of_dropout():
     base = dict(x=0x1000, y=0x2000, rows=4, cols=16, dtype_tag=F32)
     assert _refused("eri_dropout", None) == NULL
