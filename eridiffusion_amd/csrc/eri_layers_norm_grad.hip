@@ -278,8 +278,10 @@ uint64_t rms_norm_grad_workspace(uint64_t rows, uint64_t cols, uint32_t compute_
 int launch_rms_norm_grad(const EriRmsNormGrad &e, const Drop &d, uint32_t compute_units, void *stream) {
     const Shape shape = shape_of(e.rows, e.cols, compute_units);
     const uint32_t padded = (uint32_t)padded_of(e.cols);
-    // grad and h are read twice where that saves the second launch; not when one of them is being replaced
-    const bool replaces = (e.grad_x && (e.grad_x == e.grad || e.grad_x == e.h)) || (e.grad_residual && (e.grad_residual == e.grad || e.grad_residual == e.h));
+    // Where that saves the second launch, grad and h are read by other workgroups too, and grad_weight is written while weight is
+    // still read: not when one of them is being replaced.
+    auto over = [&](const void *out, const void *in) { return out && out == in; };
+    const bool replaces = over(e.grad_x, e.grad) || over(e.grad_x, e.h) || over(e.grad_residual, e.grad) || over(e.grad_residual, e.h) || over(e.grad_weight, e.weight);
     const bool few = e.grad_weight && e.rows && is_few(e.rows, e.cols) && shape.nv && !replaces;
     float *partial = e.grad_weight && !few ? (float *)e.workspace : nullptr;
     const NormGradArgs a = {e.grad, e.h, e.weight, e.grad_h, e.rstd, e.grad_x, e.grad_residual, partial, few ? e.grad_weight : nullptr, (uint32_t)e.rows,

@@ -12,7 +12,10 @@
  * The argument structs are plain data: zero them first, so that fields added later read as "not used".  Rows lie
  * `*_stride` elements apart, with 0 for rows without gaps; the elements of a row are adjacent.  An address needs
  * the alignment of its element only; rows that begin at 16-byte addresses are read in whole words and run fastest.
- * An output may be the input that it replaces (same address, stride and dtype), and overlaps nothing else.
+ * Outputs overlap neither each other nor an input, but for rows written over rows of the same address, stride and dtype:
+ *     eri_dropout        y over x
+ *     eri_rms_norm       y and h, each over x or residual
+ *     eri_rms_norm_grad  grad_x and grad_residual, each over grad, h or grad_h;  grad_weight over weight
  */
 #ifndef ERI_LAYERS_H
 #define ERI_LAYERS_H

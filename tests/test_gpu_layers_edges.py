@@ -5,8 +5,8 @@ import pytest
 import torch
 
 from oracle import layers_f64 as of
-from test_gpu_layers import BF, F32, OFFSET, SEED, U, U32, _depth, _ids, _near, _new, layers  # noqa: F401
-from test_layers_host import EmbeddingGrad
+from test_gpu_layers import BF, F32, OFFSET, SEED, U, U32, _depth, _ids, _near, _new, _norm_bounds, layers  # noqa: F401
+from test_layers_host import EmbeddingGrad, Norm, NormGrad
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,42 @@ def test_one_workspace_for_batches_of_all_sizes():
         deep = int(torch.bincount(ids[(ids >= 0) & (ids < vocab)]).max()) + 4
         _near(out, want, U32 * want.abs() + deep * U32 * terms, tokens)
         assert bool((ws[size:] == 77).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 40), (300, 200), (70, 1281), (40, 9001), (900, 1281), (5, 20000)])
+@pytest.mark.parametrize("over", ["weight", "x on h", "x on grad_h, residual on grad", "all"])
+def test_norm_gradient_over_each_of_its_inputs(rows, cols, over):
+    """Every pair that the header allows, with grad_weight wanted, in one launch and in two."""
+    from eridiffusion_amd import _lib as L
+    (gy, h, gh), w = (_new(rows, cols, seed=s) for s in range(3)), _new(cols, std=0.3, mean=1.0)
+    rstd = (1 / torch.sqrt((h.double() ** 2).mean(-1) + 1e-6)).float()
+    dx, dr, dw, size, size_w = of.rms_norm_grad(gy, h, rstd, w, gh, 0.25, SEED, OFFSET)
+    g, hh, r, q, ww = gy.cuda(), h.cuda(), gh.cuda(), rstd.cuda(), w.cuda()
+    new = lambda t: torch.empty_like(t)  # noqa: E731
+    x, res, weight = {"weight": (new(g), new(g), ww), "x on h": (hh, new(g), new(ww)), "x on grad_h, residual on grad": (r, g, new(ww)), "all": (hh, g, ww)}[over]
+    need = _need("eri_rms_norm_grad_workspace", rows, cols)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    a = NormGrad(grad=g.data_ptr(), h=hh.data_ptr(), rstd=q.data_ptr(), weight=ww.data_ptr(), grad_h=r.data_ptr(), grad_x=x.data_ptr(), grad_residual=res.data_ptr(),
+                 grad_weight=weight.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=need, rows=rows, cols=cols)
+    a.key.seed, a.key.offset, a.key.p = SEED, OFFSET, 0.25
+    L.check(L.lib().eri_rms_norm_grad(C.byref(a), _stream()), "eri_rms_norm_grad")
+    off = U32 * (_depth(cols) + 12) * size
+    _near(res, dr, U32 * dr.abs() + off, "residual")
+    _near(x, dx, 3 * U32 * dx.abs() + 1.4 * off, "x")
+    _near(weight, dw, U32 * dw.abs() + U32 * (rows + 130) * size_w, "weight")
+
+
+@pytest.mark.parametrize("cols", [40, 1001, 6000, 34000])
+@pytest.mark.parametrize("y_on,h_on", [("residual", "x"), ("residual", None), (None, "x")])
+def test_norm_over_each_of_its_inputs(cols, y_on, h_on):
+    from eridiffusion_amd import _lib as L
+    x, r, w = _new(9, cols), _new(9, cols, seed=1), _new(cols, std=0.3, mean=1.0)
+    y, h, rstd = of.rms_norm(x, w, 1e-6, r, 0.25, SEED, OFFSET)
+    dev = {"x": x.cuda(), "residual": r.cuda(), None: torch.empty(9, cols, device="cuda")}
+    dw = w.cuda()
+    a = Norm(x=dev["x"].data_ptr(), residual=dev["residual"].data_ptr(), weight=dw.data_ptr(), y=dev[y_on].data_ptr(), h=dev[h_on].data_ptr(), rows=9, cols=cols, eps=1e-6)
+    a.key.seed, a.key.offset, a.key.p = SEED, OFFSET, 0.25
+    L.check(L.lib().eri_rms_norm(C.byref(a), _stream()), "eri_rms_norm")
+    off_h, off_y = _norm_bounds(x, w, r, 0.25, y, h, rstd, cols)
+    _near(dev[h_on], h, U32 * h.abs() + off_h, "h")
+    _near(dev[y_on], y, U32 * y.abs() + off_y, "y")
