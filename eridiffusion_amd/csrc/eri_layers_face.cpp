@@ -61,6 +61,7 @@ const at::Tensor &tensor(PyObject *o, const char *name) {
     const at::Tensor &t = THPVariable_Unpack(o);
     ERI_VALUE(t.defined() && t.layout() == at::kStrided && t.has_storage() && !t.unsafeGetTensorImpl()->is_python_dispatch(),
               std::string(name) + " is no plain tensor");
+    ERI_VALUE(!t._fw_grad(0).defined(), std::string(name) + " carries a forward-mode tangent, which these layers do not take along");
     ERI_VALUE(t.is_cuda(), std::string(name) + " is on " + t.device().str() + ": these layers take device tensors");
     ERI_VALUE(!t.is_conj() && !t.is_neg(), std::string(name) + " is a lazy view");
     return t;

@@ -178,6 +178,32 @@ def test_the_python_calls_refuse_host_tensors_and_other_types():
         _layers_face.dropout(x)
 
 
+def _calls(x, ids):
+    """Each call, with x wherever a tensor of floats may stand."""
+    w = x[0]
+    return [lambda: layers.dropout(x, 0.1, 1), lambda: layers.rms_norm(x), lambda: layers.rms_norm(x, w, residual=x), lambda: layers.embedding(ids, x),
+            lambda: layers.embedding_grad(ids, x, 8), lambda: layers.rms_norm_grad(x, x, x[:, 0])]
+
+
+def test_forward_mode_tangents_are_refused():
+    """They would be lost without a word: torch reads a result without a tangent as one that does not change."""
+    from torch.autograd import forward_ad as fa
+    x, t, ids = torch.zeros(4, 8), torch.ones(4, 8), torch.zeros(4, dtype=torch.long)
+    with fa.dual_level():
+        d = fa.make_dual(x, t)
+        for call in _calls(d, ids):
+            with pytest.raises(ValueError, match="forward-mode tangent"):
+                call()
+        for call in _calls(fa.make_dual(x.clone().requires_grad_(), t), ids):  # beside a gradient that is recorded
+            with pytest.raises(ValueError, match="forward-mode tangent"):
+                call()
+        for call in _calls(fa.unpack_dual(d).primal, ids):
+            with pytest.raises(ValueError, match="take device tensors"):
+                call()
+    with pytest.raises(ValueError, match="no plain tensor|forward-mode tangent"):
+        torch.func.jvp(lambda x: layers.dropout(x, 0.1, 1), (x,), (t,))
+
+
 def _words(got):
     return ["%08x" % int(w) for w in got[0]]
 
