@@ -10,7 +10,9 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -50,6 +52,16 @@ struct Raised : std::exception {}; // a Python error has been set
 }
 void check(int code, const char *call) {
     if (code) raise_code(code, call);
+}
+
+/* Tracers record torch's operations to run them again, or run them on tensors without values.  These kernels are none: what was
+ * recorded would be outputs that nobody writes.  A dispatch mode of a user's own (one that counts or logs) stays: the call runs under it. */
+void not_traced() {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    using Key = c10::impl::TorchDispatchModeKey;
+    const bool jit = at::tracer::impl::is_dispatch_enabled();
+    const bool mode = Modes::any_modes_set() && (Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL));
+    ERI_VALUE(!jit && !mode, "these layers cannot be traced: a recorded program would not run their kernels");
 }
 
 int tag_of(at::ScalarType t) {
@@ -448,6 +460,7 @@ template <PyObject *(*F)(PyObject *const *), Py_ssize_t N> PyObject *entry(PyObj
         return nullptr;
     }
     try {
+        not_traced();
         return F(args);
     } catch (const Raised &) {
         return nullptr;

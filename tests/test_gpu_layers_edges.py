@@ -3,6 +3,7 @@ import ctypes as C
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from oracle import layers_f64 as of
 from test_gpu_layers import BF, F32, OFFSET, SEED, U, U32, _depth, _ids, _near, _new, _norm_bounds, layers  # noqa: F401
@@ -105,3 +106,28 @@ def test_norm_over_each_of_its_inputs(cols, y_on, h_on):
     off_h, off_y = _norm_bounds(x, w, r, 0.25, y, h, rstd, cols)
     _near(dev[h_on], h, U32 * h.abs() + off_h, "h")
     _near(dev[y_on], y, U32 * y.abs() + off_y, "y")
+
+
+def test_under_a_dispatch_mode_that_only_looks_on(layers):  # noqa: F811
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Count(TorchDispatchMode):
+        seen = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.seen += 1
+            return func(*args, **(kwargs or {}))
+    x, w = _new(5, 40).cuda(), _new(40).cuda().requires_grad_()
+    want = layers.rms_norm(x, w, residual=x, p=0.2, seed=1)
+    with Count() as mode:
+        got = layers.rms_norm(x, w, residual=x, p=0.2, seed=1)
+    assert mode.seen and torch.equal(got.y, want.y) and torch.equal(got.h, want.h)
+
+    def block(x, w):
+        return layers.rms_norm(torch.nn.functional.gelu(x), w, residual=x, p=0.2, seed=1).y
+    grads = []
+    for run in (block, lambda *a: torch.utils.checkpoint.checkpoint(block, *a, use_reentrant=False)):
+        xs, ws = x.clone().requires_grad_(), w.detach().clone().requires_grad_()
+        run(xs, ws).square().sum().backward()
+        grads.append((xs.grad, ws.grad))
+    assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])

@@ -180,9 +180,9 @@ def test_the_python_calls_refuse_host_tensors_and_other_types():
 
 def _calls(x, ids):
     """Each call, with x wherever a tensor of floats may stand."""
-    w = x[0]
+    w, q = x[0], x[:, 0]
     return [lambda: layers.dropout(x, 0.1, 1), lambda: layers.rms_norm(x), lambda: layers.rms_norm(x, w, residual=x), lambda: layers.embedding(ids, x),
-            lambda: layers.embedding_grad(ids, x, 8), lambda: layers.rms_norm_grad(x, x, x[:, 0])]
+            lambda: layers.embedding_grad(ids, x, 8), lambda: layers.rms_norm_grad(x, x, q)]
 
 
 def test_forward_mode_tangents_are_refused():
@@ -202,6 +202,21 @@ def test_forward_mode_tangents_are_refused():
                 call()
     with pytest.raises(ValueError, match="no plain tensor|forward-mode tangent"):
         torch.func.jvp(lambda x: layers.dropout(x, 0.1, 1), (x,), (t,))
+
+
+def test_tracers_are_refused():
+    """What they record is the making of the outputs; the program would return memory that nobody wrote."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, ids = torch.zeros(4, 8), torch.zeros(4, dtype=torch.long)
+    for k, call in enumerate(_calls(x, ids)):
+        for trace in (lambda f: torch.jit.trace(f, (x, ids)), lambda f: make_fx(f)(x, ids), lambda f: make_fx(f, tracing_mode="fake")(x, ids)):
+            with pytest.raises(ValueError, match="cannot be traced"):
+                trace(lambda a, b: _calls(a, b)[k]())
+        with FakeTensorMode(), pytest.raises(ValueError, match="cannot be traced"):
+            call()
+        with pytest.raises(ValueError, match="take device tensors"):  # and not what comes after them
+            call()
 
 
 def _words(got):
