@@ -123,6 +123,28 @@ struct Rows {
     }
 };
 
+/* Bytes that rows take: `count` of them, `width` long and `step` apart. */
+struct Span {
+    uint64_t at, count, width, step;
+    explicit Span(const Rows &r)
+        : at(reinterpret_cast<uint64_t>(r.t.const_data_ptr())), count((uint64_t)r.rows), width((uint64_t)r.cols * r.t.element_size()), step(r.stride * r.t.element_size()) {
+        if (step == width || count == 1) width *= count, step = width, count = 1; // without gaps: one long row
+    }
+    uint64_t end() const { return at + (count - 1) * step + width; }
+    bool operator==(const Span &o) const { return at == o.at && count == o.count && width == o.width && step == o.step; }
+    /* Rows at the same distance may lie beside each other, columns of one matrix; at different distances they are taken to meet. */
+    bool meets(const Span &o) const {
+        if (!count || !width || !o.count || !o.width || end() <= o.at || o.end() <= at) return false;
+        if (count > 1 && o.count > 1 && step != o.step) return true;
+        if (count == 1 && o.count == 1) return true;
+        const uint64_t s = count > 1 ? step : o.step;
+        const uint64_t from = o.at >= at ? (o.at - at) % s : (s - (at - o.at) % s) % s; // where the other's row begins, seen from the beginning of this one's
+        return from < width || from + o.width > s;
+    }
+};
+/* Refuses a given output whose memory meets an input's: some workgroups write it while others still read. */
+void apart(const Rows &out, const Rows &in, const char *name) { ERI_VALUE(!Span(out).meets(Span(in)), std::string("out overlaps ") + name); }
+
 double number(PyObject *o, const char *name) {
     const double v = PyFloat_AsDouble(o);
     if (v == -1.0 && PyErr_Occurred()) {
@@ -238,6 +260,7 @@ PyObject *embedding(PyObject *const *args) {
     const auto shape = with_last(ids.sizes(), weight.size(1));
     const Rows out(args[3] == Py_None ? made.empty(shape, weight.scalar_type(), weight) : written(args[3], "out", weight), "out");
     ERI_VALUE(out.t.sizes() == at::IntArrayRef(shape) && out.t.scalar_type() == weight.scalar_type(), "out has another shape or dtype than the rows");
+    if (args[3] != Py_None) apart(out, table, "weight"), apart(out, Rows(ids), "ids");
     a.ids = ids.const_data_ptr();
     a.table = table.t.const_data_ptr();
     a.out = out.t.data_ptr();
@@ -284,6 +307,7 @@ PyObject *embedding_grad(PyObject *const *args) {
     const Rows out(args[6] == Py_None ? made.empty(shape, dtype, grad) : written(args[6], "out", grad), "out");
     ERI_VALUE(out.t.sizes() == at::IntArrayRef(shape) && (args[5] == Py_None || out.t.scalar_type() == dtype), "out has another shape or dtype than the gradient");
     const Rows rows(grad);
+    if (args[6] != Py_None) apart(out, rows, "grad"), apart(out, Rows(ids), "ids");
     check(eri_embedding_grad_workspace((uint64_t)ids.numel(), vocab, (uint64_t)grad.size(-1), &a.workspace_bytes), "eri_embedding_grad_workspace");
     const at::Tensor workspace = made.empty({(int64_t)a.workspace_bytes}, at::kByte, grad);
     a.ids = ids.const_data_ptr();
@@ -318,6 +342,10 @@ PyObject *dropout(PyObject *const *args) {
     made.guard.reset_device(given.device());
     const Rows out(args[4] == Py_None ? made.empty(given.sizes(), given.scalar_type(), given) : written(args[4], "out", given), "out");
     ERI_VALUE(out.t.sizes() == given.sizes() && out.t.scalar_type() == given.scalar_type(), "out has another shape or dtype than x");
+    if (args[4] != Py_None) {
+        if (!(Span(out) == Span(x))) apart(out, x, "x"); // over x itself: each element by the thread that has read it
+        if (a.key.offset_ptr) apart(out, Rows(THPVariable_Unpack(args[3])), "offset");
+    }
     a.x = x.t.const_data_ptr();
     a.y = out.t.data_ptr();
     a.rows = (uint64_t)x.rows;

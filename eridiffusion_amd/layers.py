@@ -4,7 +4,7 @@ generator, and the residual's addition with root-mean-square norm, each with its
 Tensors are float32 or bfloat16 on the GPU; the calls run on the current stream of their device and wait for nothing.
 `embedding`, `dropout` and `rms_norm` are differentiable: where an input requires a gradient, autograd records them.
 Forward-mode tangents are refused, and so are tracers (`torch.jit.trace`, `make_fx`, fake tensors): they record torch's operations,
-and these kernels are none.
+and these kernels are none.  An `out` that overlaps an input is refused too; only `dropout` may write over x itself.
 `embedding_grad` and `rms_norm_grad` are the backward passes themselves, for trainers that keep their own: the
 table's gradient may be float32 beside a bfloat16 table and may be accumulated over micro-batches, which is what
 `Adam8bit` takes as `.grad` as it stands.

@@ -131,3 +131,46 @@ def test_under_a_dispatch_mode_that_only_looks_on(layers):  # noqa: F811
         run(xs, ws).square().sum().backward()
         grads.append((xs.grad, ws.grad))
     assert torch.equal(grads[0][0], grads[1][0]) and torch.equal(grads[0][1], grads[1][1])
+
+
+def test_outputs_that_overlap_inputs_are_refused(layers):  # noqa: F811
+    w, g = _new(12, 40).cuda(), _new(12, 40).cuda()
+    ids = torch.randperm(12).cuda()
+    flat = _new(1000).cuda()
+    wide = _new(12, 90).cuda()
+    for what, call in [
+            ("weight", lambda: layers.embedding(ids, w, out=w)), ("weight", lambda: layers.embedding(ids[:5], w, out=w[:5])),
+            ("weight", lambda: layers.embedding(ids[:1], w, out=w[11:])), ("weight", lambda: layers.embedding(ids, wide[:, :40], out=wide[:, 39:79])),
+            ("weight", lambda: layers.embedding(ids, wide[:, 50:], out=wide[:, 11:51])), ("weight", lambda: layers.embedding(ids[:3], wide[:, :40], out=wide[::2][:3, 50:])),
+            ("ids", lambda: layers.embedding(flat[:24].view(torch.long), w, out=flat[20:500].view(12, 40))),
+            ("grad", lambda: layers.embedding_grad(ids, g, 12, out=g)), ("grad", lambda: layers.embedding_grad(ids[:6], g[:6], 6, out=g[5:11])),
+            ("grad", lambda: layers.embedding_grad(ids, g.view(BF)[:, :40], 12, out=g)),
+            ("grad", lambda: layers.embedding_grad(ids, wide[:, 45:85], 12, out=wide[:, 10:50], accumulate=True)),
+            ("ids", lambda: layers.embedding_grad(flat[476:500].view(torch.long), g, 12, out=flat[:480].view(12, 40))),
+            ("x", lambda: layers.dropout(w[1:], 0.5, 1, out=w[:-1])), ("x", lambda: layers.dropout(flat[1:], 0.5, 1, out=flat[:-1])),
+            ("x", lambda: layers.dropout(wide[:, :40], 0.5, 1, out=wide[:, 1:41])), ("x", lambda: layers.dropout(wide[:6, :40], 0.5, 1, out=wide[::2, :40])),
+            ("x", lambda: layers.dropout(flat[:480].view(12, 40), 0.5, 1, out=flat[:960].view(12, 80)[:, :40])),
+            ("offset", lambda: layers.dropout(w, 0.5, 1, flat[500:502].view(torch.long), out=flat[30:510].view(12, 40)))]:
+        before = [t.clone() for t in (w, g, flat, wide)]
+        with pytest.raises(ValueError, match="out overlaps " + what):
+            call()
+        assert all(torch.equal(a, b) for a, b in zip(before, (w, g, flat, wide)))
+
+
+def test_outputs_beside_their_inputs_are_not_refused(layers):  # noqa: F811
+    wide, ids = _new(12, 90).cuda(), torch.randperm(12).cuda()
+    a, b, one = wide[:, :40], wide[:, 40:80], wide[3, 80:].clone()
+    want = a[ids]
+    assert torch.equal(layers.embedding(ids, a, out=b), want)
+    want = layers.embedding_grad(ids, b, 12)
+    assert torch.equal(layers.embedding_grad(ids, b, 12, out=a), want)
+    want = layers.dropout(a, 0.5, 1)
+    assert torch.equal(layers.dropout(a, 0.5, 1, out=b), want) and torch.equal(layers.dropout(a, 0.5, 1, out=a), want)  # beside it, then over itself
+    assert torch.equal(layers.dropout(wide[:6, :40], 0.5, 2, out=wide[6:, :40]), layers.dropout(wide[:6, :40], 0.5, 2))  # rows behind
+    assert torch.equal(layers.embedding(ids[:1], a, out=wide[5:6, 50:]), a[ids[:1]]) and torch.equal(wide[3, 80:], one)  # one row between the others
+    assert torch.equal(layers.embedding(ids, wide[2:3, :40], out=wide[:, 45:85])[ids != 0], torch.zeros(11, 40, device="cuda"))  # and several beside one
+    square = _new(30, 30).cuda()
+    want = layers.dropout(square.t(), 0.5, 1)  # no rows: what the kernel reads is a copy
+    assert torch.equal(layers.dropout(square.t(), 0.5, 1, out=square), want)
+    empty = wide[:0]
+    assert layers.dropout(empty, 0.5, 1, out=empty) is empty
