@@ -294,10 +294,16 @@ int launch_rms_norm_grad(const EriRmsNormGrad &e, const Drop &d, uint32_t comput
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return (int)err;
     }
-    if (e.grad_weight && !few)
-        hipLaunchKernelGGL(rms_norm_grad_weight_kernel, dim3(padded / 64), dim3(1024), 0, s, partial, shape.groups, padded, e.grad_weight,
-                           (uint32_t)e.cols, (uint32_t)(e.grad_weight_dtype == ERI_DTYPE_F32));
-    return (int)hipGetLastError();
+    const uint32_t w32 = e.grad_weight_dtype == ERI_DTYPE_F32;
+    constexpr uint32_t kMost = 1u << 27; // columns of a launch: its threads are counted in 32 bits, 16 for each
+    for (uint32_t at = 0; e.grad_weight && !few && at < padded; at += kMost) {
+        const uint32_t now = padded - at < kMost ? padded - at : kMost;
+        hipLaunchKernelGGL(rms_norm_grad_weight_kernel, dim3(now / 64), dim3(1024), 0, s, partial + at, shape.groups, padded, (char *)e.grad_weight + (uint64_t)at * (w32 ? 4 : 2),
+                           (uint32_t)e.cols - at, w32);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return (int)err;
+    }
+    return 0;
 }
 
 } // namespace eri_layers

@@ -174,3 +174,15 @@ def test_outputs_beside_their_inputs_are_not_refused(layers):  # noqa: F811
     assert torch.equal(layers.dropout(square.t(), 0.5, 1, out=square), want)
     empty = wide[:0]
     assert layers.dropout(empty, 0.5, 1, out=empty) is empty
+
+
+@pytest.mark.parametrize("cols", [2 ** 27 + 70, 2 ** 28 + 100])
+def test_weight_gradient_of_a_very_long_row(layers, cols):  # noqa: F811
+    """16 threads to a column, and a launch counts its threads in 32 bits.  One row: each element is a product of three."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    g, h = (torch.randn(1, cols, generator=gen, device="cuda", dtype=BF) for _ in range(2))
+    got = layers.rms_norm_grad(g, h, torch.full((1,), 0.75, device="cuda"), torch.ones(cols, device="cuda"), needs=(False, False, True)).weight
+    for at in range(0, cols, 2 ** 26):
+        part = slice(at, at + 2 ** 26)
+        want = g[0, part].double() * h[0, part].double() * 0.75
+        assert bool(((got[part].double() - want).abs() <= 4 * U32 * want.abs()).all()), at
