@@ -343,12 +343,12 @@ template <typename TG, typename TO, int L, bool ACC, bool SHORT, bool ONCE> __gl
 /* Runs of several pieces: a wave looks for the one that begins in its places, as many as a piece is long, and sums its pieces
  * for 512 columns.  The pieces of a long one are shared out among the waves of the workgroup. */
 constexpr uint32_t kTeam = 16;
-template <typename TO, bool SHORT> __global__ __launch_bounds__(kTeam * kWave) void embedding_join_kernel(const GradArgs a) {
+template <typename TO, bool SHORT> __global__ __launch_bounds__(kTeam * kWave) void embedding_join_kernel(const GradArgs a, uint32_t first_team) {
     static_assert(kLogPieceMost <= 6, "a lane to a place");
     __shared__ Place runs[kTeam]; // token: where it begins
     __shared__ float sums[kTeam][512];
     const uint32_t used = *a.used, wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, tile = blockIdx.x % a.tiles;
-    const uint32_t begin = (blockIdx.x / a.tiles * kTeam + wave) << a.log_piece, piece = 1u << a.log_piece, col = tile * 512 + lane * 8;
+    const uint32_t begin = ((first_team + blockIdx.x / a.tiles) * kTeam + wave) << a.log_piece, piece = 1u << a.log_piece, col = tile * 512 + lane * 8;
     Place p = {0, 0, 1, 0};
     if (lane < piece && begin + lane < used) p = a.sorted[begin + lane];
     const bool found = p.at == 0 && p.run > piece; // one lane at most
@@ -566,7 +566,10 @@ template <typename TG, typename TO, int L, bool SHORT = false> void launch_sum(G
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, a);
     if (a.tokens <= piece) return;
     a.tiles = (a.dim + 511) / 512;
-    hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT>), dim3((a.tokens + kTeam * piece - 1) / (kTeam * piece) * a.tiles), dim3(kTeam * kWave), 0, s, a);
+    // teams of a launch, whose threads are counted in 32 bits; one launch up to 2^30 tokens of 512 columns
+    const uint32_t teams = (a.tokens + kTeam * piece - 1) / (kTeam * piece), most = a.tiles < 1u << 21 ? (1u << 21) / a.tiles : 1;
+    for (uint32_t at = 0; at < teams; at += most)
+        hipLaunchKernelGGL((embedding_join_kernel<TO, SHORT>), dim3((teams - at < most ? teams - at : most) * a.tiles), dim3(kTeam * kWave), 0, s, a, at);
 }
 template <typename TG, typename TO> void launch_sums(const GradArgs &a, hipStream_t s) {
     const uint32_t lanes = lanes_of(a.dim);

@@ -186,3 +186,16 @@ def test_weight_gradient_of_a_very_long_row(layers, cols):  # noqa: F811
         part = slice(at, at + 2 ** 26)
         want = g[0, part].double() * h[0, part].double() * 0.75
         assert bool(((got[part].double() - want).abs() <= 4 * U32 * want.abs()).all()), at
+
+
+def test_table_gradient_of_the_most_tokens(layers):  # noqa: F811
+    """2^31 - 1 of them, and the last to be joined stand in a launch of their own.  Sums of ones below 2^24 are exact."""
+    tokens, vocab = 2 ** 31 - 1, 1000
+    ids = torch.randint(0, vocab, (tokens,), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda", dtype=torch.int32)
+    ids[-5:] = vocab - 1
+    grad = torch.ones(tokens, 1, device="cuda", dtype=BF)
+    grad[-5:] = 3
+    got = layers.embedding_grad(ids, grad, vocab, dtype=F32)[:, 0]
+    want = sum(torch.bincount(part, minlength=vocab) for part in ids.split(2 ** 27))
+    want[vocab - 1] += 10
+    assert torch.equal(got.double(), want.double())
