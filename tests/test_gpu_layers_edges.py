@@ -6,7 +6,8 @@ import torch
 import torch.utils.checkpoint
 
 from oracle import layers_f64 as of
-from test_gpu_layers import BF, F32, OFFSET, SEED, U, U32, _depth, _ids, _near, _new, _norm_bounds, layers  # noqa: F401
+from test_gpu_layers import (BF, F8, F32, OFFSET, SEED, U, U32, _depth, _grad_inputs, _ids, _near, _new, _norm_bounds,
+                             layers)  # noqa: F401
 from test_layers_host import EmbeddingGrad, Norm, NormGrad
 
 pytestmark = pytest.mark.gpu
@@ -199,3 +200,112 @@ def test_table_gradient_of_the_most_tokens(layers):  # noqa: F811
     want = sum(torch.bincount(part, minlength=vocab) for part in ids.split(2 ** 27))
     want[vocab - 1] += 10
     assert torch.equal(got.double(), want.double())
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# launches and layouts that only certain sizes reach
+# ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,out", [(BF, BF), (BF, F32), (F32, F32)])
+@pytest.mark.parametrize("tokens,vocab,dim,common", [(20000, 5000, 16, 0.9), (12000, 900, 40, 1.0), (30001, 3000, 300, 0.6)])
+def test_table_gradient_of_a_batch_with_most_tokens_on_one_id(layers, dtype, out, tokens, vocab, dim, common):  # noqa: F811
+    """More than 512 tokens of a bucket in a wave's share of the ids: the sort looks at them a second time."""
+    ids, grad = _ids(tokens, vocab, common=common), _new(tokens, dim, dtype=dtype)
+    share = (tokens + 1023) // 1024 * 64
+    assert int((ids[share:2 * share] == vocab // 2).sum()) > 512
+    deep = int((ids == vocab // 2).sum()) + 4
+    for pad in (None, 3):
+        want, size = of.embedding_grad(ids, grad, vocab, 0.75, pad)
+        got = layers.embedding_grad(ids.cuda(), grad.cuda(), vocab, 0.75, padding_id=pad, dtype=out)
+        _near(got, want, U[out] * want.abs() + deep * U32 * size, pad)
+        assert torch.equal(got, layers.embedding_grad(ids.int().cuda(), grad.cuda(), vocab, 0.75, padding_id=pad, dtype=out))
+        old = _new(vocab, dim, dtype=out, seed=3)
+        into = layers.embedding_grad(ids.cuda(), grad.cuda(), vocab, 0.75, padding_id=pad, out=old.cuda(), accumulate=True)
+        _near(into, want + old.double(), U[out] * (want + old.double()).abs() + (deep + 1) * U32 * (size + old.double().abs()), "accumulate")
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("out,vocab", [(BF, 270000), (F32, 140000)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_table_gradient_that_reads_grad_past_the_caches(layers, dtype, out, vocab, accumulate):  # noqa: F811
+    """A table of more than 256 MB, rows of an odd length in two tiles, runs of one piece and of many."""
+    tokens, dim, some = 3000, 513, 400
+    rows = torch.randperm(vocab, generator=torch.Generator().manual_seed(1))[:some].sort().values  # the rows that are named
+    local, grad = _ids(tokens, some, common=0.3, outside=False), _new(tokens, dim, dtype=dtype)
+    ids = torch.where(torch.arange(tokens) % 97 == 5, -1, rows[local])
+    want, size = of.embedding_grad(torch.where(ids < 0, -1, local), grad, some, 1.5)
+    deep = int(torch.bincount(local).max()) + 5
+    table = torch.full((vocab, dim), 2.0, dtype=out, device="cuda") if accumulate else None
+    got = layers.embedding_grad(ids.cuda(), grad.cuda(), vocab, 1.5, dtype=out, out=table, accumulate=accumulate)
+    base = 2.0 if accumulate else 0.0
+    _near(got[rows.cuda()], want + base, U[out] * (want + base).abs() + deep * U32 * (size + base))
+    rest = torch.ones(vocab, dtype=torch.bool, device="cuda")
+    rest[ids[ids >= 0].cuda()] = False
+    assert bool((got[rest] == base).all())
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("tokens,dim", [(140000, 40), (140000, 7), (40000, 200), (4500, 1300), (5000, 4099), (2 ** 22 + 5, 8), (2 ** 22 + 5, 70)])
+def test_lookup_of_many_tokens(layers, dtype, tokens, dim):  # noqa: F811
+    """Several rows at a time in a thread, for each number of lanes to a row, and more tokens than a launch takes."""
+    w, ids = _new(300, dim, dtype=dtype).cuda(), _ids(tokens, 300).cuda()
+    fits = (ids >= 0) & (ids < 300)
+    want = torch.where(fits[:, None], w[torch.where(fits, ids, 0)], 0)
+    for some in (ids, ids.int()):
+        assert torch.equal(layers.embedding(some, w), want)
+    back = torch.full((tokens, dim + 3), 7.0, dtype=dtype, device="cuda")
+    layers.embedding(ids, w, 2.0, out=back[:, 1:dim + 1])
+    assert torch.equal(back[:, 1:dim + 1], want * 2) and bool((back[:, 0] == 7).all()) and bool((back[:, dim + 1:] == 7).all())
+
+
+@pytest.mark.parametrize("group", [0, 128])
+def test_norm_of_more_rows_than_a_launch_takes(layers, group):  # noqa: F811
+    rows, cols = 2 ** 21 + 5, 8
+    x, r, w = _new(rows, cols, dtype=BF), _new(rows, cols, dtype=BF, seed=1), _new(cols, std=0.3, mean=1.0)
+    y, h, rstd = of.rms_norm(x, w, 1e-6, r, 0.3, SEED, OFFSET)
+    off_h, off_y = _norm_bounds(x, w, r, 0.3, y, h, rstd, cols)
+    got = layers.rms_norm(x.cuda(), w.cuda(), 1e-6, residual=r.cuda(), p=0.3, seed=SEED, offset=OFFSET)
+    _near(got.y, y, U[BF] * y.abs() + off_y, "y")
+    _near(got.h, h, U[BF] * h.abs() + off_h, "h")
+    _near(got.rstd, rstd, rstd * U32 * (_depth(cols) + 8) + rstd ** 3 * (off_h * h.abs()).mean(-1), "rstd")
+    whole = layers.rms_norm(x.cuda(), w.cuda(), dtype=F8, scale_group=group)
+    for part in (slice(0, 70), slice(2 ** 21 - 9, 2 ** 21 + 5)):
+        some = layers.rms_norm(x[part].cuda(), w.cuda(), dtype=F8, scale_group=group)
+        assert torch.equal(whole.y[part].view(torch.uint8), some.y.view(torch.uint8))
+        assert torch.equal(whole.scales[part], some.scales) and torch.equal(whole.rstd[part], some.rstd)
+
+
+@pytest.mark.parametrize("cols", [1025, 1281, 2048, 2500, 4095, 5001, 6144, 6150, 8192, 9001, 12288, 12290])
+@pytest.mark.parametrize("dtype,out", [(BF, BF), (BF, F8), (F32, BF), (F32, F32)])
+@pytest.mark.parametrize("p", [0.0, 0.3])
+def test_norm_without_a_residual(layers, cols, dtype, out, p):  # noqa: F811
+    """Layouts of their own where the row moves few bytes."""
+    rows = 5
+    x, w = _new(rows, cols, dtype=dtype), _new(cols, dtype=dtype, std=0.3, mean=1.0)
+    y, h, rstd = of.rms_norm(x, w, 1e-6, None, p, SEED, OFFSET)
+    off_h, off_y = _norm_bounds(x, w, None, p, y, h, rstd, cols)
+    got = layers.rms_norm(x.cuda(), w.cuda(), 1e-6, p=p, seed=SEED, offset=OFFSET, dtype=out)
+    _near(got.rstd, rstd, rstd * U32 * (_depth(cols) + 8) + rstd ** 3 * (off_h * h.abs()).mean(-1), "rstd")
+    _near(got.h, h, U[dtype] * h.abs() + off_h, "h")
+    if out != F8:
+        _near(got.y, y, U[out] * y.abs() + off_y, "y")
+        return
+    scales = of.scales_of(y, 0)
+    off_scales = off_y.amax(-1, keepdim=True) / of.F8_MAX + 2 * U32 * scales
+    _near(got.scales, scales, off_scales, "scales")
+    q = y / scales
+    step = torch.exp2(torch.floor(torch.log2(q.abs().clamp(min=2.0 ** -6))) - 3)
+    _near(got.y.float(), q, 0.5 * step + 2 * (off_y / scales + q.abs() * (off_scales / scales + 3 * U32)), "codes")
+
+
+@pytest.mark.parametrize("rows,cols", [(2000, 200), (2000, 400), (1537, 129), (1600, 512), (600, 9001), (800, 9001), (770, 16384)])
+@pytest.mark.parametrize("dtype,stream,w", [(BF, BF, F32), (F32, F32, F32), (BF, F32, BF)])
+def test_norm_gradient_of_more_rows_than_workgroups(layers, rows, cols, dtype, stream, w):  # noqa: F811
+    """Every width whose sums the waves of a workgroup join, and long rows several to a workgroup, in one launch and in two."""
+    gy, h, rstd, weight, gh = _grad_inputs(rows, cols, dtype, stream, w)
+    dx, dr, dw, size, size_w = of.rms_norm_grad(gy, h, rstd, weight, gh, 0.3, SEED, OFFSET)
+    got = layers.rms_norm_grad(gy.cuda(), h.cuda(), rstd.cuda(), weight.cuda(), grad_h=gh.cuda(), p=0.3, seed=SEED, offset=OFFSET, dtype=dtype)
+    off = U32 * (_depth(cols) + 12) * size
+    _near(got.residual, dr, U[stream] * dr.abs() + off, "residual")
+    _near(got.x, dx, U[dtype] * dx.abs() + 1.5 * off + 2 * U32 * dx.abs(), "x")
+    _near(got.weight, dw, U[w] * dw.abs() + U32 * (rows + 130) * size_w, "weight")
