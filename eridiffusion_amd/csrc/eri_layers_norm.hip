@@ -16,6 +16,10 @@
  *   bf16 to bf16    2560 16.4, was 19.6;   4096 21.5, 22.9;   5120 30.1, 35.6;   8192 44.7, 52.5;   12288 72.9, 80.4
  *   fp32 to bf16    2560 22.9, was 26.2;   4096 32.8, 32.5;   5120 41.6, 43.8;   8192 72.4, 76.2;   12288 105.9, 117.7
  *   bf16 to fp32    2560 22.2, not so 22.8; 4096 37.3, 35.3; 5120 45.3, 47.7; 8192 76.8, 75.6;   2048 19.5, 18.1: not worth it
+ * and of 1025 to 2048 columns, 32768 rows: 128 threads with two vectors each, before them 256 with one:
+ *   bf16 to 8 bits  1100 39.1, was 49.1;   1536 38.5, 48.7;   2048 40.4, 49.4
+ *   bf16 to bf16    1100 38.3, was 45.9;   1536 37.9, 45.1;   2048 44.9, 48.3
+ *   fp32 to bf16    1100 40.0, was 47.2;   1536 48.7, 52.9;   2048 68.1, 67.6
  * A row's layout, and so its rounding, does not depend on how many rows there are.
  * Dropout is drawn beside the loads and costs nothing: 16384 x 4096 bf16 with residual and dropout 91 us, 5.9 TB/s (a copy of that
  * size runs at 5.2); 8192 x 5120 to 8 bits 51-57 us, 5.2-5.8 TB/s; one row of 4096 2.2 us, a launch and two trips to memory.

@@ -148,7 +148,7 @@ __global__ __launch_bounds__(TPR < 256 ? 256 : TPR) void rms_norm_grad_kernel(co
 }
 
 /* Rows too long for registers (with 32 elements of four rows in each of 1024 threads the compiler spills 200 of them, and 4096 x 20000
- * bf16 took 535 us; this takes 254): read twice, and the sums of grad_weight kept in the workgroup's row of partial. */
+ * bf16 took 535 us; this takes 254; with 16 elements, up to 16384 columns, it spills two, in fp32 only): read twice, and the sums of grad_weight kept in the workgroup's row of partial. */
 template <typename TG, typename TR, bool DROP> __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(const NormGradArgs a) {
     __shared__ float slots[2][16];
     const uint64_t offset = DROP ? drop_offset(a.drop) : 0;
@@ -221,7 +221,9 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_weight_kernel(const float 
 }
 
 /* Few rows: grad_weight comes out of the same launch, from workgroups that read grad and h once more, instead of a second one
- * over the sums that the rows' workgroups leave.  us, one launch | two, at so many rows:
+ * over the sums that the rows' workgroups leave.  One line for all widths over 512 columns lies between those where one launch
+ * wins for longer (4096 bf16) and those where it stops winning earlier (8192 fp32), 2 us to either side.  us, one launch | two, at so
+ * many rows:
  *   rows            128          512          768          1024         1536
  *   256 bf16     5.8 | 9.0    5.8 | 9.1    6.0 | 9.0    5.9 | 9.1    6.1 | 9.3
  *   1024 fp32    5.8 | 8.9    5.6 | 8.9    6.6 | 8.8    8.7 | 9.2   11.3 | 10.4

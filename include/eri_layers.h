@@ -50,7 +50,7 @@ int eri_embedding(const EriEmbedding *args, void *stream);
  * rows that no token names with zeros.  accumulate: the sum is added to what out holds, and rows without a token are
  * not touched.  Tokens whose id is padding_id or lies outside [0, vocab) add nothing.  The workspace that some tokens need does
  * for fewer tokens of the same table too.  Sums are F32 in an order that
- * the sizes alone decide: the same inputs give the same bits.
+ * the sizes and accumulate decide: the same call on the same inputs gives the same bits.
  * ------------------------------------------------------------------------------------------- */
 typedef struct EriEmbeddingGrad {
     const void *ids;
@@ -104,8 +104,10 @@ int eri_dropout(const EriDropout *args, void *stream);
  *     h = residual + dropout(x)           rstd = 1 / sqrt(mean of h^2 over the row + eps)
  *     y = h * rstd * weight               (from h before it is rounded to its dtype)
  * with y in F32, BF16, or F8E4M3 with scales: for each row (scale_group 0) or each 128 columns of a row (scale_group
- * 128, the last group of a row may be shorter) scale = max|y| / 448, or 1 where max|y| is below 2^-100, and the 8-bit
- * value is y / scale rounded to nearest even.  NaN is left out of max|y| and stays NaN.
+ * 128, the last group of a row may be shorter) scale = max|y| / 448, or 1 where max|y| is below 2^-100.  The 8-bit value
+ * is y * (448 / max|y|) (y itself where the scale is 1 for that reason), computed in F32 and rounded to nearest even: where y / scale
+ * lies within F32's rounding of the middle between two 8-bit values it may be either.  NaN is left out of max|y| and
+ * stays NaN.
  * ------------------------------------------------------------------------------------------- */
 typedef struct EriRmsNorm {
     const void *x;        /* rows of cols elements */
@@ -128,9 +130,9 @@ int eri_rms_norm(const EriRmsNorm *args, void *stream);
 /* Its gradient, from grad = dL/dy and grad_h = dL/dh (what reaches h besides the norm; NULL: nothing):
  *     dh = grad_h + rstd * (grad * weight) - h * rstd^3 * mean(grad * weight * h)
  *     grad_residual = dh     grad_x = dropout(dh)     grad_weight = sum over rows of grad * h * rstd
- * Any of the three outputs may be NULL.  Sums are F32; grad_weight's order is decided by the sizes and the device's
- * number of compute units: the same inputs give the same bits.  The workspace that some rows need does for fewer rows of the
- * same length too. */
+ * Any of the three outputs may be NULL.  Sums are F32; grad_weight's order is decided by the sizes, the device's
+ * number of compute units and whether an output lies over grad, h or weight: the same call on the same inputs gives the
+ * same bits.  The workspace that some rows need does for fewer rows of the same length too. */
 typedef struct EriRmsNormGrad {
     const void *grad;
     const void *h;
