@@ -1,31 +1,15 @@
 /*
  * Host side of include/eri_layers.h: checks the arguments, then launches.  Nothing is allocated and nothing waits.
  */
-#include <hip/hip_runtime.h>
-
 #include <atomic>
 #include <cmath>
-#include <cstdio>
-#include <string>
 
 #include "eri_layers_device.h"
+#include "eri_layers_host.h"
 
 namespace {
 
 using eri_layers::Drop;
-
-int fail(int code, const char *msg) {
-    eri_set_last_error(msg);
-    return code;
-}
-int fail(int code, const char *call, const char *what) {
-    char buf[160];
-    std::snprintf(buf, sizeof buf, "%s: %s", call, what);
-    return fail(code, buf);
-}
-int done(int hip_error, const char *call) {
-    return hip_error == 0 ? 0 : fail(hip_error, call, hipGetErrorString((hipError_t)hip_error));
-}
 
 /* Compute units of the current device, asked for once. */
 int compute_units(uint32_t *out, const char *call) {
@@ -48,19 +32,6 @@ int compute_units(uint32_t *out, const char *call) {
     return 0;
 }
 
-constexpr uint64_t kCountMost = 0x7fffffffull;                 // rows, columns, tokens, ids
-constexpr uint64_t kStrideMost = (uint64_t)1 << 40;            // so that no offset leaves 64 bits
-
-bool floating(int tag) { return tag == ERI_DTYPE_F32 || tag == ERI_DTYPE_BF16; }
-uint32_t size_of(int tag) { return tag == ERI_DTYPE_F32 ? 4 : tag == ERI_DTYPE_BF16 ? 2 : 1; }
-bool aligned(const void *p, uint32_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-
-/* Sets a stride of 0 to the row's length and refuses one that is shorter. */
-bool stride(uint64_t *s, uint64_t cols) {
-    if (*s == 0) *s = cols;
-    return *s >= cols && *s <= kStrideMost;
-}
-
 int key_of(const EriDropoutKey &k, Drop *d, const char *call) {
     if (!(k.p >= 0.0 && k.p <= 1.0)) return fail(ERI_ERR_ARG, call, "p is not between 0 and 1");
     if (!aligned(k.offset_ptr, 8)) return fail(ERI_ERR_ALIGN, call, "offset_ptr is not 8-byte aligned");
@@ -71,11 +42,6 @@ int key_of(const EriDropoutKey &k, Drop *d, const char *call) {
     d->scale = d->below < 65536 ? (float)(65536.0 / (65536.0 - d->below)) : 0.0f;
     return 0;
 }
-
-#define ERI_NEED(cond, code, what) \
-    do {                           \
-        if (!(cond)) return fail(code, kCall, what); \
-    } while (0)
 
 int ids_ok(const void *ids, int ids_64, uint64_t tokens, uint64_t vocab, uint64_t dim, const char *kCall) {
     ERI_NEED(ids || tokens == 0, ERI_ERR_NULL, "ids is NULL");

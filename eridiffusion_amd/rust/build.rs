@@ -47,6 +47,10 @@ fn main() {
         ("eri_layers_norm.hip", "layers_norm", "", true),
         ("eri_layers_norm_grad.hip", "layers_norm_grad", "", true),
         ("eri_layers_embedding.hip", "layers_embedding", "", true),
+        ("eri_losses_api.cpp", "losses_api", "", true),
+        ("eri_losses_score.hip", "losses_score", "", true),
+        ("eri_losses_distill.hip", "losses_distill", "", true),
+        ("eri_losses_grad.hip", "losses_grad", "", true),
     ] {
         let obj = out.join(format!("{obj_name}.o"));
         let mut cmd = Command::new(&hipcc);
@@ -72,7 +76,7 @@ fn main() {
     println!("cargo:rustc-link-search=native=/opt/rocm/lib");
     println!("cargo:rustc-link-lib=dylib=amdhip64");
     println!("cargo:rustc-link-lib=dylib=stdc++");
-    for h in ["eri_adam8_device.h", "eri_adam8_inline.h", "eri_dynamic_maps.inc", "eri_layers_device.h"] {
+    for h in ["eri_adam8_device.h", "eri_adam8_inline.h", "eri_dynamic_maps.inc", "eri_layers_device.h", "eri_layers_host.h", "eri_losses_device.h"] {
         println!("cargo:rerun-if-changed=csrc/{h}");
     }
 }
