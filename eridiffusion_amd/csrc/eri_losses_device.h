@@ -33,6 +33,37 @@ template <typename T> __device__ __forceinline__ void load_last(float (&v)[8], c
     for (uint32_t e = 0; e < 8; ++e) v[e] = e < n ? r.get(e) : -kInf;
 }
 
+/* Vectors first .. last-1 of a row, dealt to TPR threads in turn, N of each at a time: all loads of a batch are under way before the first is
+ * wanted.  `use(values, at, full)` gets an array of C vectors, those that begin at vector at + k TPR + t; in the last of them there is nothing but
+ * minus infinity for threads past the end, unless `full`.  The rest of the row is one smaller batch: vector by vector it took a trip to memory for each. */
+template <int TPR, int C, bool FULL, typename T, typename Use> __device__ __forceinline__ void walk_batch(const T *row, uint32_t at, uint32_t last, uint32_t t, Use &use) {
+    Raw<T> raw[C];
+    float v[C][8];
+#pragma unroll
+    for (int k = 0; k < C; ++k) {
+        const uint32_t vec = at + k * TPR + t;
+        if (FULL || k < C - 1) raw[k].load(row + (uint64_t)vec * 8);
+        else {
+            all_least(raw[k]);
+            if (vec < last) raw[k].load(row + (uint64_t)vec * 8);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < C; ++k) values_of(v[k], raw[k]);
+    use(v, at, FULL);
+}
+template <int TPR, typename T, typename Use> __device__ __forceinline__ void walk(const T *row, uint32_t first, uint32_t last, uint32_t t, Use use) {
+    constexpr int N = sizeof(T) == 2 ? 4 : 2; // 64 bytes of a row for each thread
+    uint32_t at = first;
+    for (; at + N * TPR <= last; at += N * TPR) walk_batch<TPR, N, true>(row, at, last, t, use);
+    if (at >= last) return;
+    const uint32_t left = (last - at + TPR - 1) / TPR;
+    if (left == 1) walk_batch<TPR, 1, false>(row, at, last, t, use);
+    else if (N == 2 || left == 2) walk_batch<TPR, 2, false>(row, at, last, t, use);
+    else if (left == 3) walk_batch<TPR, 3, false>(row, at, last, t, use);
+    else walk_batch<TPR, 4, false>(row, at, last, t, use);
+}
+
 /* The running softmax: m the largest logit, s the sum of exp((x - m) / T), t the sum of exp((x - m) / T) (x - m), whose terms are all
  * of one sign, so that the entropy ln s - t / (s T) loses nothing.  c = log2(e) / T.  Differences are taken before they are scaled: x c - m c in
  * one fused product would overflow for the lowest values of a type, which stand for masks, and round m c on the way. */
@@ -48,7 +79,7 @@ template <bool ENT> __device__ __forceinline__ void scale_to(Sums &a, float m, f
     a.s *= f;
     a.m = m;
 }
-template <bool ENT, int N> __device__ __forceinline__ void add(Sums &a, const float (&v)[N][8], float c) {
+template <bool ENT, int N> __device__ __forceinline__ void add(Sums &a, float (&v)[N][8], float c) {
     float m = a.m;
 #pragma unroll
     for (int k = 0; k < N; ++k) m = fmaxf(m, largest(v[k]));

@@ -85,8 +85,8 @@ template <typename T, bool REST> __device__ __forceinline__ void finish(const Di
 }
 
 template <typename T, int TPR, bool REST, bool SPLIT> __global__ __launch_bounds__(TPR) void distill_kernel(const DistillArgs a) {
-    constexpr int WAVES = TPR / (int)kWave, N = sizeof(T) == 2 ? 4 : 2;
-    constexpr uint32_t kTurns = 64, kSegment = kTurns * TPR; // vectors whose bits a thread holds at a time
+    constexpr int WAVES = TPR / (int)kWave;
+    constexpr uint32_t kTurns = TPR > 256 ? 32 : 64, kSegment = kTurns * TPR; // vectors whose bits a thread holds at a time
     __shared__ Sums slots[WAVES];
     __shared__ uint32_t named[REST ? kSegment / 4 : 1], hits[REST ? 2 * TPR : 1];
     const uint32_t t = threadIdx.x, slice = SPLIT ? blockIdx.x % a.slices : 0;
@@ -126,36 +126,20 @@ template <typename T, int TPR, bool REST, bool SPLIT> __global__ __launch_bounds
             for (uint32_t e = 0; e < 8; ++e)
                 if (which >> e & 1) v[e] = -kInf;
         };
-        uint32_t at = begin;
-        for (; at + N * TPR <= last; at += N * TPR) {
-            Raw<T> raw[N];
-            float v[N][8];
-#pragma unroll
-            for (int k = 0; k < N; ++k) raw[k].load(row + (uint64_t)(at + k * TPR + t) * 8);
-#pragma unroll
-            for (int k = 0; k < N; ++k) values_of(v[k], raw[k]);
+        walk<TPR>(row, begin, last, t, [&](auto &v, uint32_t at, bool) {
             if (REST) {
                 const uint32_t bits = (uint32_t)(mine >> ((at - begin) / TPR));
 #pragma unroll
-                for (int k = 0; k < N; ++k)
-                    if (bits >> k & 1) leave_out(v[k], at - begin + k * TPR + t);
+                for (uint32_t k = 0; k < sizeof v / sizeof v[0]; ++k)
+                    if (bits >> k & 1) leave_out(v[k], at - begin + k * TPR + t); // the last, shorter vector has its turn below
             }
-            add<false, N>(r, v, a.c);
-        }
-        for (; at < last; at += TPR) {
-            float v[1][8];
-            Raw<T> raw;
-            all_least(raw);
-            if (at + t < last) raw.load(row + (uint64_t)(at + t) * 8);
-            values_of(v[0], raw);
-            if (REST && at + t < last && (mine >> ((at - begin) / TPR) & 1)) leave_out(v[0], at - begin + t);
-            add<false, 1>(r, v, a.c);
-        }
+            add<false>(r, v, a.c);
+        });
         if (stop > whole && t == (whole - begin) % TPR) { // the row's last vector, of less than eight elements
             float v[1][8];
             load_last(v[0], row + (uint64_t)whole * 8, a.vocab % 8);
             if (REST && (mine >> ((whole - begin) / TPR) & 1)) leave_out(v[0], whole - begin);
-            add<false, 1>(r, v, a.c);
+            add<false>(r, v, a.c);
         }
         if (REST) __syncthreads(); // the bytes have been read
     }

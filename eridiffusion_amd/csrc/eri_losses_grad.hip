@@ -24,30 +24,16 @@ struct GradArgs {
 };
 
 template <typename T, typename O, int TPR, typename Of> __device__ __forceinline__ void each(const T *row, O *out, uint32_t first, uint32_t end, uint32_t vocab, uint32_t t, Of of) {
-    constexpr int N = sizeof(T) == 2 ? 4 : 2;
     const uint32_t whole = vocab / 8, last = end < whole ? end : whole;
-    uint32_t at = first;
-    for (; at + N * TPR <= last; at += N * TPR) {
-        Raw<T> raw[N];
+    walk<TPR>(row, first, last, t, [&](auto &v, uint32_t at, bool full) {
+        constexpr uint32_t C = sizeof v / sizeof v[0];
 #pragma unroll
-        for (int k = 0; k < N; ++k) raw[k].load(row + (uint64_t)(at + k * TPR + t) * 8);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            float v[8];
-            values_of(v, raw[k]);
-            of(v, (at + k * TPR + t) * 8);
-            store_n(out + (uint64_t)(at + k * TPR + t) * 8, 8, v);
+        for (uint32_t k = 0; k < C; ++k) {
+            const uint32_t vec = at + k * TPR + t;
+            of(v[k], vec * 8);
+            if (full || k < C - 1 || vec < last) store_n(out + (uint64_t)vec * 8, 8, v[k]);
         }
-    }
-    for (; at < last; at += TPR)
-        if (at + t < last) {
-            Raw<T> raw;
-            raw.load(row + (uint64_t)(at + t) * 8);
-            float v[8];
-            values_of(v, raw);
-            of(v, (at + t) * 8);
-            store_n(out + (uint64_t)(at + t) * 8, 8, v);
-        }
+    });
     if (end > whole && t == (whole - first) % TPR) {
         float v[8];
         load_last(v, row + (uint64_t)whole * 8, vocab % 8);

@@ -3,15 +3,16 @@
  *
  * Alternatives.  Every thread remembers the largest logit that it has seen and the vector that held it.  The k-th largest of these (value,
  * vector) pairs is a bound: k threads have an element above it or on it, so that whatever is below is not among the k largest, and only those k threads
- * can have seen one of them.  Their vectors, k of TPR of the row, are read once more, from the caches, and what passes the bound (about
- * k elements) is sorted: 64 keys of 64 bits to a wave, by a bitonic network over its lanes.
+ * can have seen one of them.  Each thread also leaves the largest of every few of its vectors in LDS (16 bits, rounded up); where that reaches the
+ * bound, in little more than k places, the vectors are read once more, from the caches, and what passes the bound (about k elements) is sorted: 64 keys
+ * of 64 bits to a wave, by a bitonic network over its lanes.
  */
 #include "eri_losses_device.h"
 
 namespace eri_losses {
 namespace {
 
-constexpr uint32_t kFound = 1024; // elements that pass the bound and are kept at a time
+constexpr uint32_t kFound = 256; // elements that pass the bound and are kept at a time
 
 struct ScoreArgs {
     const void *logits, *ids;
@@ -52,33 +53,67 @@ template <typename T> __device__ __forceinline__ bool token_of(const ScoreArgs &
     return true;
 }
 
+constexpr uint32_t kMarks = 8192; // largest values of a few vectors each, over all threads
 template <int TPR> struct TopSpace {
-    Key lists[TPR], found[kFound];
+    uint16_t marks[kMarks];
+    union {
+        Key lists[TPR];
+        Key found[kFound];
+    };
+    uint16_t places[kWave * (kMarks / TPR)]; // marks that reach the bound: only k threads have any
     Key bound;
-    uint32_t chosen[kWave], chosen_n, count;
+    uint32_t places_n, count;
 };
 
-/* The row's (or slice's) largest elements in the lanes of the first wave, in descending order.  `best` is the largest of this thread's elements and
- * `place` its first vector that holds it; vectors first .. end-1 are dealt to the threads in turn. */
-template <typename T, int TPR> __device__ __forceinline__ Key largest_of(const T *row, float best, uint32_t place, uint32_t first, uint32_t end, uint32_t vocab, uint32_t top_n, TopSpace<TPR> &sp) {
-    const uint32_t t = threadIdx.x, lane = t % kWave, whole = vocab / 8;
-    Key k = first + t < end ? key_of(best, place) : 0;
+/* The upper 16 bits of a value, rounded up. */
+__device__ __forceinline__ uint32_t mark_of(float v, bool exact) {
+    const uint32_t u = as_bits(v);
+    return exact || (int32_t)u < 0 ? u >> 16 : (u + 0xffffu) >> 16;
+}
+
+/* What a thread knows of its elements: the largest, its first vector that holds it, and the largest of every `each` of its vectors (a power
+ * of two), which it leaves in marks[turn / each]. */
+template <typename T, int TPR> struct Seen {
+    float best, run;
+    uint32_t place;
+    __device__ __forceinline__ void take(const float (&v)[8], uint32_t vec) {
+        const float m = largest(v);
+        if (m > best) best = m, place = vec;
+        run = fmaxf(run, m);
+    }
+    /* after each one or two vectors from `turn` on */
+    __device__ __forceinline__ void mark(TopSpace<TPR> &sp, uint32_t turn, uint32_t shift) {
+        sp.marks[(turn >> shift) * TPR + threadIdx.x] = (uint16_t)mark_of(run, sizeof(T) == 2);
+        if (((turn + 2) & ((1u << shift) - 1)) < 2) run = -kInf;
+    }
+};
+
+/* The row's (or slice's) largest elements in the lanes of the first wave, in descending order; vectors first .. end-1 are dealt to the threads in turn. */
+template <typename T, int TPR> __device__ __forceinline__ Key largest_of(const T *row, const Seen<T, TPR> &seen, uint32_t shift, uint32_t first, uint32_t end, uint32_t vocab, uint32_t top_n, TopSpace<TPR> &sp) {
+    constexpr uint32_t WAVES = TPR / kWave;
+    const uint32_t t = threadIdx.x, lane = t % kWave, wave = t / kWave, whole = vocab / 8;
+    const Key own = first + t < end ? key_of(seen.best, seen.place) : 0;
+    Key k = own;
     sort64(k, lane);
-    if (TPR > (int)kWave) {
-        sp.lists[t] = k;
+    if (WAVES > 1) sp.lists[t] = k;
+    for (uint32_t half = WAVES / 2; half > 0; half /= 2) {
         __syncthreads();
+        if (wave < half) {
+            merge64(k, sp.lists[(wave + half) * kWave + (kWave - 1 - lane)], lane);
+            sp.lists[t] = k;
+        }
     }
-    if (t < kWave) {
-#pragma unroll 1
-        for (uint32_t w = 1; w < TPR / kWave; ++w) merge64(k, sp.lists[w * kWave + (kWave - 1 - lane)], lane);
-        const uint32_t n = (uint32_t)__popcll(__ballot(lane < top_n && k != 0));
-        if (lane < n) sp.chosen[lane] = (place_of(k) - first) % TPR;
-        if (lane == top_n - 1) sp.bound = k; // 0, which all pass, where fewer threads have seen anything
-        if (lane == 0) sp.chosen_n = n;
-    }
+    if (t == top_n - 1) sp.bound = k; // 0, which all pass, where fewer threads have seen anything
+    if (t == 0) sp.places_n = 0;
     __syncthreads();
-    const uint32_t n = sp.chosen_n, total = n * ((end - first + TPR - 1) / TPR);
     const Key bound = sp.bound;
+    const uint32_t turns = (end - first + TPR - 1) / TPR;
+    const float least = bound ? value_of(bound) : -kInf;
+    if (own >= bound && own != 0) // one of top_n threads; marks of vectors behind the end hold anything, and lead nowhere
+        for (uint32_t i = 0; i << shift < turns; ++i)
+            if (as_float((uint32_t)sp.marks[i * TPR + t] << 16) >= least) sp.places[atomicAdd(&sp.places_n, 1u)] = (uint16_t)(i * TPR + t);
+    __syncthreads();
+    const uint32_t total = sp.places_n << shift;
     uint32_t per = total;
     Key top = 0;
     for (uint32_t from = 0; from < total;) {
@@ -86,7 +121,7 @@ template <typename T, int TPR> __device__ __forceinline__ Key largest_of(const T
         __syncthreads();
         const uint32_t to = per < total - from ? from + per : total;
         for (uint32_t j = from + t; j < to; j += TPR) {
-            const uint32_t vec = first + sp.chosen[j % n] + j / n * TPR;
+            const uint32_t place = sp.places[j >> shift], vec = first + place % TPR + ((place / TPR << shift) + (j & ((1u << shift) - 1))) * TPR;
             if (vec >= end) continue;
             float v[8];
             if (vec < whole) {
@@ -122,7 +157,7 @@ template <typename T, int TPR> __device__ __forceinline__ Key largest_of(const T
 }
 
 template <typename T, int TPR, bool ENT, bool TOP, bool SPLIT> __global__ __launch_bounds__(TPR) void score_kernel(const ScoreArgs a) {
-    constexpr int WAVES = TPR / (int)kWave, N = sizeof(T) == 2 ? 4 : 2;
+    constexpr int WAVES = TPR / (int)kWave;
     __shared__ Sums slots[WAVES];
     __shared__ char space[TOP ? sizeof(TopSpace<TPR>) : 1] __attribute__((aligned(16)));
     const uint32_t t = threadIdx.x, slice = SPLIT ? blockIdx.x % a.slices : 0;
@@ -134,48 +169,37 @@ template <typename T, int TPR, bool ENT, bool TOP, bool SPLIT> __global__ __laun
     const uint32_t first = SPLIT ? slice * a.per : 0, end = SPLIT && all - first > a.per ? first + a.per : all, last = end < whole ? end : whole;
 
     Sums r = {kLowest, 0.0f, 0.0f};
-    float best = -kInf;
-    uint32_t place = first + t;
-    uint32_t at = first;
-    for (; at + N * TPR <= last; at += N * TPR) {
-        Raw<T> raw[N];
-        float v[N][8];
+    Seen<T, TPR> seen = {-kInf, -kInf, first + t};
+    TopSpace<TPR> &sp = *reinterpret_cast<TopSpace<TPR> *>(space);
+    uint32_t shift = 1; // so that the marks suffice
+    while (TOP && (a.per / TPR) >> shift >= kMarks / TPR) ++shift;
+    walk<TPR>(row, first, last, t, [&](auto &v, uint32_t at, bool) {
+        constexpr uint32_t C = sizeof v / sizeof v[0];
+        if (TOP)
 #pragma unroll
-        for (int k = 0; k < N; ++k) raw[k].load(row + (uint64_t)(at + k * TPR + t) * 8);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            values_of(v[k], raw[k]);
-            if (TOP) {
-                const float m = largest(v[k]);
-                if (m > best) best = m, place = at + k * TPR + t;
+            for (uint32_t k = 0; k < C; ++k) {
+                seen.take(v[k], at + k * TPR + t);
+                if (k % 2 == 1 || k == C - 1) seen.mark(sp, (at - first) / TPR + k / 2 * 2, shift);
             }
-        }
-        add<ENT, N>(r, v, a.c);
-    }
-    for (; at < last; at += TPR) {
-        float v[1][8];
-        Raw<T> raw;
-        all_least(raw);
-        if (at + t < last) raw.load(row + (uint64_t)(at + t) * 8);
-        values_of(v[0], raw);
-        if (TOP) {
-            const float m = largest(v[0]);
-            if (m > best) best = m, place = at + t;
-        }
-        add<ENT, 1>(r, v, a.c);
-    }
+        add<ENT>(r, v, a.c);
+    });
     if (end > whole && t == (whole - first) % TPR) { // the row's last vector, of less than eight elements
         float v[1][8];
         load_last(v[0], row + (uint64_t)whole * 8, a.vocab % 8);
         if (TOP) {
+            const uint32_t turn = (whole - first) / TPR;
             const float m = largest(v[0]);
-            if (m > best) best = m, place = whole;
+            seen.take(v[0], whole);
+            // its mark may hold vectors before it
+            if (turn & ((1u << shift) - 1)) seen.run = fmaxf(m, as_float((uint32_t)sp.marks[(turn >> shift) * TPR + t] << 16));
+            else seen.run = m;
+            sp.marks[(turn >> shift) * TPR + t] = (uint16_t)mark_of(seen.run, sizeof(T) == 2);
         }
-        add<ENT, 1>(r, v, a.c);
+        add<ENT>(r, v, a.c);
     }
     group_join<ENT, WAVES>(r, a.c, slots);
     Key k = 0;
-    if (TOP) k = largest_of<T, TPR>(row, best, place, first, end, a.vocab, a.top_n, *reinterpret_cast<TopSpace<TPR> *>(space));
+    if (TOP) k = largest_of<T, TPR>(row, seen, shift, first, end, a.vocab, a.top_n, sp);
     if (t >= kWave) return;
     if (SPLIT) {
         if (t == 0) a.parts[blockIdx.x] = r;
