@@ -17,7 +17,7 @@ struct DistillArgs {
     Sums *parts;
     uint64_t stride, ids_stride, teacher_stride;
     uint32_t first, rows;
-    uint32_t vocab, slices, per;
+    uint32_t vocab, slices;
     uint32_t k, ids_64, teacher_f32;
     float c, inv_t;
 };
@@ -84,63 +84,58 @@ template <typename T, bool REST> __device__ __forceinline__ void finish(const Di
     st[5] = (float)over;
 }
 
-template <typename T, int TPR, bool REST, bool SPLIT> __global__ __launch_bounds__(TPR) void distill_kernel(const DistillArgs a) {
+/* Rows of more than kLong vectors are cut where there are no more than kFew of them, into slices of 4 vectors a thread. */
+constexpr uint32_t kLong = 8192, kFew = 64, kSlicesMost = 64, kSlice = kBatch * 256;
+
+template <typename T, int TPR, bool REST, bool SPLIT, bool ONCE> __global__ __launch_bounds__(TPR) void distill_kernel(const DistillArgs a) {
     constexpr int WAVES = TPR / (int)kWave;
     constexpr uint32_t kTurns = TPR > 256 ? 32 : 64, kSegment = kTurns * TPR; // vectors whose bits a thread holds at a time
     __shared__ Sums slots[WAVES];
     __shared__ uint32_t named[REST ? kSegment / 4 : 1], hits[REST ? 2 * TPR : 1];
     const uint32_t t = threadIdx.x, slice = SPLIT ? blockIdx.x % a.slices : 0;
     const uint64_t index = a.first + (SPLIT ? blockIdx.x / a.slices : blockIdx.x);
-    const T *row = (const T *)a.logits + index * a.stride;
-    const uint32_t whole = a.vocab / 8, all = (a.vocab + 7) / 8;
-    const uint32_t first = SPLIT ? slice * a.per : 0, end = SPLIT && all - first > a.per ? first + a.per : all;
+    const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
+    const uint32_t all = row.vectors(), first = SPLIT ? (slice * kSlice < all ? slice * kSlice : all) : 0, end = SPLIT && all - first > kSlice ? first + kSlice : all;
     int32_t id = -1;
     float x = -kInf, teacher = -kInf;
     if (t < kWave && (REST || !SPLIT)) {
         id = entry_of(a, index, t);
         if (!SPLIT && id >= 0) {
-            x = at(row + id);
+            x = at(row.from + row.skip + id);
             teacher = bf16_or_f32{a.teacher, a.teacher_f32 != 0}[index * a.teacher_stride + t];
         }
     }
     Sums r = {kLowest, 0.0f, 0.0f};
     for (uint32_t begin = first; begin < end; begin += REST ? kSegment : end - first) {
-        const uint32_t stop = REST && end - begin > kSegment ? begin + kSegment : end, last = stop < whole ? stop : whole;
+        const uint32_t stop = REST && end - begin > kSegment ? begin + kSegment : end;
         uint64_t mine = 0;
         if (REST) {
-            const uint32_t vec = (uint32_t)id / 8 - begin; // of the segment
-            const bool here = id >= 0 && (uint32_t)id / 8 >= begin && (uint32_t)id / 8 < stop;
+            const uint32_t place = row.skip + (uint32_t)id, vec = place / kEach<T> - begin; // of the segment
+            const bool here = id >= 0 && place / kEach<T> >= begin && place / kEach<T> < stop;
             hits[t] = hits[TPR + t] = 0;
             if (here) ((uint8_t *)named)[vec] = 0;
             __syncthreads();
             if (here) {
-                atomicOr(&named[vec / 4], 1u << (vec % 4 * 8 + (uint32_t)id % 8));
+                atomicOr(&named[vec / 4], 1u << (vec % 4 * 8 + place % kEach<T>));
                 atomicOr(&hits[vec / TPR / 32 * TPR + vec % TPR], 1u << (vec / TPR % 32));
             }
             __syncthreads();
             mine = (uint64_t)hits[TPR + t] << 32 | hits[t];
         }
-        auto leave_out = [&](float(&v)[8], uint32_t vec) { // vec of the segment
-            const uint32_t which = ((const uint8_t *)named)[vec];
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-                if (which >> e & 1) v[e] = -kInf;
-        };
-        walk<TPR>(row, begin, last, t, [&](auto &v, uint32_t at, bool) {
+        walk<TPR, ONCE>(row, begin, stop, t, [&](auto &v, uint32_t at, bool) {
             if (REST) {
                 const uint32_t bits = (uint32_t)(mine >> ((at - begin) / TPR));
 #pragma unroll
                 for (uint32_t k = 0; k < sizeof v / sizeof v[0]; ++k)
-                    if (bits >> k & 1) leave_out(v[k], at - begin + k * TPR + t); // the last, shorter vector has its turn below
+                    if (bits >> k & 1) {
+                        const uint32_t which = ((const uint8_t *)named)[at - begin + k * TPR + t];
+#pragma unroll
+                        for (uint32_t e = 0; e < kEach<T>; ++e)
+                            if (which >> e & 1) v[k][e] = -kInf;
+                    }
             }
             add<false>(r, v, a.c);
         });
-        if (stop > whole && t == (whole - begin) % TPR) { // the row's last vector, of less than eight elements
-            float v[1][8];
-            load_last(v[0], row + (uint64_t)whole * 8, a.vocab % 8);
-            if (REST && (mine >> ((whole - begin) / TPR) & 1)) leave_out(v[0], whole - begin);
-            add<false>(r, v, a.c);
-        }
         if (REST) __syncthreads(); // the bytes have been read
     }
     group_join<false, WAVES>(r, a.c, slots);
@@ -166,31 +161,35 @@ template <typename T, bool REST> __global__ __launch_bounds__(64) void distill_j
     finish<T, REST>(a, index, r, id, x, teacher, lane);
 }
 
-/* Slices of a row.  Rows that fill the chip by themselves are not cut. */
-constexpr uint32_t kFill = 1024, kSlicesMost = 64;
-uint32_t slices_most(uint64_t vocab) {
-    const uint64_t n = (vocab + 7) / 8 / 512;
-    return n < 1 ? 1 : n > kSlicesMost ? kSlicesMost : (uint32_t)n;
-}
-uint32_t slices_of(uint64_t rows, uint64_t vocab) {
-    const uint64_t n = kFill / rows, most = slices_most(vocab);
-    return n < 2 ? 1 : (uint32_t)(n < most ? n : most);
-}
+uint32_t slices_of(uint64_t vectors) { return (uint32_t)((vectors + kSlice - 1) / kSlice); }
 
-template <typename T, bool REST> void launch(const DistillArgs &a, hipStream_t s) {
-    const uint32_t rows = a.rows - a.first;
-    if (a.slices > 1) {
-        hipLaunchKernelGGL((distill_kernel<T, 256, REST, true>), dim3(rows * a.slices), dim3(256), 0, s, a);
+/* Threads to a row.  us for a call with 20 tokens, without and with the rest as a class:
+ *                        256 threads              1024                     slices, joined
+ *     1 row  of  4000 vectors    6.3  8.6            5.9  7.6                 7.9  8.0
+ *    64          6250            7.4 10.5            6.7  9.5                 7.7  9.2
+ *    64         16000           14.7 19.2           10.3 13.7                 8.1 10.6
+ *   128         16000           15.5 20.0           11.2 14.3                11.0 13.5
+ *   256         32000           21.5 25.9           21.8 24.4                24.1 26.6
+ *   400         16000           19.4 23.6           21.7 25.6                23.0 25.5 */
+template <typename T, bool REST> void launch(DistillArgs &a, uint64_t all_rows, hipStream_t s) {
+    const uint32_t rows = a.rows - a.first, n = vectors_most<T>(a.vocab);
+#define ERI_DISTILL(TPR, ONCE) hipLaunchKernelGGL((distill_kernel<T, TPR, REST, false, ONCE>), dim3(rows), dim3(TPR), 0, s, a)
+    a.slices = slices_of(n);
+    if (n > kLong && all_rows <= kFew && a.slices <= kSlicesMost) {
+        hipLaunchKernelGGL((distill_kernel<T, 256, REST, true, false>), dim3(rows * a.slices), dim3(256), 0, s, a);
         hipLaunchKernelGGL((distill_join_kernel<T, REST>), dim3(rows), dim3(64), 0, s, a);
-    } else if (a.vocab <= 2048) hipLaunchKernelGGL((distill_kernel<T, 64, REST, false>), dim3(rows), dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((distill_kernel<T, 256, REST, false>), dim3(rows), dim3(256), 0, s, a);
+    } else if (n <= 256) ERI_DISTILL(64, false);
+    else if (n > 2048 && all_rows <= 256) ERI_DISTILL(1024, false);
+    else if (all_rows * a.vocab * sizeof(T) > kCache) ERI_DISTILL(256, true);
+    else ERI_DISTILL(256, false);
+#undef ERI_DISTILL
 }
 
 } // namespace
 
 uint64_t distill_top_workspace(uint64_t rows, uint64_t vocab) {
-    const uint64_t most = slices_most(vocab), parts = rows * most < kFill ? rows * most : kFill;
-    return most > 1 ? parts * sizeof(Sums) : 0;
+    const uint64_t n = vectors_most<float>(vocab), most = kSlicesMost * kSlice;
+    return n > kLong ? (rows < kFew ? rows : kFew) * slices_of(n < most ? n : most) * sizeof(Sums) : 0;
 }
 
 int launch_distill_top(const EriDistillTop &e, void *stream) {
@@ -199,16 +198,13 @@ int launch_distill_top(const EriDistillTop &e, void *stream) {
     a.stride = e.logits_stride, a.ids_stride = e.ids_stride, a.teacher_stride = e.teacher_stride;
     a.vocab = (uint32_t)e.vocab, a.k = (uint32_t)e.k, a.ids_64 = (uint32_t)e.ids_64, a.teacher_f32 = e.teacher_dtype == ERI_DTYPE_F32;
     a.c = (float)(kLog2e / e.temperature), a.inv_t = (float)(1.0 / e.temperature);
-    const uint32_t n = (a.vocab + 7) / 8, want = slices_of(e.rows, e.vocab);
-    a.per = ((n + want - 1) / want + 255) / 256 * 256;
-    a.slices = (n + a.per - 1) / a.per;
     hipStream_t s = static_cast<hipStream_t>(stream);
     constexpr uint32_t kMost = 1u << 21; // rows of a launch
     for (uint64_t first = 0; first < e.rows; first += kMost) {
         a.first = (uint32_t)first;
         a.rows = (uint32_t)(e.rows - first < kMost ? e.rows : first + kMost);
-        if (e.dtype_tag == ERI_DTYPE_F32) e.rest ? launch<float, true>(a, s) : launch<float, false>(a, s);
-        else e.rest ? launch<bf16, true>(a, s) : launch<bf16, false>(a, s);
+        if (e.dtype_tag == ERI_DTYPE_F32) e.rest ? launch<float, true>(a, e.rows, s) : launch<float, false>(a, e.rows, s);
+        else e.rest ? launch<bf16, true>(a, e.rows, s) : launch<bf16, false>(a, e.rows, s);
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return (int)err;
     }

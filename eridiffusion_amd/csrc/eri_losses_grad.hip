@@ -23,29 +23,47 @@ struct GradArgs {
     float c, inv_t;
 };
 
-template <typename T, typename O, int TPR, typename Of> __device__ __forceinline__ void each(const T *row, O *out, uint32_t first, uint32_t end, uint32_t vocab, uint32_t t, Of of) {
-    const uint32_t whole = vocab / 8, last = end < whole ? end : whole;
-    walk<TPR>(row, first, last, t, [&](auto &v, uint32_t at, bool full) {
-        constexpr uint32_t C = sizeof v / sizeof v[0];
+#define ERI_PUT(TYPE, P, ...) \
+    do { \
+        if (ONCE) __builtin_nontemporal_store(__VA_ARGS__, (TYPE *)(P)); \
+        else *(TYPE *)(P) = __VA_ARGS__; \
+    } while (0)
+template <bool ONCE> __device__ __forceinline__ void store_whole(float *p, const float (&v)[4]) { ERI_PUT(u32x4_at4, p, u32x4{as_bits(v[0]), as_bits(v[1]), as_bits(v[2]), as_bits(v[3])}); }
+template <bool ONCE> __device__ __forceinline__ void store_whole(float *p, const float (&v)[8]) {
+    ERI_PUT(u32x4_at4, p, u32x4{as_bits(v[0]), as_bits(v[1]), as_bits(v[2]), as_bits(v[3])});
+    ERI_PUT(u32x4_at4, p + 4, u32x4{as_bits(v[4]), as_bits(v[5]), as_bits(v[6]), as_bits(v[7])});
+}
+template <bool ONCE> __device__ __forceinline__ void store_whole(bf16 *p, const float (&v)[4]) { ERI_PUT(u32x2_at2, p, u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])}); }
+template <bool ONCE> __device__ __forceinline__ void store_whole(bf16 *p, const float (&v)[8]) {
+    ERI_PUT(u32x4_at2, p, u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])});
+}
+#undef ERI_PUT
+__device__ __forceinline__ void store_one(float *p, float v) { *p = v; }
+__device__ __forceinline__ void store_one(bf16 *p, float v) { p->bits = (uint16_t)bf16_pair(v, 0.0f); }
+
+/* A vector of the gradient, where the row's vector lies; `out` is its beginning, taken down as the row's. */
+template <bool ONCE, typename T, typename O, int E> __device__ __forceinline__ void store_any(O *out, const Row<T> &row, uint32_t vec, uint32_t end, const float (&v)[E]) {
+    if (vec >= end) return;
+    if (vec >= row.whole_from() && vec < row.whole_to()) store_whole<ONCE>(out + (uint64_t)vec * E, v);
+    else
 #pragma unroll
-        for (uint32_t k = 0; k < C; ++k) {
+        for (uint32_t e = 0; e < (uint32_t)E; ++e)
+            if (row.has(vec, e)) store_one(out + (uint64_t)vec * E + e, v[e]);
+}
+template <int TPR, bool ONCE, typename T, typename O, typename Of> __device__ __forceinline__ void each(const Row<T> &row, O *out, uint32_t first, uint32_t end, uint32_t t, Of of) {
+    walk<TPR, ONCE>(row, first, end, t, [&](auto &v, uint32_t at, bool full) {
+#pragma unroll
+        for (uint32_t k = 0; k < sizeof v / sizeof v[0]; ++k) {
             const uint32_t vec = at + k * TPR + t;
-            of(v[k], vec * 8);
-            if (full || k < C - 1 || vec < last) store_n(out + (uint64_t)vec * 8, 8, v[k]);
+            of(v[k], vec * kEach<T>);
+            if (full) store_whole<ONCE>(out + (uint64_t)vec * kEach<T>, v[k]);
+            else store_any<ONCE>(out, row, vec, end, v[k]);
         }
     });
-    if (end > whole && t == (whole - first) % TPR) {
-        float v[8];
-        load_last(v, row + (uint64_t)whole * 8, vocab % 8);
-        of(v, whole * 8);
-        store_n(out + (uint64_t)whole * 8, vocab % 8, v);
-    }
 }
-template <typename O, int TPR> __device__ __forceinline__ void zeros(O *out, uint32_t first, uint32_t end, uint32_t vocab, uint32_t t) {
-    const float v[8] = {};
-    const uint32_t whole = vocab / 8, last = end < whole ? end : whole;
-    for (uint32_t at = first + t; at < last; at += TPR) store_n(out + (uint64_t)at * 8, 8, v);
-    if (end > whole && t == (whole - first) % TPR) store_n(out + (uint64_t)whole * 8, vocab % 8, v);
+template <int TPR, bool ONCE, typename T, typename O> __device__ __forceinline__ void zeros(const Row<T> &row, O *out, uint32_t first, uint32_t end, uint32_t t) {
+    const float v[kEach<T>] = {};
+    for (uint32_t vec = first + t; vec < end; vec += TPR) store_any<ONCE>(out, row, vec, end, v);
 }
 
 /* log2 p of an element, from {m, ln s}: nothing is left of a row where ln s is minus infinity. */
@@ -58,13 +76,14 @@ struct LogP {
     __device__ __forceinline__ float operator()(float x) const { return fmaf(x - m, c, -log2_s); }
 };
 
-template <typename T, typename O, int TPR, bool ENT> __global__ __launch_bounds__(256) void token_grad_kernel(const GradArgs a) {
+template <typename T, typename O, int TPR, bool ENT, bool ONCE> __global__ __launch_bounds__(256) void token_grad_kernel(const GradArgs a) {
     constexpr uint32_t ROWS = 256 / TPR;
     const uint32_t t = threadIdx.x % TPR, slice = blockIdx.x % a.slices;
-    const uint64_t index = a.first + (uint64_t)(blockIdx.x / a.slices) * ROWS + threadIdx.x / TPR;
+    const uint64_t index = a.first + (uint64_t)(blockIdx.x / a.slices) * ROWS + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / TPR));
     if (index >= a.rows) return;
-    const uint32_t all = (a.vocab + 7) / 8, first = slice * a.per, end = all - first > a.per ? first + a.per : all;
-    O *out = (O *)a.out + index * a.out_stride;
+    const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
+    const uint32_t all = row.vectors(), first = slice * a.per < all ? slice * a.per : all, end = all - first > a.per ? first + a.per : all;
+    O *out = (O *)a.out + index * a.out_stride - row.skip;
     int64_t id = -1;
     float g = 0.0f, h = 0.0f;
     if (a.grad) {
@@ -73,32 +92,32 @@ template <typename T, typename O, int TPR, bool ENT> __global__ __launch_bounds_
         else id = -1;
     }
     if (ENT) h = a.grad_entropy[index];
-    if (g == 0.0f && h == 0.0f) return zeros<O, TPR>(out, first, end, a.vocab, t);
+    if (g == 0.0f && h == 0.0f) return zeros<TPR, ONCE>(row, out, first, end, t);
     const LogP log2p(a.stats + index * 2, a.c);
-    const uint32_t named = g == 0.0f || log2p.log2_s == kInf ? ~0u : (uint32_t)id;
+    const uint32_t named = g == 0.0f || log2p.log2_s == kInf ? ~0u : row.skip + (uint32_t)id;
     const float u = -(ENT ? fmaf(h, log2p.log2_s == kInf ? 0.0f : a.entropy[index], g) : g) * a.inv_t, w = -h * kLn2 * a.inv_t, more = g * a.inv_t;
-    each<T, O, TPR>((const T *)a.logits + index * a.stride, out, first, end, a.vocab, t, [&](float(&v)[8], uint32_t col) {
+    each<TPR, ONCE>(row, out, first, end, t, [&](float(&v)[kEach<T>], uint32_t place) {
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
+        for (uint32_t e = 0; e < kEach<T>; ++e) {
             const float l = log2p(v[e]), p = exp2_of(l);
             v[e] = p * (ENT ? fmaf(w, fmaxf(l, kFloor), u) : u);
         }
-        const uint32_t there = named - col;
-        if (there < 8)
+        const uint32_t there = named - place;
+        if (there < kEach<T>)
 #pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
+            for (uint32_t e = 0; e < kEach<T>; ++e)
                 if (e == there) v[e] += more;
     });
 }
 
-template <typename T, typename O, int TPR> __global__ __launch_bounds__(TPR) void distill_grad_kernel(const GradArgs a) {
+template <typename T, typename O, int TPR, bool ONCE> __global__ __launch_bounds__(TPR) void distill_grad_kernel(const GradArgs a) {
     const uint32_t t = threadIdx.x, slice = blockIdx.x % a.slices;
     const uint64_t index = a.first + blockIdx.x / a.slices;
-    const uint32_t all = (a.vocab + 7) / 8, first = slice * a.per, end = all - first > a.per ? first + a.per : all;
-    const T *row = (const T *)a.logits + index * a.stride;
-    O *out = (O *)a.out + index * a.out_stride;
+    const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
+    const uint32_t all = row.vectors(), first = slice * a.per < all ? slice * a.per : all, end = all - first > a.per ? first + a.per : all;
+    O *out = (O *)a.out + index * a.out_stride - row.skip;
     const float g = a.grad[index] * a.inv_t, *st = a.stats + index * 6;
-    if (a.grad[index] == 0.0f || st[1] == -kInf) return zeros<O, TPR>(out, first, end, a.vocab, t);
+    if (a.grad[index] == 0.0f || st[1] == -kInf) return zeros<TPR, ONCE>(row, out, first, end, t);
     int32_t id = -1;
     float value = 0.0f;
     if (t < kWave) {
@@ -111,28 +130,36 @@ template <typename T, typename O, int TPR> __global__ __launch_bounds__(TPR) voi
         float sum = 0.0f; // over the entries of the same token
         for (uint32_t j = 0; j < a.k; ++j)
             if (__builtin_amdgcn_readlane(id, (int)j) == id) sum += lane_of(q, (int)j);
-        const bool here = id >= 0 && (uint32_t)id / 8 >= first && (uint32_t)id / 8 < end;
-        if (here) {
+        const uint32_t vec = (row.skip + (uint32_t)id) / kEach<T>;
+        if (id >= 0 && vec >= first && vec < end) {
             const LogP log2p(st, a.c);
-            const float p = st[4] == -kInf ? 0.0f : exp2_of(log2p(at(row + id)));
+            const float p = st[4] == -kInf ? 0.0f : exp2_of(log2p(at(row.from + row.skip + id)));
             value = (p - sum) * g;
         } else id = -1;
     }
     __syncthreads(); // the named logits have been read, before out may be written over them
     const LogP log2r(st + 2, a.c);
     const float over = st[5] * g;
-    each<T, O, TPR>(row, out, first, end, a.vocab, t, [&](float(&v)[8], uint32_t) {
+    each<TPR, ONCE>(row, out, first, end, t, [&](float(&v)[kEach<T>], uint32_t) {
 #pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) v[e] = exp2_of(log2r(v[e])) * over;
+        for (uint32_t e = 0; e < kEach<T>; ++e) v[e] = exp2_of(log2r(v[e])) * over;
     });
     __syncthreads();
-    if (id >= 0) {
-        const float v[8] = {value};
-        store_n(out + id, 1, v);
-    }
+    if (id >= 0) store_one(out + row.skip + id, value);
 }
 
 constexpr uint32_t kBlocks = 1u << 23; // of a launch
+
+/* Cuts rows into slices of one batch for each thread, or of `per` vectors; whether what is read and written passes the caches by.
+ * With one batch to a workgroup the chip works within one window of the memory: 8192 x 128000 bf16 729 us for the scores and 689 for the
+ * distillation, where a workgroup had a row 759 and 750, and 791 and 774 with what is stored passing the caches and what is read not.  A
+ * float32 gradient of bf16 logits, whose 16-byte stores leave gaps for one another, takes 522 in the caches and 599 past them. */
+template <typename T, typename O> bool cut(GradArgs &a, uint64_t rows, uint32_t per) {
+    const uint32_t n = vectors_most<T>(a.vocab);
+    a.per = n < per ? n : per;
+    a.slices = (n + a.per - 1) / a.per;
+    return sizeof(O) <= sizeof(T) && rows * a.vocab * sizeof(T) > kCache;
+}
 
 /* Launches over parts of the rows, so that a launch can count its threads. */
 template <typename F> int in_parts(GradArgs &a, uint64_t rows, uint32_t rows_of_block, F launch) {
@@ -148,24 +175,20 @@ template <typename F> int in_parts(GradArgs &a, uint64_t rows, uint32_t rows_of_
 }
 
 template <typename T, typename O> int token_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
-#define ERI_GRAD(TPR, ENT) in_parts(a, rows, 256 / TPR, [&](uint32_t n) { hipLaunchKernelGGL((token_grad_kernel<T, O, TPR, ENT>), dim3(n), dim3(256), 0, s, a); })
-    if (a.vocab <= 2048) return a.grad_entropy ? ERI_GRAD(64, true) : ERI_GRAD(64, false);
-    return a.grad_entropy ? ERI_GRAD(256, true) : ERI_GRAD(256, false);
+#define ERI_GRAD(TPR, ENT, ONCE) in_parts(a, rows, 256 / TPR, [&](uint32_t n) { hipLaunchKernelGGL((token_grad_kernel<T, O, TPR, ENT, ONCE>), dim3(n), dim3(256), 0, s, a); })
+    const bool once = cut<T, O>(a, rows, kBatch * 256);
+    if (a.per <= 256) return a.grad_entropy ? ERI_GRAD(64, true, false) : ERI_GRAD(64, false, false);
+    if (once) return a.grad_entropy ? ERI_GRAD(256, true, true) : ERI_GRAD(256, false, true);
+    return a.grad_entropy ? ERI_GRAD(256, true, false) : ERI_GRAD(256, false, false);
 #undef ERI_GRAD
 }
 template <typename T, typename O> int distill_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
-#define ERI_GRAD(TPR) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR>), dim3(n), dim3(TPR), 0, s, a); })
-    return a.vocab <= 2048 ? ERI_GRAD(64) : ERI_GRAD(256);
+#define ERI_GRAD(TPR, ONCE) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR, ONCE>), dim3(n), dim3(TPR), 0, s, a); })
+    // looking up the teacher's tokens costs each workgroup a few us: worth it in rows of some length, or where there are few of them
+    const bool once = cut<T, O>(a, rows, rows >= 1024 && vectors_most<T>(a.vocab) <= 4 * kBatch * 256 ? 4 * kBatch * 256 : kBatch * 256);
+    return a.per <= 256 ? ERI_GRAD(64, false) : once ? ERI_GRAD(256, true) : ERI_GRAD(256, false);
 #undef ERI_GRAD
 }
-void cut(GradArgs &a, uint64_t rows, uint32_t per) {
-    const uint32_t n = (a.vocab + 7) / 8;
-    a.per = rows >= 1024 ? n : per;
-    if (a.per > n) a.per = n;
-    a.slices = (n + a.per - 1) / a.per;
-    if (a.slices > kBlocks) a.per = n, a.slices = 1;
-}
-
 } // namespace
 
 int launch_token_logprobs_grad(const EriTokenLogprobsGrad &e, void *stream) {
@@ -173,7 +196,6 @@ int launch_token_logprobs_grad(const EriTokenLogprobsGrad &e, void *stream) {
     a.logits = e.logits, a.ids = e.ids, a.stats = e.stats, a.grad = e.grad, a.grad_entropy = e.grad_entropy, a.entropy = e.entropy, a.out = e.out;
     a.stride = e.logits_stride, a.out_stride = e.out_stride, a.vocab = (uint32_t)e.vocab, a.ids_64 = (uint32_t)e.ids_64;
     a.c = (float)(kLog2e / e.temperature), a.inv_t = (float)(1.0 / e.temperature);
-    cut(a, e.rows, 1024);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool f32 = e.dtype_tag == ERI_DTYPE_F32, out_f32 = e.out_dtype == ERI_DTYPE_F32;
     if (f32) return out_f32 ? token_grad<float, float>(a, e.rows, s) : token_grad<float, bf16>(a, e.rows, s);
@@ -186,7 +208,6 @@ int launch_distill_top_grad(const EriDistillTopGrad &e, void *stream) {
     a.stride = e.logits_stride, a.out_stride = e.out_stride, a.ids_stride = e.ids_stride, a.teacher_stride = e.teacher_stride;
     a.vocab = (uint32_t)e.vocab, a.k = (uint32_t)e.k, a.ids_64 = (uint32_t)e.ids_64, a.teacher_f32 = e.teacher_dtype == ERI_DTYPE_F32;
     a.c = (float)(kLog2e / e.temperature), a.inv_t = (float)(1.0 / e.temperature);
-    cut(a, e.rows, 4096);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const bool f32 = e.dtype_tag == ERI_DTYPE_F32, out_f32 = e.out_dtype == ERI_DTYPE_F32;
     if (f32) return out_f32 ? distill_grad<float, float>(a, e.rows, s) : distill_grad<float, bf16>(a, e.rows, s);

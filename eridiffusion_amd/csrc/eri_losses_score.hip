@@ -12,8 +12,6 @@
 namespace eri_losses {
 namespace {
 
-constexpr uint32_t kFound = 256; // elements that pass the bound and are kept at a time
-
 struct ScoreArgs {
     const void *logits, *ids;
     float *logprob, *entropy, *stats, *top;
@@ -22,7 +20,7 @@ struct ScoreArgs {
     Key *part_keys; // top of each
     uint64_t stride;
     uint32_t first, rows; // rows first .. rows-1
-    uint32_t vocab, slices, per; // per: vectors to a slice
+    uint32_t vocab, slices, shift; // 1 << shift vectors to a mark
     uint32_t top_n, ids_64;
     float c, inv_t;
 };
@@ -53,16 +51,17 @@ template <typename T> __device__ __forceinline__ bool token_of(const ScoreArgs &
     return true;
 }
 
+/* What the threads of a workgroup tell each other about their elements. */
 constexpr uint32_t kMarks = 8192; // largest values of a few vectors each, over all threads
 template <int TPR> struct TopSpace {
-    uint16_t marks[kMarks];
-    union {
-        Key lists[TPR];
-        Key found[kFound];
-    };
-    uint16_t places[kWave * (kMarks / TPR)]; // marks that reach the bound: only k threads have any
+    Key lists[TPR];
+    uint32_t found[TPR]; // columns, 64 to a wave
     Key bound;
-    uint32_t places_n, count;
+    uint32_t places_n;
+};
+template <int TPR> struct Marks {
+    uint16_t values[kMarks];
+    uint16_t places[kWave * (kMarks / TPR)]; // those that reach the bound: only 64 threads have any
 };
 
 /* The upper 16 bits of a value, rounded up. */
@@ -71,140 +70,230 @@ __device__ __forceinline__ uint32_t mark_of(float v, bool exact) {
     return exact || (int32_t)u < 0 ? u >> 16 : (u + 0xffffu) >> 16;
 }
 
-/* What a thread knows of its elements: the largest, its first vector that holds it, and the largest of every `each` of its vectors (a power
- * of two), which it leaves in marks[turn / each]. */
-template <typename T, int TPR> struct Seen {
-    float best, run;
+/* The largest element of a thread and its first vector that holds it. */
+struct Best {
+    float value;
     uint32_t place;
-    __device__ __forceinline__ void take(const float (&v)[8], uint32_t vec) {
-        const float m = largest(v);
-        if (m > best) best = m, place = vec;
-        run = fmaxf(run, m);
-    }
-    /* after each one or two vectors from `turn` on */
-    __device__ __forceinline__ void mark(TopSpace<TPR> &sp, uint32_t turn, uint32_t shift) {
-        sp.marks[(turn >> shift) * TPR + threadIdx.x] = (uint16_t)mark_of(run, sizeof(T) == 2);
-        if (((turn + 2) & ((1u << shift) - 1)) < 2) run = -kInf;
+    template <int E> __device__ __forceinline__ float take(const float (&v)[E], uint32_t vec) {
+        const float m = largest(v, -kInf);
+        if (m > value) value = m, place = vec;
+        return m;
     }
 };
 
-/* The row's (or slice's) largest elements in the lanes of the first wave, in descending order; vectors first .. end-1 are dealt to the threads in turn. */
-template <typename T, int TPR> __device__ __forceinline__ Key largest_of(const T *row, const Seen<T, TPR> &seen, uint32_t shift, uint32_t first, uint32_t end, uint32_t vocab, uint32_t top_n, TopSpace<TPR> &sp) {
-    constexpr uint32_t WAVES = TPR / kWave;
-    const uint32_t t = threadIdx.x, lane = t % kWave, wave = t / kWave, whole = vocab / 8;
-    const Key own = first + t < end ? key_of(seen.best, seen.place) : 0;
-    Key k = own;
-    sort64(k, lane);
-    if (WAVES > 1) sp.lists[t] = k;
-    for (uint32_t half = WAVES / 2; half > 0; half /= 2) {
+/* A thread's first vector that holds anything of the row, which may begin some vectors after the first. */
+template <int TPR, typename T> __device__ __forceinline__ uint32_t first_of(const Row<T> &row, uint32_t first, uint32_t t) {
+    return first + t + (first + t < row.skip / kEach<T> ? TPR : 0);
+}
+
+/* The 64 largest of the lists that the waves have, in the first one. */
+template <int TPR> __device__ __forceinline__ void join_lists(Key &k, TopSpace<TPR> &sp) {
+    const uint32_t t = threadIdx.x, lane = t % kWave, wave = t / kWave;
+    if (TPR > (int)kWave) sp.lists[t] = k;
+#pragma unroll
+    for (uint32_t half = TPR / kWave / 2; half > 0; half /= 2) {
         __syncthreads();
         if (wave < half) {
             merge64(k, sp.lists[(wave + half) * kWave + (kWave - 1 - lane)], lane);
-            sp.lists[t] = k;
+            if (half > 1) sp.lists[t] = k;
         }
     }
-    if (t == top_n - 1) sp.bound = k; // 0, which all pass, where fewer threads have seen anything
-    if (t == 0) sp.places_n = 0;
-    __syncthreads();
-    const Key bound = sp.bound;
-    const uint32_t turns = (end - first + TPR - 1) / TPR;
-    const float least = bound ? value_of(bound) : -kInf;
-    if (own >= bound && own != 0) // one of top_n threads; marks of vectors behind the end hold anything, and lead nowhere
-        for (uint32_t i = 0; i << shift < turns; ++i)
-            if (as_float((uint32_t)sp.marks[i * TPR + t] << 16) >= least) sp.places[atomicAdd(&sp.places_n, 1u)] = (uint16_t)(i * TPR + t);
-    __syncthreads();
-    const uint32_t total = sp.places_n << shift;
-    uint32_t per = total;
-    Key top = 0;
-    for (uint32_t from = 0; from < total;) {
-        if (t == 0) sp.count = 0;
-        __syncthreads();
-        const uint32_t to = per < total - from ? from + per : total;
-        for (uint32_t j = from + t; j < to; j += TPR) {
-            const uint32_t place = sp.places[j >> shift], vec = first + place % TPR + ((place / TPR << shift) + (j & ((1u << shift) - 1))) * TPR;
-            if (vec >= end) continue;
-            float v[8];
-            if (vec < whole) {
-                Raw<T> r;
-                r.load(row + (uint64_t)vec * 8);
-                values_of(v, r);
-            } else load_last(v, row + (uint64_t)vec * 8, vocab % 8);
-#pragma unroll
-            for (uint32_t e = 0; e < 8; ++e)
-                if (vec * 8 + e < vocab && key_of(v[e], vec) >= bound) {
-                    const uint32_t i = atomicAdd(&sp.count, 1u);
-                    if (i < kFound) sp.found[i] = key_of(v[e], vec * 8 + e);
-                }
-        }
-        __syncthreads();
-        const uint32_t c = sp.count;
-        __syncthreads();
-        if (c > kFound) { // far more on one side of a tie than there are threads: again from the start, so few vectors at a time that they fit
-            per = kFound / 8;
-            continue;
-        }
-        if (t < kWave)
-            for (uint32_t i = 0; i < c; i += kWave) {
-                Key f = i + lane < c ? sp.found[i + lane] : 0;
-                sort64(f, lane);
-                if (i == 0 && from == 0) top = f;
-                else merge64(top, key_from(f, kWave - 1 - lane), lane);
-            }
-        __syncthreads();
-        from = to;
-    }
-    return top;
 }
 
-template <typename T, int TPR, bool ENT, bool TOP, bool SPLIT> __global__ __launch_bounds__(TPR) void score_kernel(const ScoreArgs a) {
+/* The top_n-th largest of the threads' keys, 0 where fewer threads have one. */
+template <int TPR> __device__ __forceinline__ Key bound_of(Key k, uint32_t top_n, TopSpace<TPR> &sp) {
+    sort64(k, threadIdx.x % kWave);
+    join_lists<TPR>(k, sp);
+    if (threadIdx.x == top_n - 1) sp.bound = k;
+    if (threadIdx.x == 0) sp.places_n = 0;
+    __syncthreads();
+    return sp.bound;
+}
+
+/* For n things of each lane, n below 64, how many those before it have, and all lanes together. */
+__device__ __forceinline__ uint32_t before_of(uint32_t n, uint32_t *total) {
+    uint32_t before = 0, all = 0;
+#pragma unroll
+    for (uint32_t b = 0; b < 6; ++b) {
+        const uint64_t with = __ballot(n >> b & 1);
+        before += __builtin_amdgcn_mbcnt_hi((uint32_t)(with >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)with, 0)) << b;
+        all += (uint32_t)__popcll(with) << b;
+    }
+    *total = all;
+    return before;
+}
+__device__ __forceinline__ void wave_sees() { // what its lanes have left in LDS
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+/* A wave's largest elements: columns are put down as they pass the bound, and sorted where 64 have come together. */
+template <typename T> struct Largest {
+    const Row<T> &row;
+    const Key bound;
+    uint32_t *const found; // 64 columns of this wave's
+    const uint32_t lane;
+    uint32_t n = 0;
+    bool any = false;
+    Key top = 0;
+    __device__ __forceinline__ Largest(const Row<T> &r, Key b, uint32_t *all) : row(r), bound(b), found(all + threadIdx.x / kWave * kWave), lane(threadIdx.x % kWave) {}
+    __device__ __forceinline__ void sort() {
+        if (n == 0) return;
+        wave_sees();
+        Key k = 0;
+        if (lane < n) {
+            const uint32_t col = found[lane];
+            k = key_of(at(row.from + row.skip + col), col);
+        }
+        wave_sees();
+        sort64(k, lane);
+        if (any) merge64(top, key_from(k, kWave - 1 - lane), lane);
+        else top = k;
+        any = true;
+        n = 0;
+    }
+    /* The elements on or above the bound of N vectors, vec(i) with values v[i], of lanes that are active; all lanes of the wave call. */
+    template <int N, int E, typename Vec> __device__ __forceinline__ void take(const float (&v)[N][E], bool active, Vec vec) {
+        uint32_t which = 0;
+        if (active) {
+            const float least = bound ? value_of(bound) : -kInf;
+            const uint32_t u = as_bits(least), next = (int32_t)u >= 0 ? u + 1 : u == 0x80000000u ? 1 : u - 1; // the next larger value
+#pragma unroll
+            for (uint32_t i = 0; i < (uint32_t)N; ++i) {
+                const float from = bound == 0 || vec(i) <= place_of(bound) ? least : as_float(next); // later vectors lose a tie
+                uint32_t these = 0;
+#pragma unroll
+                for (uint32_t e = 0; e < (uint32_t)E; ++e) these |= v[i][e] >= from ? 1u << e : 0u;
+                if (!(vec(i) >= row.whole_from() && vec(i) < row.whole_to()))
+#pragma unroll
+                    for (uint32_t e = 0; e < (uint32_t)E; ++e)
+                        if (!row.has(vec(i), e)) these &= ~(1u << e);
+                which |= these << (i * E);
+            }
+        }
+        uint32_t total, mine = (uint32_t)__popc(which), to = before_of(mine, &total);
+        if (total == 0) return;
+        if (n + total <= kWave) {
+            for (to += n; which != 0; which &= which - 1) {
+                const uint32_t b = (uint32_t)__builtin_ctz(which);
+                found[to++] = row.col(vec(b / E), b % E);
+            }
+            n += total;
+            return;
+        }
+        for (uint32_t b = 0; b < (uint32_t)(N * E); ++b) {
+            const bool pass = which >> b & 1;
+            const uint64_t with = __ballot(pass);
+            const uint32_t more = (uint32_t)__popcll(with);
+            if (n + more > kWave) sort();
+            if (pass) found[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(with >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)with, 0))] = row.col(vec(b / E), b % E);
+            n += more;
+        }
+    }
+};
+
+template <typename T, int TPR, bool ENT, bool TOP, bool ONCE> __global__ __launch_bounds__(TPR) void score_kernel(const ScoreArgs a) {
     constexpr int WAVES = TPR / (int)kWave;
     __shared__ Sums slots[WAVES];
-    __shared__ char space[TOP ? sizeof(TopSpace<TPR>) : 1] __attribute__((aligned(16)));
-    const uint32_t t = threadIdx.x, slice = SPLIT ? blockIdx.x % a.slices : 0;
-    const uint64_t index = a.first + (SPLIT ? blockIdx.x / a.slices : blockIdx.x);
-    const T *row = (const T *)a.logits + index * a.stride;
+    __shared__ char top_space[TOP ? sizeof(TopSpace<TPR>) : 1] __attribute__((aligned(16))), mark_space[TOP ? sizeof(Marks<TPR>) : 1] __attribute__((aligned(16)));
+    TopSpace<TPR> &sp = *reinterpret_cast<TopSpace<TPR> *>(top_space);
+    Marks<TPR> &marks = *reinterpret_cast<Marks<TPR> *>(mark_space);
+    const uint32_t t = threadIdx.x, shift = a.shift;
+    const uint64_t index = a.first + blockIdx.x;
+    const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
     float x = 0.0f;
-    const bool named = !SPLIT && token_of<T>(a, index, &x);
-    const uint32_t whole = a.vocab / 8, all = (a.vocab + 7) / 8;
-    const uint32_t first = SPLIT ? slice * a.per : 0, end = SPLIT && all - first > a.per ? first + a.per : all, last = end < whole ? end : whole;
+    const bool named = token_of<T>(a, index, &x);
+    const uint32_t end = row.vectors();
 
     Sums r = {kLowest, 0.0f, 0.0f};
-    Seen<T, TPR> seen = {-kInf, -kInf, first + t};
-    TopSpace<TPR> &sp = *reinterpret_cast<TopSpace<TPR> *>(space);
-    uint32_t shift = 1; // so that the marks suffice
-    while (TOP && (a.per / TPR) >> shift >= kMarks / TPR) ++shift;
-    walk<TPR>(row, first, last, t, [&](auto &v, uint32_t at, bool) {
+    Best best = {-kInf, first_of<TPR>(row, 0, t)};
+    float run = -kInf;
+    walk<TPR, ONCE>(row, 0, end, t, [&](auto &v, uint32_t at, bool) {
         constexpr uint32_t C = sizeof v / sizeof v[0];
         if (TOP)
 #pragma unroll
             for (uint32_t k = 0; k < C; ++k) {
-                seen.take(v[k], at + k * TPR + t);
-                if (k % 2 == 1 || k == C - 1) seen.mark(sp, (at - first) / TPR + k / 2 * 2, shift);
+                run = fmaxf(run, best.take(v[k], at + k * TPR + t));
+                if (k % 2 == 1 || k == C - 1) {
+                    const uint32_t turn = at / TPR + k / 2 * 2;
+                    marks.values[(turn >> shift) * TPR + t] = (uint16_t)mark_of(run, sizeof(T) == 2);
+                    if (((turn + 2) & ((1u << shift) - 1)) == 0) run = -kInf;
+                }
             }
         add<ENT>(r, v, a.c);
     });
-    if (end > whole && t == (whole - first) % TPR) { // the row's last vector, of less than eight elements
-        float v[1][8];
-        load_last(v[0], row + (uint64_t)whole * 8, a.vocab % 8);
-        if (TOP) {
-            const uint32_t turn = (whole - first) / TPR;
-            const float m = largest(v[0]);
-            seen.take(v[0], whole);
-            // its mark may hold vectors before it
-            if (turn & ((1u << shift) - 1)) seen.run = fmaxf(m, as_float((uint32_t)sp.marks[(turn >> shift) * TPR + t] << 16));
-            else seen.run = m;
-            sp.marks[(turn >> shift) * TPR + t] = (uint16_t)mark_of(seen.run, sizeof(T) == 2);
-        }
-        add<ENT>(r, v, a.c);
-    }
     group_join<ENT, WAVES>(r, a.c, slots);
     Key k = 0;
-    if (TOP) k = largest_of<T, TPR>(row, seen, shift, first, end, a.vocab, a.top_n, sp);
-    if (t >= kWave) return;
-    if (SPLIT) {
-        if (t == 0) a.parts[blockIdx.x] = r;
-        if (TOP && t < a.top_n) a.part_keys[(uint64_t)blockIdx.x * a.top_n + t] = k;
-    } else finish<T, ENT, TOP>(a, index, r, k, x, named, t);
+    if (TOP) {
+        const Key own = best.place < end ? key_of(best.value, best.place) : 0, bound = bound_of<TPR>(own, a.top_n, sp);
+        const uint32_t turns = (end + TPR - 1) / TPR;
+        const float least = bound ? value_of(bound) : -kInf;
+        // one of top_n threads; marks of vectors behind the end hold anything, and lead nowhere
+        for (uint32_t from = 0; from << shift < turns; from += 32) {
+            uint32_t which = 0, total;
+            if (own >= bound && own != 0)
+                for (uint32_t i = 0; i < 32 && (from + i) << shift < turns; ++i)
+                    if (as_float((uint32_t)marks.values[(from + i) * TPR + t] << 16) >= least) which |= 1u << i;
+            uint32_t to = before_of((uint32_t)__popc(which), &total), base = 0;
+            if (total == 0) continue;
+            if (t % kWave == 0) base = atomicAdd(&sp.places_n, total);
+            to += (uint32_t)__builtin_amdgcn_readfirstlane((int)base);
+            for (; which != 0; which &= which - 1) marks.places[to++] = (uint16_t)((from + __builtin_ctz(which)) * TPR + t);
+        }
+        __syncthreads();
+        Largest<T> found(row, bound, sp.found);
+        const uint32_t total = sp.places_n << shift;
+        for (uint32_t from = 0; from < total; from += TPR) {
+            const uint32_t j = from + t, place = j < total ? marks.places[j >> shift] : 0, vec = place % TPR + ((place / TPR << shift) + (j & ((1u << shift) - 1))) * TPR;
+            float v[1][kEach<T>];
+            const bool real = j < total && vec < end;
+            if (real) values_of(v[0], load_any<false>(row, vec));
+            found.take(v, real, [&](uint32_t) { return vec; });
+        }
+        found.sort();
+        k = found.top;
+        join_lists<TPR>(k, sp);
+    }
+    if (t < kWave) finish<T, ENT, TOP>(a, index, r, k, x, named, t);
+}
+
+/* Rows of more than kLong vectors are cut where there are no more than kFew of them, into slices of 4 vectors a thread. */
+constexpr uint32_t kLong = 8192, kFew = 64, kSlicesMost = 64, kSliceThreads = 256;
+
+/* A slice of a row that a workgroup's registers hold: nothing is read twice. */
+template <typename T, int TPR, bool ENT, bool TOP> __global__ __launch_bounds__(TPR) void score_slice_kernel(const ScoreArgs a) {
+    constexpr int WAVES = TPR / (int)kWave;
+    __shared__ Sums slots[WAVES];
+    __shared__ char top_space[TOP ? sizeof(TopSpace<TPR>) : 1] __attribute__((aligned(16)));
+    TopSpace<TPR> &sp = *reinterpret_cast<TopSpace<TPR> *>(top_space);
+    const uint32_t t = threadIdx.x;
+    const uint64_t index = a.first + blockIdx.x / a.slices;
+    const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
+    const uint32_t all = row.vectors(), first = blockIdx.x % a.slices * (kBatch * TPR);
+    u32x4 raw[kBatch];
+#pragma unroll
+    for (uint32_t k = 0; k < kBatch; ++k) raw[k] = load_any<false>(row, first + k * TPR + t); // nothing where the row has no such vector
+    float v[kBatch][kEach<T>];
+#pragma unroll
+    for (uint32_t k = 0; k < kBatch; ++k) values_of(v[k], raw[k]);
+    Sums r = {kLowest, 0.0f, 0.0f};
+    add<ENT>(r, v, a.c);
+    group_join<ENT, WAVES>(r, a.c, slots);
+    Key k = 0;
+    if (TOP) {
+        Best best = {-kInf, first_of<TPR>(row, first, t)};
+#pragma unroll
+        for (uint32_t i = 0; i < kBatch; ++i) best.take(v[i], first + i * TPR + t);
+        const Key own = best.place < all ? key_of(best.value, best.place) : 0, bound = bound_of<TPR>(own, a.top_n, sp);
+        Largest<T> found(row, bound, sp.found);
+        found.take(v, own >= bound && own != 0, [&](uint32_t i) { return first + i * TPR + t; });
+        found.sort();
+        k = found.top;
+        join_lists<TPR>(k, sp);
+    }
+    if (t == 0) a.parts[blockIdx.x] = r;
+    if (TOP && t < a.top_n) a.part_keys[(uint64_t)blockIdx.x * a.top_n + t] = k;
 }
 
 /* Joins the slices of a row: 8 waves, each with an eighth of the lists. */
@@ -217,14 +306,25 @@ template <typename T, bool ENT, bool TOP> __global__ __launch_bounds__(512) void
     const bool named = token_of<T>(a, index, &x);
     Key k = 0;
     if (TOP) {
-        for (uint32_t s = wave; s < a.slices; s += 8) {
-            const uint32_t up = kWave - 1 - lane;
-            merge64(k, up < a.top_n ? a.part_keys[(uint64_t)(from + s) * a.top_n + up] : 0, lane);
+        Key list[kSlicesMost / 8];
+#pragma unroll
+        for (uint32_t i = 0; i < kSlicesMost / 8; ++i) {
+            const uint32_t s = i * 8 + wave, place = i ? kWave - 1 - lane : lane; // the others upside down, for the merge
+            list[i] = s < a.slices && place < a.top_n ? a.part_keys[(uint64_t)(from + s) * a.top_n + place] : 0;
         }
+        k = list[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kSlicesMost / 8; ++i)
+            if (i * 8 < a.slices) merge64(k, list[i], lane);
         lists[t] = k;
-        __syncthreads();
-        if (wave == 0)
-            for (uint32_t w = 1; w < 8; ++w) merge64(k, lists[w * kWave + (kWave - 1 - lane)], lane);
+#pragma unroll
+        for (uint32_t half = 4; half > 0; half /= 2) {
+            __syncthreads();
+            if (wave < half) {
+                merge64(k, lists[(wave + half) * kWave + (kWave - 1 - lane)], lane);
+                lists[t] = k;
+            }
+        }
     }
     if (wave != 0) return;
     Sums r = {kLowest, 0.0f, 0.0f};
@@ -233,53 +333,60 @@ template <typename T, bool ENT, bool TOP> __global__ __launch_bounds__(512) void
     finish<T, ENT, TOP>(a, index, r, k, x, named, lane);
 }
 
-/* Slices of a row.  Rows that fill the chip by themselves are not cut. */
-constexpr uint32_t kFill = 1024, kSlicesMost = 64;
-uint32_t slices_most(uint64_t vocab) {
-    const uint64_t n = (vocab + 7) / 8 / 512;
-    return n < 1 ? 1 : n > kSlicesMost ? kSlicesMost : (uint32_t)n;
-}
-uint32_t slices_of(uint64_t rows, uint64_t vocab) {
-    const uint64_t n = kFill / rows, most = slices_most(vocab);
-    return n < 2 ? 1 : (uint32_t)(n < most ? n : most);
+uint32_t slices_of(uint64_t vectors) { return (uint32_t)((vectors + kBatch * kSliceThreads - 1) / (kBatch * kSliceThreads)); }
+uint64_t parts_most(uint64_t rows, uint64_t vocab) {
+    const uint64_t n = vectors_most<float>(vocab), slices = slices_of(n < kSlicesMost * kBatch * kSliceThreads ? n : kSlicesMost * kBatch * kSliceThreads);
+    return n > kLong ? (rows < kFew ? rows : kFew) * slices : 0;
 }
 
-template <typename T, bool ENT, bool TOP> void launch(const ScoreArgs &a, hipStream_t s) {
-    const uint32_t rows = a.rows - a.first;
-    if (a.slices > 1) {
-        hipLaunchKernelGGL((score_kernel<T, 256, ENT, TOP, true>), dim3(rows * a.slices), dim3(256), 0, s, a);
+/* Threads to a row.  us for a call, bf16 and f32, with and without 20 alternatives:
+ *                        256 threads              1024                     slices, joined
+ *     1 row  of  4000 vectors    6.0  8.7            6.2  9.8                 7.7  9.3
+ *     1          8000            6.1  9.7            5.9  9.4                 7.7  8.9
+ *     1         16000           10.3 16.7            8.7 15.0                 7.9  9.3
+ *    64         16000           12.8 19.2            9.8 16.2                 7.7 13.3
+ *   128         16000           14.4 21.0           10.5 16.8                 9.9 18.7
+ *   256         32000           26.7 34.4           21.6 27.6                24.4 41.6
+ *   400         16000           18.4 25.3           20.2 33.1                19.8 39.5 */
+template <typename T, bool ENT, bool TOP> void launch(ScoreArgs &a, uint64_t all_rows, hipStream_t s) {
+    const uint32_t rows = a.rows - a.first, n = vectors_most<T>(a.vocab);
+#define ERI_SCORE(TPR, ONCE) \
+    do { \
+        for (a.shift = 1; n / TPR >> a.shift >= kMarks / TPR;) ++a.shift; \
+        hipLaunchKernelGGL((score_kernel<T, TPR, ENT, TOP, ONCE>), dim3(rows), dim3(TPR), 0, s, a); \
+    } while (0)
+    a.slices = slices_of(n);
+    if (n > kLong && all_rows <= kFew && a.slices <= kSlicesMost) {
+        hipLaunchKernelGGL((score_slice_kernel<T, kSliceThreads, ENT, TOP>), dim3(rows * a.slices), dim3(kSliceThreads), 0, s, a);
         hipLaunchKernelGGL((score_join_kernel<T, ENT, TOP>), dim3(rows), dim3(TOP ? 512 : 64), 0, s, a);
-    } else if (a.vocab <= 2048) hipLaunchKernelGGL((score_kernel<T, 64, ENT, TOP, false>), dim3(rows), dim3(64), 0, s, a);
-    else hipLaunchKernelGGL((score_kernel<T, 256, ENT, TOP, false>), dim3(rows), dim3(256), 0, s, a);
+    } else if (n <= 256) ERI_SCORE(64, false);
+    else if (n > kLong && all_rows <= 256) ERI_SCORE(1024, false);
+    else if (all_rows * a.vocab * sizeof(T) > kCache) ERI_SCORE(256, true);
+    else ERI_SCORE(256, false);
+#undef ERI_SCORE
 }
-template <typename T> void launch_of(const ScoreArgs &a, hipStream_t s) {
-    if (a.entropy) a.top_n ? launch<T, true, true>(a, s) : launch<T, true, false>(a, s);
-    else a.top_n ? launch<T, false, true>(a, s) : launch<T, false, false>(a, s);
+template <typename T> void launch_of(ScoreArgs &a, uint64_t rows, hipStream_t s) {
+    if (a.entropy) a.top_n ? launch<T, true, true>(a, rows, s) : launch<T, true, false>(a, rows, s);
+    else a.top_n ? launch<T, false, true>(a, rows, s) : launch<T, false, false>(a, rows, s);
 }
 
 } // namespace
 
-uint64_t token_logprobs_workspace(uint64_t rows, uint64_t vocab, uint32_t top) {
-    const uint64_t most = slices_most(vocab), parts = rows * most < kFill ? rows * most : kFill;
-    return most > 1 ? parts * (16 + (uint64_t)top * sizeof(Key)) : 0;
-}
+uint64_t token_logprobs_workspace(uint64_t rows, uint64_t vocab, uint32_t top) { return parts_most(rows, vocab) * (16 + (uint64_t)top * sizeof(Key)); }
 
 int launch_token_logprobs(const EriTokenLogprobs &e, void *stream) {
     ScoreArgs a = {};
     a.logits = e.logits, a.ids = e.ids, a.logprob = e.ids ? e.logprob : nullptr, a.entropy = e.entropy, a.stats = e.stats, a.top = e.top, a.top_ids = e.top_ids;
     a.stride = e.logits_stride, a.vocab = (uint32_t)e.vocab, a.top_n = (uint32_t)e.top_n, a.ids_64 = (uint32_t)e.ids_64;
     a.c = (float)(kLog2e / e.temperature), a.inv_t = (float)(1.0 / e.temperature);
-    const uint32_t n = (a.vocab + 7) / 8, want = slices_of(e.rows, e.vocab);
-    a.per = ((n + want - 1) / want + 255) / 256 * 256;
-    a.slices = (n + a.per - 1) / a.per;
-    a.part_keys = (Key *)e.workspace; // keys first: they need more alignment
-    a.parts = (Sums *)(a.part_keys + (a.slices > 1 ? e.rows * a.slices * e.top_n : 0));
+    a.parts = (Sums *)e.workspace; // 16 bytes to each, then the keys
+    a.part_keys = (Key *)((char *)e.workspace + parts_most(e.rows, e.vocab) * 16);
     constexpr uint32_t kMost = 1u << 21; // rows of a launch
     for (uint64_t first = 0; first < e.rows; first += kMost) {
         a.first = (uint32_t)first;
         a.rows = (uint32_t)(e.rows - first < kMost ? e.rows : first + kMost);
-        if (e.dtype_tag == ERI_DTYPE_F32) launch_of<float>(a, static_cast<hipStream_t>(stream));
-        else launch_of<bf16>(a, static_cast<hipStream_t>(stream));
+        if (e.dtype_tag == ERI_DTYPE_F32) launch_of<float>(a, e.rows, static_cast<hipStream_t>(stream));
+        else launch_of<bf16>(a, e.rows, static_cast<hipStream_t>(stream));
         const hipError_t err = hipGetLastError();
         if (err != hipSuccess) return (int)err;
     }

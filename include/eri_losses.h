@@ -14,7 +14,7 @@
  * Minus infinity is a token that cannot occur.  A row whose logits are all minus infinity leaves nothing: its log probabilities are minus infinity, its
  * entropy 0, its gradient 0.  A row that holds NaN or plus infinity has no softmax: what is computed from it is NaN.
  * A token id outside [0, vocab) names no token.  Sums are F32 or wider, in an order that the sizes
- * decide: the same call on the same inputs gives the same bits.
+ * and the rows' distance from multiples of 128 bytes decide: the same call on the same inputs at the same addresses gives the same bits.
  */
 #ifndef ERI_LOSSES_H
 #define ERI_LOSSES_H
