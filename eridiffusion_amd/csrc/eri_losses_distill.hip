@@ -35,18 +35,10 @@ __device__ __forceinline__ int32_t entry_of(const DistillArgs &a, uint64_t row, 
     return id >= 0 && id < (int64_t)a.vocab ? (int32_t)id : -1;
 }
 
-/* One wave: `o` are the sums over the row, or with REST over what the teacher does not name. */
+/* One wave: `o` are the sums over the row, or with REST over what the teacher does not name.  fp64 where two numbers that may all but cancel are
+ * made: an exponential and a logarithm more or less for each row count where rows are short (16384 x 1000 with the rest 33.5 us with seven of them). */
 template <typename T, bool REST> __device__ __forceinline__ void finish(const DistillArgs &a, uint64_t row, Sums o, int32_t id, float x, float teacher, uint32_t lane) {
     const bool used = id >= 0;
-    // the teacher: the log of the sum of its probabilities
-    const bool some = used && !(teacher == -kInf); // NaN too
-    const bool has = __ballot(some) != 0;
-    float most = some ? teacher : -kInf;
-#pragma unroll
-    for (int d = 1; d < (int)kWave; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    if (most == -kInf) most = 0.0f; // nothing, or nothing but NaN
-    const double weight = wave_sum(some ? exp((double)teacher - most) : 0.0);
-    double norm = has ? (double)most + log(weight) : -(double)kInf;
     // the student: sums over the whole row, and what the named tokens hold of it, each token once
     Sums all = o;
     double held = 0.0;
@@ -62,16 +54,28 @@ template <typename T, bool REST> __device__ __forceinline__ void finish(const Di
     const bool none = all.s == 0.0f, apart = REST && !(o.s == 0.0f);
     const double inv_t = a.inv_t, log_s = log((double)all.s);
     const double logp = !used || none ? -(double)kInf : ((double)x - all.m) * inv_t - log_s;
-    if (apart && norm <= 0.0) norm = 0.0;
-    const double q = !some ? 0.0 : exp((double)teacher - norm);
-    double loss = wave_sum(q == 0.0 ? 0.0 : q * ((double)teacher - norm - logp)), over = has ? 1.0 : 0.0;
-    if (norm != norm) over = norm;
+    // the teacher: its probabilities, their sum, and the log of what they are divided by
+    const bool some = used && !(teacher == -kInf); // NaN too
+    const bool has = __ballot(some) != 0;
+    float most = wave_most(some ? teacher : -kInf);
+    if (most == -kInf) most = 0.0f; // nothing, or nothing but NaN
+    double q = some ? exp((double)teacher - most) : 0.0, total = wave_sum(q), norm = 0.0;
+    const double size = apart ? exp((double)most) : 0.0;
+    if (apart && total * size <= 1.0) q *= size, total *= size;
+    else {
+        norm = has ? (double)most + log(total) : -(double)kInf;
+        if (some) q /= total;
+        total = 1.0;
+    }
+    double loss = wave_sum(q == 0.0 ? 0.0 : q * ((double)teacher - norm - logp)), over = has ? norm == norm ? 1.0 : norm : 0.0, log_o = log_s;
     if (apart) {
-        const double total = wave_sum(q), left = 1.0 - total, qr = left < 0.0 ? 0.0 : left;
-        // the log of what is left, from what is held where that is the smaller part
-        const double log_r = held < 0.5 ? log1p(-held) : ((double)o.m - all.m) * inv_t + log((double)o.s) - log_s;
-        loss += qr == 0.0 ? 0.0 : qr * (log(qr) - log_r);
+        const double qr = 1.0 - total;
+        log_o = log((double)o.s);
+        // logs of what is left, from what is not where that is the smaller part
+        const double log_r = held < 0.5 ? (double)log1pf((float)-held) : ((double)o.m - all.m) * inv_t + log_o - log_s;
+        if (qr != 0.0) loss += qr * ((total < 0.5 ? (double)log1pf((float)-total) : log(qr)) - log_r);
         over = held < 0.5 ? total - held : exp(log_r) - qr;
+        if (norm != norm) over = norm;
     } else o = all;
     if (lane != 0) return;
     a.loss[row] = (float)loss;
@@ -79,7 +83,7 @@ template <typename T, bool REST> __device__ __forceinline__ void finish(const Di
     st[0] = none ? -kInf : all.m;
     st[1] = (float)log_s;
     st[2] = none ? -kInf : o.m;
-    st[3] = apart ? (float)log((double)o.s) : (float)log_s;
+    st[3] = (float)log_o;
     st[4] = (float)norm;
     st[5] = (float)over;
 }
@@ -170,7 +174,10 @@ uint32_t slices_of(uint64_t vectors) { return (uint32_t)((vectors + kSlice - 1) 
  *    64         16000           14.7 19.2           10.3 13.7                 8.1 10.6
  *   128         16000           15.5 20.0           11.2 14.3                11.0 13.5
  *   256         32000           21.5 25.9           21.8 24.4                24.1 26.6
- *   400         16000           19.4 23.6           21.7 25.6                23.0 25.5 */
+ *   400         16000           19.4 23.6           21.7 25.6                23.0 25.5
+ * and a wave to a row, bf16:
+ * 16384 rows of  375 vectors   33.6 63.7, not 26.4 41.4;   750   43.0 74.1, 41.9 56.4;   1500   65.3 93.7, 76.6 86.0
+ *   200          375            6.1  6.7       6.0  7.8;   1500    5.8  7.5,  7.1 10.9 */
 template <typename T, bool REST> void launch(DistillArgs &a, uint64_t all_rows, hipStream_t s) {
     const uint32_t rows = a.rows - a.first, n = vectors_most<T>(a.vocab);
 #define ERI_DISTILL(TPR, ONCE) hipLaunchKernelGGL((distill_kernel<T, TPR, REST, false, ONCE>), dim3(rows), dim3(TPR), 0, s, a)
@@ -178,7 +185,7 @@ template <typename T, bool REST> void launch(DistillArgs &a, uint64_t all_rows, 
     if (n > kLong && all_rows <= kFew && a.slices <= kSlicesMost) {
         hipLaunchKernelGGL((distill_kernel<T, 256, REST, true, false>), dim3(rows * a.slices), dim3(256), 0, s, a);
         hipLaunchKernelGGL((distill_join_kernel<T, REST>), dim3(rows), dim3(64), 0, s, a);
-    } else if (n <= 256) ERI_DISTILL(64, false);
+    } else if (n <= 256 || (all_rows >= 1024 && n <= (REST ? 2048 : 1024))) ERI_DISTILL(64, false);
     else if (n > 2048 && all_rows <= 256) ERI_DISTILL(1024, false);
     else if (all_rows * a.vocab * sizeof(T) > kCache) ERI_DISTILL(256, true);
     else ERI_DISTILL(256, false);

@@ -69,9 +69,10 @@ template <int TPR, bool ONCE, typename T, typename O> __device__ __forceinline__
 /* log2 p of an element, from {m, ln s}: nothing is left of a row where ln s is minus infinity. */
 struct LogP {
     float m, log2_s, c;
-    __device__ __forceinline__ LogP(const float *stats, float c_) : m(stats[0]), c(c_) {
-        log2_s = stats[1] == -kInf ? kInf : stats[1] * (float)kLog2e;
-        if (stats[1] == -kInf) m = 0.0f;
+    __device__ __forceinline__ LogP(const float *stats, float c_) : c(c_) {
+        const float first = stats[0], log_s = stats[1];
+        m = log_s == -kInf ? 0.0f : first;
+        log2_s = log_s == -kInf ? kInf : log_s * (float)kLog2e;
     }
     __device__ __forceinline__ float operator()(float x) const { return fmaf(x - m, c, -log2_s); }
 };
@@ -84,18 +85,15 @@ template <typename T, typename O, int TPR, bool ENT, bool ONCE> __global__ __lau
     const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
     const uint32_t all = row.vectors(), first = slice * a.per < all ? slice * a.per : all, end = all - first > a.per ? first + a.per : all;
     O *out = (O *)a.out + index * a.out_stride - row.skip;
-    int64_t id = -1;
-    float g = 0.0f, h = 0.0f;
-    if (a.grad) {
-        id = id_at(a.ids, a.ids_64, index);
-        if (id >= 0 && id < (int64_t)a.vocab) g = a.grad[index];
-        else id = -1;
-    }
-    if (ENT) h = a.grad_entropy[index];
-    if (g == 0.0f && h == 0.0f) return zeros<TPR, ONCE>(row, out, first, end, t);
+    // all that is known of the row is asked for at once, not one after the other
+    const int64_t id = a.grad ? id_at(a.ids, a.ids_64, index) : -1;
+    float g = a.grad ? a.grad[index] : 0.0f;
+    const float h = ENT ? a.grad_entropy[index] : 0.0f, entropy = ENT ? a.entropy[index] : 0.0f;
     const LogP log2p(a.stats + index * 2, a.c);
+    if (id < 0 || id >= (int64_t)a.vocab) g = 0.0f;
+    if (g == 0.0f && h == 0.0f) return zeros<TPR, ONCE>(row, out, first, end, t);
     const uint32_t named = g == 0.0f || log2p.log2_s == kInf ? ~0u : row.skip + (uint32_t)id;
-    const float u = -(ENT ? fmaf(h, log2p.log2_s == kInf ? 0.0f : a.entropy[index], g) : g) * a.inv_t, w = -h * kLn2 * a.inv_t, more = g * a.inv_t;
+    const float u = -(ENT ? fmaf(h, log2p.log2_s == kInf ? 0.0f : entropy, g) : g) * a.inv_t, w = -h * kLn2 * a.inv_t, more = g * a.inv_t;
     each<TPR, ONCE>(row, out, first, end, t, [&](float(&v)[kEach<T>], uint32_t place) {
 #pragma unroll
         for (uint32_t e = 0; e < kEach<T>; ++e) {
@@ -174,10 +172,16 @@ template <typename F> int in_parts(GradArgs &a, uint64_t rows, uint32_t rows_of_
     return 0;
 }
 
+/* Whether a wave has a row: short ones, and longer ones where there are many: 16384 x 3000 bf16 35 us for 51, and 44 for 61 (scores, distillation), 6000 75
+ * for 77, and 100 for 93; 200 x 6000 5.1 for 7.1. */
+template <typename T> bool by_waves(uint64_t vocab, uint64_t rows, uint32_t many) {
+    const uint32_t n = vectors_most<T>(vocab);
+    return n <= 256 || (rows >= 1024 && n <= many);
+}
 template <typename T, typename O> int token_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
 #define ERI_GRAD(TPR, ENT, ONCE) in_parts(a, rows, 256 / TPR, [&](uint32_t n) { hipLaunchKernelGGL((token_grad_kernel<T, O, TPR, ENT, ONCE>), dim3(n), dim3(256), 0, s, a); })
     const bool once = cut<T, O>(a, rows, kBatch * 256);
-    if (a.per <= 256) return a.grad_entropy ? ERI_GRAD(64, true, false) : ERI_GRAD(64, false, false);
+    if (by_waves<T>(a.vocab, rows, 512)) return a.grad_entropy ? ERI_GRAD(64, true, false) : ERI_GRAD(64, false, false);
     if (once) return a.grad_entropy ? ERI_GRAD(256, true, true) : ERI_GRAD(256, false, true);
     return a.grad_entropy ? ERI_GRAD(256, true, false) : ERI_GRAD(256, false, false);
 #undef ERI_GRAD
@@ -186,7 +190,7 @@ template <typename T, typename O> int distill_grad(GradArgs &a, uint64_t rows, h
 #define ERI_GRAD(TPR, ONCE) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR, ONCE>), dim3(n), dim3(TPR), 0, s, a); })
     // looking up the teacher's tokens costs each workgroup a few us: worth it in rows of some length, or where there are few of them
     const bool once = cut<T, O>(a, rows, rows >= 1024 && vectors_most<T>(a.vocab) <= 4 * kBatch * 256 ? 4 * kBatch * 256 : kBatch * 256);
-    return a.per <= 256 ? ERI_GRAD(64, false) : once ? ERI_GRAD(256, true) : ERI_GRAD(256, false);
+    return by_waves<T>(a.vocab, rows, 1024) ? ERI_GRAD(64, false) : once ? ERI_GRAD(256, true) : ERI_GRAD(256, false);
 #undef ERI_GRAD
 }
 } // namespace

@@ -52,7 +52,7 @@ template <typename T> __device__ __forceinline__ bool token_of(const ScoreArgs &
 }
 
 /* What the threads of a workgroup tell each other about their elements. */
-constexpr uint32_t kMarks = 8192; // largest values of a few vectors each, over all threads
+template <int TPR> constexpr uint32_t kMarks = TPR > (int)kWave ? 8192 : 1024; // largest values of a few vectors each, over all threads; a wave has shorter rows
 template <int TPR> struct TopSpace {
     Key lists[TPR];
     uint32_t found[TPR]; // columns, 64 to a wave
@@ -60,8 +60,8 @@ template <int TPR> struct TopSpace {
     uint32_t places_n;
 };
 template <int TPR> struct Marks {
-    uint16_t values[kMarks];
-    uint16_t places[kWave * (kMarks / TPR)]; // those that reach the bound: only 64 threads have any
+    uint16_t values[kMarks<TPR>];
+    uint16_t places[kWave * (kMarks<TPR> / TPR)]; // those that reach the bound: only 64 threads have any
 };
 
 /* The upper 16 bits of a value, rounded up. */
@@ -258,8 +258,9 @@ template <typename T, int TPR, bool ENT, bool TOP, bool ONCE> __global__ __launc
     if (t < kWave) finish<T, ENT, TOP>(a, index, r, k, x, named, t);
 }
 
-/* Rows of more than kLong vectors are cut where there are no more than kFew of them, into slices of 4 vectors a thread. */
+/* Rows of more than kLong vectors are cut where there are no more than kFew of them, into slices of 32 columns a thread. */
 constexpr uint32_t kLong = 8192, kFew = 64, kSlicesMost = 64, kSliceThreads = 256;
+template <typename T> constexpr uint32_t kSliceBatch = 32 / kEach<T>;
 
 /* A slice of a row that a workgroup's registers hold: nothing is read twice. */
 template <typename T, int TPR, bool ENT, bool TOP> __global__ __launch_bounds__(TPR) void score_slice_kernel(const ScoreArgs a) {
@@ -270,13 +271,13 @@ template <typename T, int TPR, bool ENT, bool TOP> __global__ __launch_bounds__(
     const uint32_t t = threadIdx.x;
     const uint64_t index = a.first + blockIdx.x / a.slices;
     const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
-    const uint32_t all = row.vectors(), first = blockIdx.x % a.slices * (kBatch * TPR);
-    u32x4 raw[kBatch];
+    const uint32_t all = row.vectors(), first = blockIdx.x % a.slices * (kSliceBatch<T> * TPR);
+    u32x4 raw[kSliceBatch<T>];
 #pragma unroll
-    for (uint32_t k = 0; k < kBatch; ++k) raw[k] = load_any<false>(row, first + k * TPR + t); // nothing where the row has no such vector
-    float v[kBatch][kEach<T>];
+    for (uint32_t k = 0; k < kSliceBatch<T>; ++k) raw[k] = load_any<false>(row, first + k * TPR + t); // nothing where the row has no such vector
+    float v[kSliceBatch<T>][kEach<T>];
 #pragma unroll
-    for (uint32_t k = 0; k < kBatch; ++k) values_of(v[k], raw[k]);
+    for (uint32_t k = 0; k < kSliceBatch<T>; ++k) values_of(v[k], raw[k]);
     Sums r = {kLowest, 0.0f, 0.0f};
     add<ENT>(r, v, a.c);
     group_join<ENT, WAVES>(r, a.c, slots);
@@ -284,8 +285,13 @@ template <typename T, int TPR, bool ENT, bool TOP> __global__ __launch_bounds__(
     if (TOP) {
         Best best = {-kInf, first_of<TPR>(row, first, t)};
 #pragma unroll
-        for (uint32_t i = 0; i < kBatch; ++i) best.take(v[i], first + i * TPR + t);
-        const Key own = best.place < all ? key_of(best.value, best.place) : 0, bound = bound_of<TPR>(own, a.top_n, sp);
+        for (uint32_t i = 0; i < kSliceBatch<T>; ++i) best.take(v[i], first + i * TPR + t);
+        const Key own = best.place < all ? key_of(best.value, best.place) : 0;
+        Key bound = own;
+        if (a.top_n <= kWave / 2) { // each wave by itself: it keeps about as many elements as are wanted, and the waves need not wait for each other
+            sort64(bound, t % kWave);
+            bound = (Key)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bound >> 32), (int)a.top_n - 1) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bound, (int)a.top_n - 1);
+        } else bound = bound_of<TPR>(own, a.top_n, sp);
         Largest<T> found(row, bound, sp.found);
         found.take(v, own >= bound && own != 0, [&](uint32_t i) { return first + i * TPR + t; });
         found.sort();
@@ -333,10 +339,10 @@ template <typename T, bool ENT, bool TOP> __global__ __launch_bounds__(512) void
     finish<T, ENT, TOP>(a, index, r, k, x, named, lane);
 }
 
-uint32_t slices_of(uint64_t vectors) { return (uint32_t)((vectors + kBatch * kSliceThreads - 1) / (kBatch * kSliceThreads)); }
+uint32_t slices_of(uint64_t vocab) { return (uint32_t)((vocab + 63 + 32 * kSliceThreads - 1) / (32 * kSliceThreads)); } // up to 63 columns of the first are none
 uint64_t parts_most(uint64_t rows, uint64_t vocab) {
-    const uint64_t n = vectors_most<float>(vocab), slices = slices_of(n < kSlicesMost * kBatch * kSliceThreads ? n : kSlicesMost * kBatch * kSliceThreads);
-    return n > kLong ? (rows < kFew ? rows : kFew) * slices : 0;
+    const uint64_t slices = slices_of(vocab);
+    return vectors_most<float>(vocab) > kLong ? (rows < kFew ? rows : kFew) * (slices < kSlicesMost ? slices : kSlicesMost) : 0;
 }
 
 /* Threads to a row.  us for a call, bf16 and f32, with and without 20 alternatives:
@@ -347,19 +353,23 @@ uint64_t parts_most(uint64_t rows, uint64_t vocab) {
  *    64         16000           12.8 19.2            9.8 16.2                 7.7 13.3
  *   128         16000           14.4 21.0           10.5 16.8                 9.9 18.7
  *   256         32000           26.7 34.4           21.6 27.6                24.4 41.6
- *   400         16000           18.4 25.3           20.2 33.1                19.8 39.5 */
+ *   400         16000           18.4 25.3           20.2 33.1                19.8 39.5
+ * and a wave to a row, bf16:
+ * 16384 rows of  375 vectors   23.6 75.6, not 18.2 30.9;   750   35.7 88.9, 37.0 46.5;   1500   60.2 113,  71.7 84.5
+ *   200          375            6.1  7.0       6.1  7.2;   1500    5.8  7.6,  5.9  9.3
+ * With 64 alternatives each lane of a wave is above the bound: 16384 rows of 750 vectors 93.3, not 96.5, of 1500 129 and 172; with 48 and fewer a wave wins. */
 template <typename T, bool ENT, bool TOP> void launch(ScoreArgs &a, uint64_t all_rows, hipStream_t s) {
     const uint32_t rows = a.rows - a.first, n = vectors_most<T>(a.vocab);
 #define ERI_SCORE(TPR, ONCE) \
     do { \
-        for (a.shift = 1; n / TPR >> a.shift >= kMarks / TPR;) ++a.shift; \
+        for (a.shift = 1; n / TPR >> a.shift >= kMarks<TPR> / TPR;) ++a.shift; \
         hipLaunchKernelGGL((score_kernel<T, TPR, ENT, TOP, ONCE>), dim3(rows), dim3(TPR), 0, s, a); \
     } while (0)
-    a.slices = slices_of(n);
+    a.slices = slices_of(a.vocab);
     if (n > kLong && all_rows <= kFew && a.slices <= kSlicesMost) {
         hipLaunchKernelGGL((score_slice_kernel<T, kSliceThreads, ENT, TOP>), dim3(rows * a.slices), dim3(kSliceThreads), 0, s, a);
         hipLaunchKernelGGL((score_join_kernel<T, ENT, TOP>), dim3(rows), dim3(TOP ? 512 : 64), 0, s, a);
-    } else if (n <= 256) ERI_SCORE(64, false);
+    } else if (n <= 256 || (all_rows >= 1024 && n <= (TOP && a.top_n <= 48 ? 2048u : 512u))) ERI_SCORE(64, false);
     else if (n > kLong && all_rows <= 256) ERI_SCORE(1024, false);
     else if (all_rows * a.vocab * sizeof(T) > kCache) ERI_SCORE(256, true);
     else ERI_SCORE(256, false);
