@@ -2,8 +2,8 @@
  * The logits' gradients of include/eri_losses.h: one pass that reads a row and writes a row.
  *
  *     scores        (g ([j = id] - p) - h p (ln p + H)) / T = p (u + w log2 p) + [j = id] g / T,  u = -(g + h H) / T,  w = -h ln 2 / T
- *     distillation  p_j / p_r (p_r - q_r) g / T for the tokens that the teacher does not name, written everywhere; the named ones,
- *                   (p_j - q_j) g / T, are computed by one wave before and put in their places afterwards
+ *     distillation  p_j / p_r (p_r - q_r) g / T for the tokens that the teacher does not name, (p_j - q_j) g / T for those it names, which each workgroup
+ *                   marks in LDS before it begins
  * with log2 p = (x - m) log2(e) / T - log2 s in one fused product: one exponential an element, which is a quarter of the arithmetic.
  */
 #include "eri_losses_device.h"
@@ -50,14 +50,16 @@ template <bool ONCE, typename T, typename O, int E> __device__ __forceinline__ v
         for (uint32_t e = 0; e < (uint32_t)E; ++e)
             if (row.has(vec, e)) store_one(out + (uint64_t)vec * E + e, v[e]);
 }
-template <int TPR, bool ONCE, typename T, typename O, typename Of> __device__ __forceinline__ void each(const Row<T> &row, O *out, uint32_t first, uint32_t end, uint32_t t, Of of) {
-    walk<TPR, ONCE>(row, first, end, t, [&](auto &v, uint32_t at, bool full) {
+enum Past { kNothing, kStores, kBoth }; // what passes the caches by
+
+template <int TPR, Past PAST, typename T, typename O, typename Of> __device__ __forceinline__ void each(const Row<T> &row, O *out, uint32_t first, uint32_t end, uint32_t t, Of of) {
+    walk<TPR, PAST == kBoth>(row, first, end, t, [&](auto &v, uint32_t at, bool full) {
 #pragma unroll
         for (uint32_t k = 0; k < sizeof v / sizeof v[0]; ++k) {
             const uint32_t vec = at + k * TPR + t;
             of(v[k], vec * kEach<T>);
-            if (full) store_whole<ONCE>(out + (uint64_t)vec * kEach<T>, v[k]);
-            else store_any<ONCE>(out, row, vec, end, v[k]);
+            if (full) store_whole<PAST != kNothing>(out + (uint64_t)vec * kEach<T>, v[k]);
+            else store_any<PAST != kNothing>(out, row, vec, end, v[k]);
         }
     });
 }
@@ -77,7 +79,7 @@ struct LogP {
     __device__ __forceinline__ float operator()(float x) const { return fmaf(x - m, c, -log2_s); }
 };
 
-template <typename T, typename O, int TPR, bool ENT, bool ONCE> __global__ __launch_bounds__(256) void token_grad_kernel(const GradArgs a) {
+template <typename T, typename O, int TPR, bool ENT, Past PAST> __global__ __launch_bounds__(256) void token_grad_kernel(const GradArgs a) {
     constexpr uint32_t ROWS = 256 / TPR;
     const uint32_t t = threadIdx.x % TPR, slice = blockIdx.x % a.slices;
     const uint64_t index = a.first + (uint64_t)(blockIdx.x / a.slices) * ROWS + (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x / TPR));
@@ -91,10 +93,10 @@ template <typename T, typename O, int TPR, bool ENT, bool ONCE> __global__ __lau
     const float h = ENT ? a.grad_entropy[index] : 0.0f, entropy = ENT ? a.entropy[index] : 0.0f;
     const LogP log2p(a.stats + index * 2, a.c);
     if (id < 0 || id >= (int64_t)a.vocab) g = 0.0f;
-    if (g == 0.0f && h == 0.0f) return zeros<TPR, ONCE>(row, out, first, end, t);
+    if (g == 0.0f && h == 0.0f) return zeros<TPR, PAST != kNothing>(row, out, first, end, t);
     const uint32_t named = g == 0.0f || log2p.log2_s == kInf ? ~0u : row.skip + (uint32_t)id;
     const float u = -(ENT ? fmaf(h, log2p.log2_s == kInf ? 0.0f : entropy, g) : g) * a.inv_t, w = -h * kLn2 * a.inv_t, more = g * a.inv_t;
-    each<TPR, ONCE>(row, out, first, end, t, [&](float(&v)[kEach<T>], uint32_t place) {
+    each<TPR, PAST>(row, out, first, end, t, [&](float(&v)[kEach<T>], uint32_t place) {
 #pragma unroll
         for (uint32_t e = 0; e < kEach<T>; ++e) {
             const float l = log2p(v[e]), p = exp2_of(l);
@@ -108,55 +110,79 @@ template <typename T, typename O, int TPR, bool ENT, bool ONCE> __global__ __lau
     });
 }
 
-template <typename T, typename O, int TPR, bool ONCE> __global__ __launch_bounds__(TPR) void distill_grad_kernel(const GradArgs a) {
+constexpr uint32_t kDistillMost = 4096; // vectors of a row or slice
+
+template <typename T, typename O, int TPR, Past PAST> __global__ __launch_bounds__(TPR) void distill_grad_kernel(const GradArgs a) {
+    constexpr uint32_t MOST = TPR > (int)kWave ? kDistillMost : kDistillMost / 4;
+    __shared__ uint32_t named[MOST / 4]; // a byte for each vector: which of its elements the teacher names
+    __shared__ uint32_t places[kWave] __attribute__((aligned(16)));
+    __shared__ float shares[kWave] __attribute__((aligned(16)));
     const uint32_t t = threadIdx.x, slice = blockIdx.x % a.slices;
     const uint64_t index = a.first + blockIdx.x / a.slices;
     const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
     const uint32_t all = row.vectors(), first = slice * a.per < all ? slice * a.per : all, end = all - first > a.per ? first + a.per : all;
     O *out = (O *)a.out + index * a.out_stride - row.skip;
-    const float g = a.grad[index] * a.inv_t, *st = a.stats + index * 6;
-    if (a.grad[index] == 0.0f || st[1] == -kInf) return zeros<TPR, ONCE>(row, out, first, end, t);
-    int32_t id = -1;
-    float value = 0.0f;
-    if (t < kWave) {
-        float q = 0.0f;
-        if (t < a.k) {
-            const int64_t given = id_at(a.ids, a.ids_64, index * a.ids_stride + t);
-            if (given >= 0 && given < (int64_t)a.vocab) id = (int32_t)given;
-            if (id >= 0 && st[4] != -kInf) q = exp2_of((bf16_or_f32{a.teacher, a.teacher_f32 != 0}[index * a.teacher_stride + t] - st[4]) * (float)kLog2e);
-        }
-        float sum = 0.0f; // over the entries of the same token
-        for (uint32_t j = 0; j < a.k; ++j)
-            if (__builtin_amdgcn_readlane(id, (int)j) == id) sum += lane_of(q, (int)j);
-        const uint32_t vec = (row.skip + (uint32_t)id) / kEach<T>;
-        if (id >= 0 && vec >= first && vec < end) {
-            const LogP log2p(st, a.c);
-            const float p = st[4] == -kInf ? 0.0f : exp2_of(log2p(at(row.from + row.skip + id)));
-            value = (p - sum) * g;
-        } else id = -1;
+    const float given = a.grad[index], g = given * a.inv_t, *st = a.stats + index * 6, norm = st[4], over = st[5] * g;
+    int64_t id = -1;
+    float q = 0.0f;
+    if (t < a.k) {
+        id = id_at(a.ids, a.ids_64, index * a.ids_stride + t);
+        q = bf16_or_f32{a.teacher, a.teacher_f32 != 0}[index * a.teacher_stride + t];
     }
-    __syncthreads(); // the named logits have been read, before out may be written over them
-    const LogP log2r(st + 2, a.c);
-    const float over = st[5] * g;
-    each<TPR, ONCE>(row, out, first, end, t, [&](float(&v)[kEach<T>], uint32_t) {
-#pragma unroll
-        for (uint32_t e = 0; e < kEach<T>; ++e) v[e] = exp2_of(log2r(v[e])) * over;
-    });
+    const LogP log2p(st, a.c), log2r(st + 2, a.c);
+    if (given == 0.0f || st[1] == -kInf) return zeros<TPR, PAST != kNothing>(row, out, first, end, t);
+    for (uint32_t i = t; i < (end - first + 3) / 4; i += TPR) named[i] = 0;
+    const uint32_t place = row.skip + (uint32_t)id, vec = place / kEach<T> - first;
+    const bool here = id >= 0 && id < (int64_t)a.vocab && place / kEach<T> >= first && place / kEach<T> < end;
     __syncthreads();
-    if (id >= 0) store_one(out + row.skip + id, value);
+    if (t < kWave) {
+        if (here) atomicOr(&named[vec / 4], 1u << (vec % 4 * 8 + place % kEach<T>));
+        places[t] = here ? place : ~0u;
+        shares[t] = here && norm != -kInf ? exp2_of((q - norm) * (float)kLog2e) : 0.0f;
+    }
+    __syncthreads();
+    each<TPR, PAST>(row, out, first, end, t, [&](float(&v)[kEach<T>], uint32_t from) {
+        float r[kEach<T>];
+#pragma unroll
+        for (uint32_t e = 0; e < kEach<T>; ++e) r[e] = exp2_of(log2r(v[e])) * over;
+        uint32_t which = from / kEach<T> < end ? ((const uint8_t *)named)[from / kEach<T> - first] : 0;
+        for (; which != 0; which &= which - 1) {
+            const uint32_t e = (uint32_t)__builtin_ctz(which);
+            float x = v[0], sum = 0.0f; // over the entries of this token
+            for (uint32_t j = 0; j < a.k; j += 4) {
+                const u32x4 p = *(const u32x4 *)&places[j], q4 = *(const u32x4 *)&shares[j];
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) sum += p[i] == from + e ? as_float(q4[i]) : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t i = 1; i < kEach<T>; ++i) x = i == e ? v[i] : x;
+            const float value = ((norm == -kInf ? 0.0f : exp2_of(log2p(x))) - sum) * g;
+#pragma unroll
+            for (uint32_t i = 0; i < kEach<T>; ++i) r[i] = i == e ? value : r[i];
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < kEach<T>; ++e) v[e] = r[e];
+    });
 }
 
 constexpr uint32_t kBlocks = 1u << 23; // of a launch
 
-/* Cuts rows into slices of one batch for each thread, or of `per` vectors; whether what is read and written passes the caches by.
- * With one batch to a workgroup the chip works within one window of the memory: 8192 x 128000 bf16 729 us for the scores and 689 for the
- * distillation, where a workgroup had a row 759 and 750, and 791 and 774 with what is stored passing the caches and what is read not.  A
- * float32 gradient of bf16 logits, whose 16-byte stores leave gaps for one another, takes 522 in the caches and 599 past them. */
-template <typename T, typename O> bool cut(GradArgs &a, uint64_t rows, uint32_t per) {
+/* Cuts rows into slices; whether the logits are more than the last cache holds.  A small part of a row to each workgroup keeps the chip within one
+ * window of the memory, and what is stored, and for float32 scores what is read too, passes the caches by.  us with 2048, 1024 and 512
+ * vectors to a workgroup, both past the caches, and (the stores alone):
+ *     scores        8192 x 128000 bf16     768 (785)  758 (749)  726 (892)      distillation  776 (793)  771 (796)  671 (668)
+ *                  16384 x 32000           371 (383)  370 (330)  358 (425)                    391 (400)  390 (399)  390 (400)
+ *                  16384 x 50257           624 (628)  538 (510)  599 (659)                    603 (610)  553 (592)  552 (510)
+ *                   4096 x 128000 f32      763 (784)  708 (776)  684 (700)                    765 (785)  772 (797)  662 (643)
+ * before, with a row to a workgroup and all of it through the caches, 8192 x 128000 took 817 and 842.  A float32 gradient of bf16 logits, whose
+ * 16-byte stores leave gaps for one another, takes 522 through the caches and 599 past them. */
+template <typename T, typename O> bool cut(GradArgs &a, uint64_t rows, uint32_t per, uint32_t per_large) {
     const uint32_t n = vectors_most<T>(a.vocab);
-    a.per = n < per ? n : per;
+    const bool large = sizeof(O) <= sizeof(T) && rows * a.vocab * sizeof(T) > kCache;
+    a.per = large ? per_large : per;
+    if (a.per > n) a.per = n;
     a.slices = (n + a.per - 1) / a.per;
-    return sizeof(O) <= sizeof(T) && rows * a.vocab * sizeof(T) > kCache;
+    return large;
 }
 
 /* Launches over parts of the rows, so that a launch can count its threads. */
@@ -179,18 +205,26 @@ template <typename T> bool by_waves(uint64_t vocab, uint64_t rows, uint32_t many
     return n <= 256 || (rows >= 1024 && n <= many);
 }
 template <typename T, typename O> int token_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
-#define ERI_GRAD(TPR, ENT, ONCE) in_parts(a, rows, 256 / TPR, [&](uint32_t n) { hipLaunchKernelGGL((token_grad_kernel<T, O, TPR, ENT, ONCE>), dim3(n), dim3(256), 0, s, a); })
-    const bool once = cut<T, O>(a, rows, kBatch * 256);
-    if (by_waves<T>(a.vocab, rows, 512)) return a.grad_entropy ? ERI_GRAD(64, true, false) : ERI_GRAD(64, false, false);
-    if (once) return a.grad_entropy ? ERI_GRAD(256, true, true) : ERI_GRAD(256, false, true);
-    return a.grad_entropy ? ERI_GRAD(256, true, false) : ERI_GRAD(256, false, false);
+#define ERI_GRAD(TPR, ENT, PAST) in_parts(a, rows, 256 / TPR, [&](uint32_t n) { hipLaunchKernelGGL((token_grad_kernel<T, O, TPR, ENT, PAST>), dim3(n), dim3(256), 0, s, a); })
+    constexpr bool kWide = sizeof(T) == 4;
+    const bool large = cut<T, O>(a, rows, kBatch * 256, kWide ? 512 : kBatch * 256);
+    if (by_waves<T>(a.vocab, rows, 512)) {
+        a.per = vectors_most<T>(a.vocab), a.slices = 1;
+        return a.grad_entropy ? ERI_GRAD(64, true, kNothing) : ERI_GRAD(64, false, kNothing);
+    }
+    if (!large) return a.grad_entropy ? ERI_GRAD(256, true, kNothing) : ERI_GRAD(256, false, kNothing);
+    return a.grad_entropy ? ERI_GRAD(256, true, (kWide ? kBoth : kStores)) : ERI_GRAD(256, false, (kWide ? kBoth : kStores));
 #undef ERI_GRAD
 }
 template <typename T, typename O> int distill_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
-#define ERI_GRAD(TPR, ONCE) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR, ONCE>), dim3(n), dim3(TPR), 0, s, a); })
-    // looking up the teacher's tokens costs each workgroup a few us: worth it in rows of some length, or where there are few of them
-    const bool once = cut<T, O>(a, rows, rows >= 1024 && vectors_most<T>(a.vocab) <= 4 * kBatch * 256 ? 4 * kBatch * 256 : kBatch * 256);
-    return by_waves<T>(a.vocab, rows, 1024) ? ERI_GRAD(64, false) : once ? ERI_GRAD(256, true) : ERI_GRAD(256, false);
+#define ERI_GRAD(TPR, PAST) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR, PAST>), dim3(n), dim3(TPR), 0, s, a); })
+    // looking up the teacher's tokens costs each workgroup something: longer slices, unless the rows are few
+    const bool large = cut<T, O>(a, rows, rows >= 1024 && vectors_most<T>(a.vocab) <= kDistillMost ? kDistillMost : kBatch * 256, 512);
+    if (by_waves<T>(a.vocab, rows, kDistillMost / 4)) {
+        a.per = vectors_most<T>(a.vocab), a.slices = 1;
+        return ERI_GRAD(64, kNothing);
+    }
+    return large ? ERI_GRAD(256, kStores) : ERI_GRAD(256, kNothing);
 #undef ERI_GRAD
 }
 } // namespace
