@@ -12,7 +12,9 @@ using namespace eri_layers;
 
 constexpr float kInf = __builtin_inff();
 constexpr float kLowest = -3.40282347e38f; // the running maximum before the first element: finite, so that its distance to minus infinity is no NaN
-constexpr float kFloor = -1e30f;           // below any distance that counts: 0 * kFloor is 0 where 0 * -infinity would be NaN
+constexpr float kFloor = -1e28f;           // below any distance that counts: 0 * kFloor is 0 where 0 * -infinity would be NaN, and 2^31 of them are finite
+/* Rows of more than kLong vectors are cut where there are no more than kFew of them. */
+constexpr uint32_t kLong = 8192, kFew = 64, kSlicesMost = 64;
 constexpr uint64_t kCache = 256u << 20;        // bytes of the last cache
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr float kLn2 = 0.693147181f;

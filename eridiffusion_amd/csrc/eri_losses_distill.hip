@@ -88,8 +88,7 @@ template <typename T, bool REST> __device__ __forceinline__ void finish(const Di
     st[5] = (float)over;
 }
 
-/* Rows of more than kLong vectors are cut where there are no more than kFew of them, into slices of 4 vectors a thread. */
-constexpr uint32_t kLong = 8192, kFew = 64, kSlicesMost = 64, kSlice = kBatch * 256;
+constexpr uint32_t kSlice = kBatch * 256; // vectors
 
 template <typename T, int TPR, bool REST, bool SPLIT, bool ONCE> __global__ __launch_bounds__(TPR) void distill_kernel(const DistillArgs a) {
     constexpr int WAVES = TPR / (int)kWave;
@@ -180,14 +179,17 @@ uint32_t slices_of(uint64_t vectors) { return (uint32_t)((vectors + kSlice - 1) 
  *   200          375            6.1  6.7       6.0  7.8;   1500    5.8  7.5,  7.1 10.9 */
 template <typename T, bool REST> void launch(DistillArgs &a, uint64_t all_rows, hipStream_t s) {
     const uint32_t rows = a.rows - a.first, n = vectors_most<T>(a.vocab);
+    const bool large = all_rows * a.vocab * sizeof(T) > kCache;
 #define ERI_DISTILL(TPR, ONCE) hipLaunchKernelGGL((distill_kernel<T, TPR, REST, false, ONCE>), dim3(rows), dim3(TPR), 0, s, a)
     a.slices = slices_of(n);
     if (n > kLong && all_rows <= kFew && a.slices <= kSlicesMost) {
         hipLaunchKernelGGL((distill_kernel<T, 256, REST, true, false>), dim3(rows * a.slices), dim3(256), 0, s, a);
         hipLaunchKernelGGL((distill_join_kernel<T, REST>), dim3(rows), dim3(64), 0, s, a);
-    } else if (n <= 256 || (all_rows >= 1024 && n <= (REST ? 2048 : 1024))) ERI_DISTILL(64, false);
-    else if (n > 2048 && all_rows <= 256) ERI_DISTILL(1024, false);
-    else if (all_rows * a.vocab * sizeof(T) > kCache) ERI_DISTILL(256, true);
+    } else if (n <= 256 || (all_rows >= 1024 && n <= (REST ? 2048 : 1024))) {
+        if (large) ERI_DISTILL(64, true);
+        else ERI_DISTILL(64, false);
+    } else if (n > 2048 && all_rows <= 256) ERI_DISTILL(1024, false);
+    else if (large) ERI_DISTILL(256, true);
     else ERI_DISTILL(256, false);
 #undef ERI_DISTILL
 }

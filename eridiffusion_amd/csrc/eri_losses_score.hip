@@ -258,9 +258,8 @@ template <typename T, int TPR, bool ENT, bool TOP, bool ONCE> __global__ __launc
     if (t < kWave) finish<T, ENT, TOP>(a, index, r, k, x, named, t);
 }
 
-/* Rows of more than kLong vectors are cut where there are no more than kFew of them, into slices of 32 columns a thread. */
-constexpr uint32_t kLong = 8192, kFew = 64, kSlicesMost = 64, kSliceThreads = 256;
-template <typename T> constexpr uint32_t kSliceBatch = 32 / kEach<T>;
+constexpr uint32_t kSliceThreads = 256;
+template <typename T> constexpr uint32_t kSliceBatch = 32 / kEach<T>; // 32 columns to a thread
 
 /* A slice of a row that a workgroup's registers hold: nothing is read twice. */
 template <typename T, int TPR, bool ENT, bool TOP> __global__ __launch_bounds__(TPR) void score_slice_kernel(const ScoreArgs a) {
@@ -360,6 +359,7 @@ uint64_t parts_most(uint64_t rows, uint64_t vocab) {
  * With 64 alternatives each lane of a wave is above the bound: 16384 rows of 750 vectors 93.3, not 96.5, of 1500 129 and 172; with 48 and fewer a wave wins. */
 template <typename T, bool ENT, bool TOP> void launch(ScoreArgs &a, uint64_t all_rows, hipStream_t s) {
     const uint32_t rows = a.rows - a.first, n = vectors_most<T>(a.vocab);
+    const bool large = all_rows * a.vocab * sizeof(T) > kCache; // for a wave with alternatives it does not pay: their vectors are read again (65536 x 4000 132 us, so 147)
 #define ERI_SCORE(TPR, ONCE) \
     do { \
         for (a.shift = 1; n / TPR >> a.shift >= kMarks<TPR> / TPR;) ++a.shift; \
@@ -369,9 +369,12 @@ template <typename T, bool ENT, bool TOP> void launch(ScoreArgs &a, uint64_t all
     if (n > kLong && all_rows <= kFew && a.slices <= kSlicesMost) {
         hipLaunchKernelGGL((score_slice_kernel<T, kSliceThreads, ENT, TOP>), dim3(rows * a.slices), dim3(kSliceThreads), 0, s, a);
         hipLaunchKernelGGL((score_join_kernel<T, ENT, TOP>), dim3(rows), dim3(TOP ? 512 : 64), 0, s, a);
-    } else if (n <= 256 || (all_rows >= 1024 && n <= (TOP && a.top_n <= 48 ? 2048u : 512u))) ERI_SCORE(64, false);
-    else if (n > kLong && all_rows <= 256) ERI_SCORE(1024, false);
-    else if (all_rows * a.vocab * sizeof(T) > kCache) ERI_SCORE(256, true);
+    } else if (n <= 256 || (all_rows >= 1024 && n <= (TOP && a.top_n <= 48 ? 2048u : 512u))) {
+        if constexpr (TOP) ERI_SCORE(64, false);
+        else if (large) ERI_SCORE(64, true);
+        else ERI_SCORE(64, false);
+    } else if (n > kLong && all_rows <= 256) ERI_SCORE(1024, false);
+    else if (large) ERI_SCORE(256, true);
     else ERI_SCORE(256, false);
 #undef ERI_SCORE
 }

@@ -447,6 +447,41 @@ def test_past_32_bit_offsets(losses):
     assert int((x[:16000] != 0).any(1).sum()) == 2
 
 
+@pytest.mark.parametrize("dtype,rows,vocab", [(BF, 140001, 1001), (BF, 70001, 2507), (BF, 36000, 5003), (BF, 1100, 131071), (F32, 70001, 1003), (F32, 33001, 2100),
+                                              (F32, 2100, 33333), (F32, 500, 140003)])
+def test_logits_that_the_caches_do_not_hold(losses, dtype, rows, vocab):
+    """More than 256 MB, in rows of all the lengths that are dealt with differently."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x = (torch.randn(rows, vocab, generator=gen, device="cuda") * 2).to(dtype)
+    assert x.numel() * x.element_size() > 2 ** 28
+    ids = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+    few = torch.randint(0, vocab, (rows, 9), generator=gen, device="cuda")
+    values = torch.log_softmax(torch.randn(rows, 10, generator=gen, device="cuda"), 1)[:, :9].contiguous()
+    g, gh = torch.randn(rows, generator=gen, device="cuda"), torch.randn(rows, generator=gen, device="cuda")
+    parts = [slice(at, at + 3) for at in (0, rows // 2, rows - 3)]
+    for top, entropy in ((0, True), (7, False), (50, True)):
+        r = losses.token_logprobs(x, ids, entropy=entropy, top=top)
+        for s in parts:
+            _check_scores(type(r)(*[None if t is None else t[s] for t in r]), x[s], ids[s], 1.0, top, (top, s))
+    for rest in (False, True):
+        d = losses.distill_top(x, few, values, rest=rest)
+        for s in parts:
+            _check_distill(type(d)(d.loss[s], d.stats[s]), x[s], few[s], values[s], 1.0, rest, s)
+        for out in (BF, F32):
+            dx = losses.distill_top_grad(x, few, values, d.stats, g, dtype=out)
+            for s in parts:
+                _check_distill_grad(dx[s], x[s], few[s], values[s], g[s], 1.0, rest, (out, s))
+    for e in (None, gh):
+        given = dict(grad_entropy=e, entropy=None if e is None else r.entropy)
+        for out in (BF, F32):
+            dx = losses.token_logprobs_grad(x, ids, r.stats, g, dtype=out, **given)
+            for s in parts:
+                _check_token_grad(dx[s], x[s], ids[s], g[s], None if e is None else e[s], 1.0, (out, s))
+    whole = losses.token_logprobs_grad(x, ids, r.stats, g)
+    losses.token_logprobs_grad(x, ids, r.stats, g, out=x)
+    assert torch.equal(x, whole)
+
+
 def _steps(losses, x, near, ids, g):
     r = losses.token_logprobs(x, ids, temperature=1.5, entropy=True, top=12)
     teacher = losses.token_logprobs(near, temperature=1.5, top=12)
