@@ -3,7 +3,8 @@
     python examples/train_tokens.py [--steps 40]
 
 Every step sums two micro-batches: table rows are looked up and scaled (`layers.embedding`), dropped, and go through blocks that
-add a dropped branch to the residual and norm it in one kernel (`layers.rms_norm`).  The table's gradient is kept in float32
+add a dropped branch to the residual and norm it in one kernel (`layers.rms_norm`); the loss is read off the bf16 logits as they are
+(`losses.token_logprobs`, where a target outside the vocabulary counts for nothing).  The table's gradient is kept in float32
 and accumulated over the micro-batches by `layers.embedding_grad`; the others come from autograd.  Both are what
 `Adam8bit` reads as they are.  The text is synthetic: each token follows from the one before it.
 """
@@ -15,7 +16,7 @@ import sys
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
-from eridiffusion_amd import layers  # noqa: E402
+from eridiffusion_amd import layers, losses  # noqa: E402
 from eridiffusion_amd.adam8bit import Adam8bit, Adam8bitConfig  # noqa: E402
 
 VOCAB, DIM, BLOCKS, PAD = 1000, 256, 2, 0
@@ -45,7 +46,7 @@ class Model:
         for i in range(BLOCKS):
             branch = torch.nn.functional.gelu(y @ self.up[i]) @ self.down[i]
             y, h, _, _ = layers.rms_norm(branch, self.norms[i + 1], residual=h, p=self.p, seed=2 + i, offset=step)
-        return torch.nn.functional.cross_entropy((y @ self.head).float().flatten(0, 1), target.flatten())
+        return -losses.token_logprobs(y @ self.head, target).logprob.sum() / (target >= 0).sum()
 
 
 def train(steps=40, batch=16, length=64, micro=2, p=0.1, seed=0, log=print):

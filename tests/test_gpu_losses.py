@@ -664,3 +664,40 @@ def test_the_c_calls_write_nothing_behind_their_outputs():
         L.check(L.lib().eri_token_logprobs_grad(C.byref(f), stream), "eri_token_logprobs_grad")
         _check_token_grad(out[:rows], x, ids, grad, None, 1.0, rows)
         assert bool((ws[size:] == 77).all()) and all(bool((t[rows] == 5).all()) for t in (logprob, entropy, stats, top, places, loss, more, out))
+
+
+def test_the_examples_loss_and_its_gradients_are_those_of_cross_entropy():
+    """The example runs, and its loss, which it reads off bf16 logits, is the mean over the tokens that are asked for."""
+    import importlib.util
+    import os
+
+    from test_losses_host import ROOT
+    spec = importlib.util.spec_from_file_location("train_tokens", os.path.join(ROOT, "examples", "train_tokens.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    torch.manual_seed(3)
+    model = example.Model(0.0)
+    rows = torch.randn(4, 16, example.DIM, device="cuda", dtype=BF).requires_grad_()
+    target = torch.randint(0, example.VOCAB, (4, 16), device="cuda")
+    target[:, -3:] = -100
+    loss = model.loss(rows, target, 0)
+    loss.backward()
+    with torch.no_grad():  # the same model up to its logits, whose gradient is then taken in 64 bits
+        from eridiffusion_amd import layers
+        h = layers.dropout(rows, 0.0, seed=1)
+        y = layers.rms_norm(h, model.norms[0]).y
+        for i in range(example.BLOCKS):
+            branch = torch.nn.functional.gelu(y @ model.up[i]) @ model.down[i]
+            y, h, _, _ = layers.rms_norm(branch, model.norms[i + 1], residual=h)
+        logits = (y @ model.head).double().flatten(0, 1)
+    real = target.flatten() >= 0
+    logp = torch.log_softmax(logits, 1)
+    want = -logp[real, target.flatten()[real]].mean()
+    assert abs(loss.item() - want.item()) < 64 * 2 * U32 * 64 * abs(want.item())  # means of 52 numbers, each a few roundings off
+    p = logp.exp()
+    p[real, target.flatten()[real]] -= 1
+    dz = torch.where(real[:, None], p / real.sum(), 0.0)
+    dw = y.double().flatten(0, 1).t() @ dz
+    # each term's gradient is rounded to bf16, and so is their sum
+    size = y.double().flatten(0, 1).abs().t() @ dz.abs()
+    _near(model.head.grad, dw.cpu(), (U[BF] * dw.abs() + (U[BF] + 100 * U32) * size).cpu())
