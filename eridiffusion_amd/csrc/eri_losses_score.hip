@@ -54,13 +54,15 @@ template <typename T> __device__ __forceinline__ bool token_of(const ScoreArgs &
 /* What the threads of a workgroup tell each other about their elements. */
 template <int TPR> constexpr uint32_t kMarks = TPR > (int)kWave ? 8192 : 1024; // largest values of a few vectors each, over all threads; a wave has shorter rows
 template <int TPR> struct TopSpace {
-    Key lists[TPR];
-    uint32_t found[TPR]; // columns, 64 to a wave
+    union {
+        Key lists[TPR];      // until the bound is known
+        uint32_t found[TPR]; // columns, 64 to a wave
+    };
     Key bound;
     uint32_t places_n;
 };
 template <int TPR> struct Marks {
-    uint16_t values[kMarks<TPR>];
+    uint16_t values[kMarks<TPR>] __attribute__((aligned(16)));
     uint16_t places[kWave * (kMarks<TPR> / TPR)]; // those that reach the bound: only 64 threads have any
 };
 
@@ -87,15 +89,15 @@ template <int TPR, typename T> __device__ __forceinline__ uint32_t first_of(cons
 }
 
 /* The 64 largest of the lists that the waves have, in the first one. */
-template <int TPR> __device__ __forceinline__ void join_lists(Key &k, TopSpace<TPR> &sp) {
+template <int TPR> __device__ __forceinline__ void join_lists(Key &k, Key *lists) {
     const uint32_t t = threadIdx.x, lane = t % kWave, wave = t / kWave;
-    if (TPR > (int)kWave) sp.lists[t] = k;
+    if (TPR > (int)kWave) lists[t] = k;
 #pragma unroll
     for (uint32_t half = TPR / kWave / 2; half > 0; half /= 2) {
         __syncthreads();
         if (wave < half) {
-            merge64(k, sp.lists[(wave + half) * kWave + (kWave - 1 - lane)], lane);
-            if (half > 1) sp.lists[t] = k;
+            merge64(k, lists[(wave + half) * kWave + (kWave - 1 - lane)], lane);
+            if (half > 1) lists[t] = k;
         }
     }
 }
@@ -103,7 +105,7 @@ template <int TPR> __device__ __forceinline__ void join_lists(Key &k, TopSpace<T
 /* The top_n-th largest of the threads' keys, 0 where fewer threads have one. */
 template <int TPR> __device__ __forceinline__ Key bound_of(Key k, uint32_t top_n, TopSpace<TPR> &sp) {
     sort64(k, threadIdx.x % kWave);
-    join_lists<TPR>(k, sp);
+    join_lists<TPR>(k, sp.lists);
     if (threadIdx.x == top_n - 1) sp.bound = k;
     if (threadIdx.x == 0) sp.places_n = 0;
     __syncthreads();
@@ -253,7 +255,7 @@ template <typename T, int TPR, bool ENT, bool TOP, bool ONCE> __global__ __launc
         }
         found.sort();
         k = found.top;
-        join_lists<TPR>(k, sp);
+        join_lists<TPR>(k, reinterpret_cast<Key *>(marks.values)); // which are done with
     }
     if (t < kWave) finish<T, ENT, TOP>(a, index, r, k, x, named, t);
 }
@@ -295,7 +297,8 @@ template <typename T, int TPR, bool ENT, bool TOP> __global__ __launch_bounds__(
         found.take(v, own >= bound && own != 0, [&](uint32_t i) { return first + i * TPR + t; });
         found.sort();
         k = found.top;
-        join_lists<TPR>(k, sp);
+        __shared__ Key lists[TPR];
+        join_lists<TPR>(k, lists);
     }
     if (t == 0) a.parts[blockIdx.x] = r;
     if (TOP && t < a.top_n) a.part_keys[(uint64_t)blockIdx.x * a.top_n + t] = k;
