@@ -15,7 +15,7 @@ constexpr float kLowest = -3.40282347e38f; // the running maximum before the fir
 constexpr float kFloor = -1e28f;           // below any distance that counts: 0 * kFloor is 0 where 0 * -infinity would be NaN, and 2^31 of them are finite
 /* Rows of more than kLong vectors are cut where there are no more than kFew of them. */
 constexpr uint32_t kLong = 8192, kFew = 64, kSlicesMost = 64;
-constexpr uint64_t kCache = 256u << 20;        // bytes of the last cache
+constexpr uint64_t kCache = 128u << 20;        // bytes, half of the last cache: the gradient wants room there too
 constexpr double kLog2e = 1.4426950408889634074;
 constexpr float kLn2 = 0.693147181f;
 
@@ -77,8 +77,9 @@ template <bool ONCE, typename T> __device__ __forceinline__ u32x4 load_any(const
 /* Vectors first .. end-1 of a row, dealt to TPR threads in turn, four of each at a time: all loads of a batch are under way before the first is
  * wanted.  `use(values, at, full)` gets an array of C vectors, those that begin at vector at + k TPR + t; unless `full`, some of them may not be whole
  * ones.  The row's end is one smaller batch: vector by vector it took a trip to memory for each.
- * ONCE: the loads pass the caches by, which pays where the logits are more than the last cache holds (kCache): read at 6.3-6.9 TB/s in place of
- * 5.6-5.9, but 82 MB in 29 us in place of 25. */
+ * ONCE: the loads pass the caches by, which pays where the logits are more than half of the last cache (kCache): read at 6.3-6.9 TB/s in place of
+ * 5.6-5.9.  us for scores and gradient right behind what wrote the logits, not so and so: 41 MB 23 and 26, 131 MB 77 and 70, 150 MB 72 and 75, 164 MB 76 and
+ * 68, 250 MB 134 and 124. */
 template <int TPR, bool ONCE, int C, bool FULL, typename T, typename Use> __device__ __forceinline__ void walk_batch(const Row<T> &row, uint32_t at, uint32_t end, uint32_t t, Use &use) {
     u32x4 raw[C];
     float v[C][kEach<T>];

@@ -167,7 +167,7 @@ template <typename T, typename O, int TPR, Past PAST> __global__ __launch_bounds
 
 constexpr uint32_t kBlocks = 1u << 23; // of a launch
 
-/* Cuts rows into slices; whether the logits are more than the last cache holds.  A small part of a row to each workgroup keeps the chip within one
+/* Cuts rows into slices; whether the logits are more than half of the last cache.  A small part of a row to each workgroup keeps the chip within one
  * window of the memory, and what is stored, and for float32 scores what is read too, passes the caches by.  us with 2048, 1024 and 512
  * vectors to a workgroup, both past the caches, and (the stores alone):
  *     scores        8192 x 128000 bf16     768 (785)  758 (749)  726 (892)      distillation  776 (793)  771 (796)  671 (668)
