@@ -7,6 +7,7 @@ threads' sums in at most 24 additions: with at most vocab / 2048 + 8 batches the
 A result is rounded once to its type, u |result| or 2^-8 |result|."""
 import ctypes as C
 import math
+import random
 
 import pytest
 import torch
@@ -482,6 +483,70 @@ def test_logits_that_the_caches_do_not_hold(losses, dtype, rows, vocab):
     assert torch.equal(x, whole)
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_any_sizes_and_places(losses, seed):
+    """Rows of any length that begin anywhere, all calls on one batch."""
+    rng = random.Random(seed)
+    dtype, out = rng.choice([BF, F32]), rng.choice([BF, F32])
+    vocab = round(math.exp(rng.uniform(math.log(1), math.log(90000))))
+    rows = max(1, min(round(math.exp(rng.uniform(0, math.log(3000)))), 6000000 // vocab))
+    gap, at, t, rest = rng.choice([0, 1, 7, 64]), rng.choice([0, 1, 2, 5, 8, 33]), rng.choice([1.0, 0.6, 2.5]), rng.random() < 0.5
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    flat = (torch.randn(rows * (vocab + gap) + at, generator=gen, device="cuda") * 3).to(dtype)
+    flat[torch.rand(flat.shape, generator=gen, device="cuda") < rng.choice([0.0, 0.4, 0.95])] = -INF
+    x = flat[at:].as_strided((rows, vocab), (vocab + gap, 1))
+    ids = torch.randint(-1, vocab + 1, (rows,), generator=gen, device="cuda")
+    top, k = rng.randint(0, min(64, vocab)), rng.randint(1, 64)
+    r = losses.token_logprobs(x, ids, temperature=t, entropy=True, top=top)
+    _check_scores(r, x, ids, t, top)
+    ids[(r.logprob == -INF)] = -100
+    g, gh = torch.randn(rows, generator=gen, device="cuda"), torch.randn(rows, generator=gen, device="cuda")
+    _check_token_grad(losses.token_logprobs_grad(x, ids, r.stats, g, grad_entropy=gh, entropy=r.entropy, temperature=t, dtype=out), x, ids, g, gh, t)
+    few = torch.randint(-1, vocab + 1, (rows, k), generator=gen, device="cuda")  # some of them twice
+    teacher = (torch.log_softmax(torch.randn(rows, k + 1, generator=gen, device="cuda") * 2, 1)[:, :k]).to(rng.choice([BF, F32]))
+    d = losses.distill_top(x, few, teacher, temperature=t, rest=rest)
+    _check_distill(d, x, few, teacher, t, rest)
+    _check_distill_grad(losses.distill_top_grad(x, few, teacher, d.stats, g, temperature=t, dtype=out), x, few, teacher, g, t, rest)
+
+
+def test_the_longest_row(losses):
+    """2^31 - 1 columns: places that just fit.  Equal logits but for a few: the sums of powers of two are exact."""
+    vocab = 2 ** 31 - 1
+    x = torch.full((1, vocab), -5.0, dtype=BF, device="cuda")
+    peaks = {0: 3.0, 7: 2.0, 2 ** 20 + 3: 2.0, 2 ** 30: 4.0, vocab - 2: 2.0, vocab - 1: 5.0}
+    for col, v in peaks.items():
+        x[0, col] = v
+    order = [vocab - 1, 2 ** 30, 0, 7, 2 ** 20 + 3, vocab - 2, 1, 2]
+    total = sum(math.exp(v + 5.0) for v in peaks.values()) + vocab - len(peaks)  # in units of a peak-less token
+    r = losses.token_logprobs(x, torch.tensor([vocab - 1], device="cuda"), entropy=True, top=8)
+    assert r.top_ids[0].tolist() == order
+    lp = lambda v: v + 5.0 - math.log(total)  # noqa: E731
+    want = [lp(peaks.get(c, -5.0)) for c in order]
+    # 2^31 terms: a thread's 2^21 are added 32 at a time, half a unit lost each time at most
+    near = 2 ** 16 * U32 + 64 * U32
+    assert all(abs(a - b) < near for a, b in zip(r.top[0].tolist(), want)) and abs(r.logprob.item() - lp(5.0)) < near
+    entropy = -sum(math.exp(lp(v)) * lp(v) for v in peaks.values()) - (vocab - len(peaks)) * math.exp(lp(-5.0)) * lp(-5.0)
+    assert abs(r.entropy.item() - entropy) < 30 * near
+    few, q = torch.tensor([[vocab - 1, 0, 2 ** 30]], device="cuda"), torch.tensor([[0.5, 0.25, 0.125]], device="cuda").log()
+    d = losses.distill_top(x, few, q, rest=True)
+    p = [math.exp(lp(v)) for v in (5.0, 3.0, 4.0)]
+    loss = sum(w * (math.log(w) - math.log(v)) for w, v in zip((0.5, 0.25, 0.125), p)) + 0.125 * (math.log(0.125) - math.log1p(-sum(p)))
+    assert abs(d.loss.item() - loss) < 4 * near
+    cols = torch.tensor([0, 1, 7, 2 ** 20 + 3, 2 ** 30, 2 ** 30 + 1, vocab - 2, vocab - 1], device="cuda")
+    one = torch.ones(1, device="cuda")
+    dx = losses.distill_top_grad(x, few, q, d.stats, one)[0, cols].tolist()
+    others = (1 - sum(p) - 0.125) / (1 - sum(p))
+    named = dict(zip(few[0].tolist(), zip(p, (0.5, 0.25, 0.125))))
+    for col, got in zip(cols.tolist(), dx):
+        pj = math.exp(lp(peaks.get(col, -5.0)))
+        exact = named[col][0] - named[col][1] if col in named else pj * others
+        assert abs(got - exact) < abs(exact) * (U[BF] + 8 * near), col
+    losses.token_logprobs_grad(x, torch.tensor([vocab - 1], device="cuda"), r.stats, one, out=x)
+    for col, got in zip(cols.tolist(), x[0, cols].tolist()):
+        exact = (1.0 if col == vocab - 1 else 0.0) - math.exp(lp(peaks.get(col, -5.0)))
+        assert abs(got - exact) < abs(exact) * (U[BF] + 8 * near), col
+
+
 def _steps(losses, x, near, ids, g):
     r = losses.token_logprobs(x, ids, temperature=1.5, entropy=True, top=12)
     teacher = losses.token_logprobs(near, temperature=1.5, top=12)
@@ -554,6 +619,53 @@ def test_autograd_is_the_backward_call(losses, rows, vocab):
         x.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         d.loss.sum().backward()
+
+
+@pytest.mark.parametrize("rows,vocab", [(3, 70001), (300, 2500)])
+def test_a_captured_autograd_pass_replays(losses, rows, vocab):
+    x, ids = _logits(rows, vocab, BF).cuda().requires_grad_(), _ids(rows, vocab).cuda()
+    few, values = (t.cuda() for t in _teacher(rows, vocab, 7))
+    g, gh = _gen(rows).cuda(), _gen(rows, seed=1).cuda()
+
+    def step():
+        r = losses.token_logprobs(x, ids, entropy=True)
+        d = losses.distill_top(x, few, values, rest=True)
+        return torch.autograd.grad([r.logprob, r.entropy, d.loss], [x], [g, gh, g])[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            got = step()
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(x.roll(1, 1))
+        g.mul_(1.5)
+        ids.copy_(ids.roll(1))
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = got.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(kept, step()), k
+
+
+def test_two_streams_at_once(losses):
+    """Each call has a workspace of its own."""
+    inputs = [(_logits(5, 90001, F32, seed=i).cuda(), _ids(5, 90001, i).cuda()) for i in range(2)]
+    few, values = (t.cuda() for t in _teacher(5, 90001, 11))
+    want = [(losses.token_logprobs(x, ids, entropy=True, top=30), losses.distill_top(x, few, values, rest=True)) for x, ids in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((losses.token_logprobs(*inputs[i], entropy=True, top=30), losses.distill_top(inputs[i][0], few, values, rest=True)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for pair in got[i]:
+            assert all(torch.equal(a, b) for one, other in zip(pair, want[i]) for a, b in zip(one, other))
 
 
 def test_autograd_against_differences(losses):
