@@ -3,7 +3,8 @@
  *
  *     scores        (g ([j = id] - p) - h p (ln p + H)) / T = p (u + w log2 p) + [j = id] g / T,  u = -(g + h H) / T,  w = -h ln 2 / T
  *     distillation  p_j / p_r (p_r - q_r) g / T for the tokens that the teacher does not name, (p_j - q_j) g / T for those it names, which each workgroup
- *                   marks in LDS before it begins
+ *                   marks in LDS before it begins: which elements of a vector, and by which entry, so that a token costs two looks at LDS and not one
+ *                   at every entry (1025 x 10007 f32 with 64 tokens 25.1 us, so 17.1)
  * with log2 p = (x - m) log2(e) / T - log2 s in one fused product: one exponential an element, which is a quarter of the arithmetic.
  */
 #include "eri_losses_device.h"
@@ -115,8 +116,9 @@ constexpr uint32_t kDistillMost = 4096; // vectors of a row or slice
 template <typename T, typename O, int TPR, Past PAST> __global__ __launch_bounds__(TPR) void distill_grad_kernel(const GradArgs a) {
     constexpr uint32_t MOST = TPR > (int)kWave ? kDistillMost : kDistillMost / 4;
     __shared__ uint32_t named[MOST / 4]; // a byte for each vector: which of its elements the teacher names
-    __shared__ uint32_t places[kWave] __attribute__((aligned(16)));
-    __shared__ float shares[kWave] __attribute__((aligned(16)));
+    __shared__ uint8_t entries[MOST];    // and one of the entries that name it
+    __shared__ uint32_t places[kWave];
+    __shared__ float shares[kWave]; // of a token: all its entries
     const uint32_t t = threadIdx.x, slice = blockIdx.x % a.slices;
     const uint64_t index = a.first + blockIdx.x / a.slices;
     const Row<T> row((const T *)a.logits + index * a.stride, a.vocab);
@@ -136,9 +138,17 @@ template <typename T, typename O, int TPR, Past PAST> __global__ __launch_bounds
     const bool here = id >= 0 && id < (int64_t)a.vocab && place / kEach<T> >= first && place / kEach<T> < end;
     __syncthreads();
     if (t < kWave) {
-        if (here) atomicOr(&named[vec / 4], 1u << (vec % 4 * 8 + place % kEach<T>));
-        places[t] = here ? place : ~0u;
-        shares[t] = here && norm != -kInf ? exp2_of((q - norm) * (float)kLog2e) : 0.0f;
+        q = here && norm != -kInf ? exp2_of((q - norm) * (float)kLog2e) : 0.0f;
+        const uint32_t mine = here ? place : ~0u, bit = 1u << (vec % 4 * 8 + place % kEach<T>);
+        float share = q;
+        if (__ballot(here && (atomicOr(&named[vec / 4], bit) & bit)) != 0) { // a token twice
+            share = 0.0f;
+            for (uint32_t j = 0; j < a.k; ++j)
+                if ((uint32_t)__builtin_amdgcn_readlane((int)mine, (int)j) == mine) share += lane_of(q, (int)j);
+        }
+        if (here) entries[vec] = (uint8_t)t;
+        places[t] = mine;
+        shares[t] = share;
     }
     __syncthreads();
     each<TPR, PAST>(row, out, first, end, t, [&](float(&v)[kEach<T>], uint32_t from) {
@@ -148,15 +158,14 @@ template <typename T, typename O, int TPR, Past PAST> __global__ __launch_bounds
         uint32_t which = from / kEach<T> < end ? ((const uint8_t *)named)[from / kEach<T> - first] : 0;
         for (; which != 0; which &= which - 1) {
             const uint32_t e = (uint32_t)__builtin_ctz(which);
-            float x = v[0], sum = 0.0f; // over the entries of this token
-            for (uint32_t j = 0; j < a.k; j += 4) {
-                const u32x4 p = *(const u32x4 *)&places[j], q4 = *(const u32x4 *)&shares[j];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) sum += p[i] == from + e ? as_float(q4[i]) : 0.0f;
-            }
+            uint32_t j = entries[from / kEach<T> - first];
+            if (places[j] != from + e) // the vector holds another token of the teacher's too
+                for (j = 0; j + 1 < kWave && places[j] != from + e;) ++j;
+            const float share = shares[j];
+            float x = v[0];
 #pragma unroll
             for (uint32_t i = 1; i < kEach<T>; ++i) x = i == e ? v[i] : x;
-            const float value = ((norm == -kInf ? 0.0f : exp2_of(log2p(x))) - sum) * g;
+            const float value = ((norm == -kInf ? 0.0f : exp2_of(log2p(x))) - share) * g;
 #pragma unroll
             for (uint32_t i = 0; i < kEach<T>; ++i) r[i] = i == e ? value : r[i];
         }
@@ -170,10 +179,11 @@ constexpr uint32_t kBlocks = 1u << 23; // of a launch
 /* Cuts rows into slices; whether the logits are more than half of the last cache.  A small part of a row to each workgroup keeps the chip within one
  * window of the memory, and what is stored, and for float32 scores what is read too, passes the caches by.  us with 2048, 1024 and 512
  * vectors to a workgroup, both past the caches, and (the stores alone):
- *     scores        8192 x 128000 bf16     768 (785)  758 (749)  726 (892)      distillation  776 (793)  771 (796)  671 (668)
- *                  16384 x 32000           371 (383)  370 (330)  358 (425)                    391 (400)  390 (399)  390 (400)
- *                  16384 x 50257           624 (628)  538 (510)  599 (659)                    603 (610)  553 (592)  552 (510)
- *                   4096 x 128000 f32      763 (784)  708 (776)  684 (700)                    765 (785)  772 (797)  662 (643)
+ *     scores        8192 x 128000 bf16     768 (785)  758 (749)  726 (892)      distillation  (775)      665 (647)  782 (899)
+ *                  16384 x 32000           371 (383)  370 (330)  358 (425)                    (380)          (345)      (487)
+ *                  16384 x 50257           624 (628)  538 (510)  599 (659)                    (646)          (545)      (778)
+ *                   4096 x 128000 f32      763 (784)  708 (776)  684 (700)                752 (770)      697 (729)  760 (828)
+ *                  16384 x 32000 f32                                                      758            700 (655)  815 (897)
  * before, with a row to a workgroup and all of it through the caches, 8192 x 128000 took 817 and 842.  A float32 gradient of bf16 logits, whose
  * 16-byte stores leave gaps for one another, takes 522 through the caches and 599 past them. */
 template <typename T, typename O> bool cut(GradArgs &a, uint64_t rows, uint32_t per, uint32_t per_large) {
@@ -220,7 +230,7 @@ template <typename T, typename O> int token_grad(GradArgs &a, uint64_t rows, hip
 template <typename T, typename O> int distill_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
 #define ERI_GRAD(TPR, PAST) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR, PAST>), dim3(n), dim3(TPR), 0, s, a); })
     // looking up the teacher's tokens costs each workgroup something: longer slices, unless the rows are few
-    const bool large = cut<T, O>(a, rows, rows >= 1024 && vectors_most<T>(a.vocab) <= kDistillMost ? kDistillMost : kBatch * 256, 512);
+    const bool large = cut<T, O>(a, rows, rows >= 1024 && vectors_most<T>(a.vocab) <= kDistillMost ? kDistillMost : kBatch * 256, kBatch * 256);
     if (by_waves<T>(a.vocab, rows, large ? 0 : kDistillMost / 4)) { // 65536 x 8000 bf16 340 us, in waves 417
         a.per = vectors_most<T>(a.vocab), a.slices = 1;
         return large ? ERI_GRAD(64, kStores) : ERI_GRAD(64, kNothing);
