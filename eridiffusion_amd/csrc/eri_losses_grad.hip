@@ -209,7 +209,7 @@ template <typename F> int in_parts(GradArgs &a, uint64_t rows, uint32_t rows_of_
 }
 
 /* Whether a wave has a row: short ones, and longer ones where there are many: 16384 x 3000 bf16 35 us for 51, and 44 for 61 (scores, distillation), 6000 75
- * for 77, and 100 for 93; 200 x 6000 5.1 for 7.1. */
+ * for 77, and 80 for 90; 200 x 6000 5.1 for 7.1. */
 template <typename T> bool by_waves(uint64_t vocab, uint64_t rows, uint32_t many) {
     const uint32_t n = vectors_most<T>(vocab);
     return n <= 256 || (rows >= 1024 && n <= many);
@@ -231,7 +231,7 @@ template <typename T, typename O> int distill_grad(GradArgs &a, uint64_t rows, h
 #define ERI_GRAD(TPR, PAST) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR, PAST>), dim3(n), dim3(TPR), 0, s, a); })
     // looking up the teacher's tokens costs each workgroup something: longer slices, unless the rows are few
     const bool large = cut<T, O>(a, rows, rows >= 1024 && vectors_most<T>(a.vocab) <= kDistillMost ? kDistillMost : kBatch * 256, kBatch * 256);
-    if (by_waves<T>(a.vocab, rows, large ? 0 : kDistillMost / 4)) { // 65536 x 8000 bf16 340 us, in waves 417
+    if (by_waves<T>(a.vocab, rows, large ? kDistillMost * 3 / 16 : kDistillMost / 4)) { // large ones, 64 tokens: 65536 x 4000 bf16 202 us for 309, x 6000 300 for 343, but x 8000 412 for 379
         a.per = vectors_most<T>(a.vocab), a.slices = 1;
         return large ? ERI_GRAD(64, kStores) : ERI_GRAD(64, kNothing);
     }

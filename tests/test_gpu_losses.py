@@ -448,8 +448,8 @@ def test_past_32_bit_offsets(losses):
     assert int((x[:16000] != 0).any(1).sum()) == 2
 
 
-@pytest.mark.parametrize("dtype,rows,vocab", [(BF, 140001, 1001), (BF, 70001, 2507), (BF, 36000, 5003), (BF, 1100, 131071), (F32, 70001, 1003), (F32, 33001, 2100),
-                                              (F32, 2100, 33333), (F32, 500, 140003)])
+@pytest.mark.parametrize("dtype,rows,vocab", [(BF, 140001, 1001), (BF, 70001, 2507), (BF, 36000, 5003), (BF, 20001, 7003), (BF, 1100, 131071), (F32, 70001, 1003),
+                                              (F32, 33001, 2100), (F32, 2100, 33333), (F32, 500, 140003)])
 def test_logits_that_the_caches_do_not_hold(losses, dtype, rows, vocab):
     """More than 256 MB, in rows of all the lengths that are dealt with differently."""
     gen = torch.Generator(device="cuda").manual_seed(rows)
