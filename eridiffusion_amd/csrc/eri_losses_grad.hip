@@ -214,27 +214,43 @@ template <typename T> bool by_waves(uint64_t vocab, uint64_t rows, uint32_t many
     const uint32_t n = vectors_most<T>(vocab);
     return n <= 256 || (rows >= 1024 && n <= many);
 }
+
+/* LDS to ask for beyond what a workgroup of 256 uses, so that no more than `groups` of them fit a unit's 160 KB.  Fewer rows' pieces under way at once
+ * leave the memory's channels less to jump between, where rows are long and begin together on 128 bytes.  us with 8, 4 and 3 workgroups to a unit:
+ *     scores, bf16, entropy    8192 x 128000  742  700  831    4096 x 230400  680  615  666    8192 x 115200  604  619  687    16384 x 50257  517  550  628
+ *     scores, bf16             8192 x 128000  757  756  678    4096 x 230400  686  682  597    8192 x 115200  630  630  601    16384 x 50257  512  513  559
+ *     scores, f32              4096 x 128000  660  634  730    8192 x 50257   510  507  568    4096 x 65536   331  321  362
+ *     distillation, f32        4096 x 128000  700       627    8192 x 50257   483       508    4096 x 65536   320       325
+ * bf16 rows of 128001 take 753, 795 and 841, and the distillation of bf16 653 and, with 3, 708. */
+constexpr uint32_t room_for(uint32_t groups, uint32_t used = 0) { return 160 * 1024 / (groups + 1) + 512 - used; }
+template <typename T> bool long_and_even(const GradArgs &a) {
+    return a.vocab >= 120 * 1024 && ((uintptr_t)a.logits | a.stride * sizeof(T)) % 128 == 0;
+}
 template <typename T, typename O> int token_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
-#define ERI_GRAD(TPR, ENT, PAST) in_parts(a, rows, 256 / TPR, [&](uint32_t n) { hipLaunchKernelGGL((token_grad_kernel<T, O, TPR, ENT, PAST>), dim3(n), dim3(256), 0, s, a); })
+#define ERI_GRAD(TPR, ENT, PAST) in_parts(a, rows, 256 / TPR, [&](uint32_t n) { hipLaunchKernelGGL((token_grad_kernel<T, O, TPR, ENT, PAST>), dim3(n), dim3(256), lds, s, a); })
     constexpr bool kWide = sizeof(T) == 4;
+    uint32_t lds = 0;
     const bool large = cut<T, O>(a, rows, kBatch * 256, kWide ? 512 : kBatch * 256);
     if (by_waves<T>(a.vocab, rows, 512)) {
         a.per = vectors_most<T>(a.vocab), a.slices = 1;
         if (large) return a.grad_entropy ? ERI_GRAD(64, true, kStores) : ERI_GRAD(64, false, kStores);
         return a.grad_entropy ? ERI_GRAD(64, true, kNothing) : ERI_GRAD(64, false, kNothing);
     }
+    if (large && (kWide || long_and_even<T>(a))) lds = room_for(kWide || a.grad_entropy ? 4 : 3);
     if (!large) return a.grad_entropy ? ERI_GRAD(256, true, kNothing) : ERI_GRAD(256, false, kNothing);
     return a.grad_entropy ? ERI_GRAD(256, true, (kWide ? kBoth : kStores)) : ERI_GRAD(256, false, (kWide ? kBoth : kStores));
 #undef ERI_GRAD
 }
 template <typename T, typename O> int distill_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
-#define ERI_GRAD(TPR, PAST) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR, PAST>), dim3(n), dim3(TPR), 0, s, a); })
+#define ERI_GRAD(TPR, PAST) in_parts(a, rows, 1, [&](uint32_t n) { hipLaunchKernelGGL((distill_grad_kernel<T, O, TPR, PAST>), dim3(n), dim3(TPR), lds, s, a); })
+    uint32_t lds = 0;
     // looking up the teacher's tokens costs each workgroup something: longer slices, unless the rows are few
     const bool large = cut<T, O>(a, rows, rows >= 1024 && vectors_most<T>(a.vocab) <= kDistillMost ? kDistillMost : kBatch * 256, kBatch * 256);
     if (by_waves<T>(a.vocab, rows, large ? kDistillMost * 3 / 16 : kDistillMost / 4)) { // large ones, 64 tokens: 65536 x 4000 bf16 202 us for 309, x 6000 300 for 343, but x 8000 412 for 379
         a.per = vectors_most<T>(a.vocab), a.slices = 1;
         return large ? ERI_GRAD(64, kStores) : ERI_GRAD(64, kNothing);
     }
+    if (large && sizeof(T) == 4 && long_and_even<T>(a)) lds = room_for(3, kDistillMost * 2);
     return large ? ERI_GRAD(256, kStores) : ERI_GRAD(256, kNothing);
 #undef ERI_GRAD
 }
