@@ -69,6 +69,10 @@ template <int TPR, bool ONCE, typename T, typename O> __device__ __forceinline__
     for (uint32_t vec = first + t; vec < end; vec += TPR) store_any<ONCE>(out, row, vec, end, v);
 }
 
+/* Below any log2 p whose p is not 0: it keeps 0 * minus infinity out of p log2 p.  w kLeast is finite for all w below 2^120, where kFloor, which is for differences
+ * of logits, made infinity of it, and NaN of a masked element, from |grad_entropy| / T of 4.9e10 on. */
+constexpr float kLeast = -256.0f;
+
 /* log2 p of an element, from {m, ln s}: nothing is left of a row where ln s is minus infinity. */
 struct LogP {
     float m, log2_s, c;
@@ -101,7 +105,7 @@ template <typename T, typename O, int TPR, bool ENT, Past PAST> __global__ __lau
 #pragma unroll
         for (uint32_t e = 0; e < kEach<T>; ++e) {
             const float l = log2p(v[e]), p = exp2_of(l);
-            v[e] = p * (ENT ? fmaf(w, fmaxf(l, kFloor), u) : u);
+            v[e] = p * (ENT ? fmaf(w, fmaxf(l, kLeast), u) : u);
         }
         const uint32_t there = named - place;
         if (there < kEach<T>)
