@@ -87,7 +87,7 @@ def distill_top(logits, ids, teacher, temperature=1.0, rest=False):
     lp = logp.gather(-1, at)
     terms = torch.where(q == 0, 0.0, q * (value - divisor[..., None] - lp))
     held = torch.where(named, p, 0.0).sum(-1)
-    qr = torch.where(apart, (1 - q.sum(-1)).clamp(min=0.0), 0.0)
+    qr = torch.where(apart & ~(norm > 0), (1 - q.sum(-1)).clamp(min=0.0), 0.0)  # none where q is divided by its sum, whatever that rounds to
     log_r = (m_o - m) / t + log_o - log_s
     log_r = torch.where(held < 0.5, torch.log1p(-held.clamp(max=0.5)), log_r)
     loss = terms.sum(-1) + torch.where(apart & (qr != 0), qr * (qr.log() - log_r), 0.0)

@@ -8,7 +8,7 @@ import torch
 
 import test_gpu_losses as tl
 from oracle import losses_f64 as of
-from test_gpu_layers import BF, F32
+from test_gpu_layers import BF, F32, U, U32, _near
 from test_gpu_losses import losses  # noqa: F401
 
 INF = math.inf
@@ -34,3 +34,80 @@ def test_entropy_gradients_of_any_size_leave_masked_logits_at_zero(losses, dtype
         got = losses.token_logprobs_grad(x.cuda(), ids.cuda(), stats.cuda(), g.cuda(), grad_entropy=gh.cuda(), entropy=entropy.cuda(), temperature=temperature, dtype=out)
         assert bool((got.cpu()[masked] == 0).all())
         tl._check_token_grad(got, x, ids, g, gh, temperature, out)
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# what little the student leaves to the rest
+# ---------------------------------------------------------------------------------------------------------------
+
+def _small_rest(rows, vocab, dtype, lift, over):
+    """Students whose named tokens stand `lift` above the others, and a teacher that leaves the rest nothing (its values come to more
+    than one) or next to nothing (to one, but for roundings)."""
+    gen = torch.Generator().manual_seed(vocab + int(lift))
+    x = torch.randn(rows, vocab, generator=gen)
+    ids = torch.stack([torch.randperm(vocab, generator=gen)[:6] for _ in range(rows)])
+    x.scatter_add_(1, ids, torch.full((rows, 6), lift))
+    teacher = torch.randn(rows, 6, generator=gen)
+    return x.to(dtype), ids, torch.log_softmax(teacher, 1) + (0.5 if over else 0.0)
+
+
+def _check_small_rest(over, dx, x, ids, teacher, grad, temperature):
+    """stats[5] = pr - qr, and the gradient of the tokens that are not named, whose every factor has it.
+
+    pr is exp of a difference of maxima, over T, and two sums' logs, in 64 bits from 32-bit parts: relative to itself it is off by what the two sums
+    are, by the rounding of 1 / T times that difference, and by what the named tokens' sum takes in of the others', together at most
+    4 u far + 8 u.  qr is one minus six doubles.  Both are rounded together.  A token's share of the rest is off as any p is."""
+    t, g = of.t32(temperature), grad.double()[:, None]
+    _, stats, dz, _, _ = of.distill_top(x, ids, teacher, temperature, True)
+    m, log_s, whole, _ = of.softmax(x, temperature)
+    named = torch.zeros(x.shape, dtype=torch.bool).scatter_(1, ids, True)
+    others = x.double().masked_fill(named, -INF)
+    m_o, log_o, part, _ = of.softmax(others, temperature)
+    far = (m - m_o) / t
+    pr = (log_o - log_s - far).exp()
+    assert bool((torch.where(named, whole, 0.0).sum(1) >= 0.5).all())
+    want = stats[:, 5]
+    qr = (1 - teacher.double().exp().sum(1)).clamp(min=0.0)
+    rel = tl._sum_off(x, whole, m, t) + tl._sum_off(others, part, m_o, t) + U32 * (4 * far + 8)
+    off = pr * rel + torch.where(qr > 0, 1e-14, 0.0) + U32 * want.abs()
+    _near(over, want, off)
+    rel_j = U32 * (4 * tl._distance(others, m_o, t) + 4 * log_o.abs()[:, None] + 10)
+    size = part * g.abs() / t
+    bound = size * (want.abs()[:, None] * (rel_j + 3 * U32) + off[:, None]) + U[dx.dtype] * (dz * g).abs() + 2.0 ** -120
+    rest = ~named
+    _near(dx.cpu()[rest], (dz * g)[rest], bound[rest])
+
+
+SMALL = [(lift, over, t) for lift in (20.0, 35.0, 52.0) for over in (True, False) for t in (1.0, 1.3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("rows,vocab", [(7, 90), (5, 5003), (2, 70001), (1050, 1501)])
+@pytest.mark.parametrize("lift,over,temperature", SMALL)
+def test_a_small_rest_keeps_its_digits(losses, dtype, rows, vocab, lift, over, temperature):  # noqa: F811
+    x, ids, teacher = _small_rest(rows, vocab, dtype, lift, over)
+    got = losses.distill_top(x.cuda(), ids.cuda(), teacher.cuda(), temperature=temperature, rest=True)
+    g = tl._gen(rows)
+    for out in (BF, F32):
+        dx = losses.distill_top_grad(x.cuda(), ids.cuda(), teacher.cuda(), got.stats, g.cuda(), temperature=temperature, dtype=out)
+        _check_small_rest(got.stats[:, 5], dx, x, ids, teacher, g, temperature)
+        tl._check_distill_grad(dx, x, ids, teacher, g, temperature, True, out)
+
+
+@pytest.mark.parametrize("lift,pr", [(20.0, 1e-5), (52.0, 1e-19)])
+def test_the_check_of_a_small_rest_refuses_one_minus_the_rest(lift, pr):
+    """The oracle's own values pass; what one minus the named tokens' share in 32 bits leaves does not."""
+    x, ids, teacher = _small_rest(7, 90, F32, lift, True)
+    g = tl._gen(7)
+    _, stats, dz, _, _ = of.distill_top(x, ids, teacher, 1.0, True)
+    dx = (dz * g.double()[:, None]).float()
+    assert bool((stats[:, 5] < pr).all())
+    _check_small_rest(stats[:, 5].float(), dx, x, ids, teacher, g, 1.0)
+    p = torch.softmax(x, 1)
+    wrong = 1 - p.gather(1, ids).sum(1)
+    with pytest.raises(AssertionError):
+        _check_small_rest(wrong, dx, x, ids, teacher, g, 1.0)
+    factor = 1 + 1e-3
+    with pytest.raises(AssertionError):
+        _check_small_rest(stats[:, 5].float(), dx * factor, x, ids, teacher, g, 1.0)
