@@ -40,7 +40,7 @@ def token_logprobs(logits: Tensor, ids: Optional[Tensor] = None, *, temperature:
     """Log probabilities of the tokens `ids` (int32 or int64, one for each row) under softmax(logits / temperature).
 
     entropy: that of each row too.  top: the log probabilities and ids of that many largest logits, up to 64.  `logprob` and
-    `entropy` are differentiable; cross entropy is the mean of -logprob."""
+    `entropy` are differentiable; cross entropy is the sum of -logprob over the number of ids that name a token."""
     got = _losses_face.token_logprobs(logits, ids, temperature, entropy, top)
     if got is not None:
         return TokenLogprobs._make(got)

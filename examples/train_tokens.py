@@ -46,7 +46,8 @@ class Model:
         for i in range(BLOCKS):
             branch = torch.nn.functional.gelu(y @ self.up[i]) @ self.down[i]
             y, h, _, _ = layers.rms_norm(branch, self.norms[i + 1], residual=h, p=self.p, seed=2 + i, offset=step)
-        return -losses.token_logprobs(y @ self.head, target).logprob.sum() / (target >= 0).sum()
+        asked = (target >= 0) & (target < VOCAB)  # the others have log probability 0, and are not counted either
+        return -losses.token_logprobs(y @ self.head, target).logprob.sum() / asked.sum()
 
 
 def train(steps=40, batch=16, length=64, micro=2, p=0.1, seed=0, log=print):

@@ -1,7 +1,9 @@
 """The losses where their numbers leave the usual range, and the launches that only certain layouts reach, against the 64-bit oracle.
 
 The bounds are those of test_gpu_losses.py unless a test says otherwise."""
+import importlib.util
 import math
+import os
 
 import pytest
 import torch
@@ -10,6 +12,7 @@ import test_gpu_losses as tl
 from oracle import losses_f64 as of
 from test_gpu_layers import BF, F32, U, U32, _near
 from test_gpu_losses import losses  # noqa: F401
+from test_losses_host import ROOT
 
 INF = math.inf
 
@@ -111,3 +114,22 @@ def test_the_check_of_a_small_rest_refuses_one_minus_the_rest(lift, pr):
     factor = 1 + 1e-3
     with pytest.raises(AssertionError):
         _check_small_rest(stats[:, 5].float(), dx * factor, x, ids, teacher, g, 1.0)
+
+
+@pytest.mark.gpu
+def test_the_examples_mean_is_over_the_targets_that_name_a_token():
+    """A target past the vocabulary counts for nothing, as a negative one: neither in the sum nor in what it is divided by."""
+    spec = importlib.util.spec_from_file_location("train_tokens", os.path.join(ROOT, "examples", "train_tokens.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    torch.manual_seed(4)
+    model = example.Model(0.0)
+    target = torch.randint(0, example.VOCAB, (4, 16), device="cuda")
+    target[:, -3:] = -100
+    got = []
+    for other in (-100, example.VOCAB, example.VOCAB + 77):
+        rows = torch.randn(4, 16, example.DIM, device="cuda", dtype=BF, generator=torch.Generator(device="cuda").manual_seed(5)).requires_grad_()
+        target[:, :5] = other
+        loss = model.loss(rows, target, 0)
+        got.append((loss.detach(), torch.autograd.grad(loss, rows)[0]))
+    assert all(torch.equal(a, b) for other in got[1:] for a, b in zip(got[0], other))
