@@ -1,3 +1,4 @@
+import gc
 import os
 import sys
 
@@ -22,3 +23,18 @@ def pytest_collection_modifyitems(config, items):
     for item in items:
         if "gpu" in item.keywords:
             item.add_marker(skip)
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _a_device_without_the_last_modules_leftovers():
+    """Device memory that the modules before still hold, in cycles or in torch's cache, goes back first.
+
+    Tests read how much is free, and the driver reports that in steps of 2 MiB: what an allocation takes off it depends on how far
+    into such a step the others reach."""
+    import torch
+
+    if torch.cuda.is_available():
+        gc.collect()
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+    yield
