@@ -188,8 +188,9 @@ constexpr uint32_t kBlocks = 1u << 23; // of a launch
  *                  16384 x 50257           624 (628)  538 (510)  599 (659)                    (646)          (545)      (778)
  *                   4096 x 128000 f32      763 (784)  708 (776)  684 (700)                752 (770)      697 (729)  760 (828)
  *                  16384 x 32000 f32                                                      758            700 (655)  815 (897)
- * before, with a row to a workgroup and all of it through the caches, 8192 x 128000 took 817 and 842.  A float32 gradient of bf16 logits, whose
- * 16-byte stores leave gaps for one another, takes 522 through the caches and 599 past them. */
+ * before, with a row to a workgroup and all of it through the caches, 8192 x 128000 took 817 and 842.  A float32 gradient of bf16 logits goes through the
+ * caches at any size: a lane's eight elements are two stores, which leave gaps for one another, and only the caches put them together.  4096 x 128000 595 us, past
+ * them 804, distillation 540 and 833; 8192 x 50257 462 and 592, 416 and 429. */
 template <typename T, typename O> bool cut(GradArgs &a, uint64_t rows, uint32_t per, uint32_t per_large) {
     const uint32_t n = vectors_most<T>(a.vocab);
     const bool large = sizeof(O) <= sizeof(T) && rows * a.vocab * sizeof(T) > kCache;
@@ -219,16 +220,22 @@ template <typename T> bool by_waves(uint64_t vocab, uint64_t rows, uint32_t many
     return n <= 256 || (rows >= 1024 && n <= many);
 }
 
-/* LDS to ask for beyond what a workgroup of 256 uses, so that no more than `groups` of them fit a unit's 160 KB.  Fewer rows' pieces under way at once
- * leave the memory's channels less to jump between, where rows are long and begin together on 128 bytes.  us with 8, 4 and 3 workgroups to a unit:
- *     scores, bf16, entropy    8192 x 128000  742  700  831    4096 x 230400  680  615  666    8192 x 115200  604  619  687    16384 x 50257  517  550  628
- *     scores, bf16             8192 x 128000  757  756  678    4096 x 230400  686  682  597    8192 x 115200  630  630  601    16384 x 50257  512  513  559
- *     scores, f32              4096 x 128000  660  634  730    8192 x 50257   510  507  568    4096 x 65536   331  321  362
- *     distillation, f32        4096 x 128000  700       627    8192 x 50257   483       508    4096 x 65536   320       325
- * bf16 rows of 128001 take 753, 795 and 841, and the distillation of bf16 653 and, with 3, 708. */
+/* LDS to ask for beyond what a workgroup of 256 uses, so that no more than `groups` of them fit a unit's 160 KB, or none.  Fewer rows' pieces under way at once
+ * leave the memory's channels less to jump between, where rows are long, begin together on 128 bytes and are many.  By their registers the scores' kernels fit 4
+ * workgroups to a unit (bf16 without entropy, 117 registers), 5 (with entropy, 82) and 8 (f32, 52), the distillation's 4 (f32, 106).  us with those and with
+ * `groups`, for a gradient of its own and (over the logits):
+ *     scores, bf16, entropy, 4     65536 x 8192    461 505 (467 511)   21845 x 24576   368 375 (360 368)   16777 x 32000   379 343 (406 342)
+ *                                   8388 x 128000  779 741 (827 761)    5336 x 50304   174 170 (179 173)    2668 x 50304  78.3 76.6 (86.0 90.5)
+ *     scores, bf16, 3               9362 x 57344   360 373 (346 362)    7281 x 73728   378 356 (390 372)    4194 x 128000  380 354 (399 348)
+ *                                   8388 x 128000  756 694 (813 693)    2097 x 128000  183 182 (192 178)    1365 x 196608  176 188 (175 182)
+ *     distillation, f32, 3          5041 x 106496  682 687 (728 706)    4369 x 122880  708 690 (743 703)    2097 x 128000  361 349 (395 357)
+ *                                   4194 x 128000  739 692 (816 709)    1048 x 128000  179 180 (187 186)     819 x 163840  175 176 (175 181)
+ * and nowhere gained: scores of f32, with 4 (53649 x 10007 692 819, 4194 x 128000 694 713); bf16 gradients of f32, 4194 x 128000, the scores' with 4 (538 686) and the
+ * distillation's with 3 (521 582); distillation of bf16, with 3 (8388 x 128000 670 727); rows that begin anywhere (8192 x 128001 bf16 753 795).  Where the gradient's
+ * rows begin does not matter: 8 elements off, 8388 x 128000 bf16 803 704. */
 constexpr uint32_t room_for(uint32_t groups, uint32_t used = 0) { return 160 * 1024 / (groups + 1) + 512 - used; }
-template <typename T> bool long_and_even(const GradArgs &a) {
-    return a.vocab >= 120 * 1024 && ((uintptr_t)a.logits | a.stride * sizeof(T)) % 128 == 0;
+template <typename T> bool long_and_even(const GradArgs &a, uint64_t rows, uint64_t cols, uint64_t bytes) {
+    return a.vocab >= cols && rows * a.vocab * sizeof(T) >= bytes && ((uintptr_t)a.logits | a.stride * sizeof(T)) % 128 == 0;
 }
 template <typename T, typename O> int token_grad(GradArgs &a, uint64_t rows, hipStream_t s) {
 #define ERI_GRAD(TPR, ENT, PAST) in_parts(a, rows, 256 / TPR, [&](uint32_t n) { hipLaunchKernelGGL((token_grad_kernel<T, O, TPR, ENT, PAST>), dim3(n), dim3(256), lds, s, a); })
@@ -240,7 +247,10 @@ template <typename T, typename O> int token_grad(GradArgs &a, uint64_t rows, hip
         if (large) return a.grad_entropy ? ERI_GRAD(64, true, kStores) : ERI_GRAD(64, false, kStores);
         return a.grad_entropy ? ERI_GRAD(64, true, kNothing) : ERI_GRAD(64, false, kNothing);
     }
-    if (large && (kWide || long_and_even<T>(a))) lds = room_for(kWide || a.grad_entropy ? 4 : 3);
+    if (large && !kWide) {
+        if (a.grad_entropy && long_and_even<T>(a, rows, 31 << 10, 1ull << 29)) lds = room_for(4);
+        if (!a.grad_entropy && long_and_even<T>(a, rows, 72 << 10, 1ull << 30)) lds = room_for(3);
+    }
     if (!large) return a.grad_entropy ? ERI_GRAD(256, true, kNothing) : ERI_GRAD(256, false, kNothing);
     return a.grad_entropy ? ERI_GRAD(256, true, (kWide ? kBoth : kStores)) : ERI_GRAD(256, false, (kWide ? kBoth : kStores));
 #undef ERI_GRAD
@@ -254,7 +264,7 @@ template <typename T, typename O> int distill_grad(GradArgs &a, uint64_t rows, h
         a.per = vectors_most<T>(a.vocab), a.slices = 1;
         return large ? ERI_GRAD(64, kStores) : ERI_GRAD(64, kNothing);
     }
-    if (large && sizeof(T) == 4 && long_and_even<T>(a)) lds = room_for(3, kDistillMost * 2);
+    if (large && sizeof(T) == 4 && sizeof(O) == 4 && long_and_even<T>(a, rows, 120 << 10, 1ull << 30)) lds = room_for(3, kDistillMost * 2);
     return large ? ERI_GRAD(256, kStores) : ERI_GRAD(256, kNothing);
 #undef ERI_GRAD
 }

@@ -133,3 +133,38 @@ def test_the_examples_mean_is_over_the_targets_that_name_a_token():
         loss = model.loss(rows, target, 0)
         got.append((loss.detach(), torch.autograd.grad(loss, rows)[0]))
     assert all(torch.equal(a, b) for other in got[1:] for a, b in zip(got[0], other))
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# launches that rows of certain lengths and places reach
+# ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,rows,vocab", [(BF, 1100, 131072), (F32, 520, 131072), (BF, 2100, 65536), (F32, 2100, 32768)])
+def test_even_rows_that_the_caches_do_not_hold(losses, dtype, rows, vocab):  # noqa: F811
+    """Rows that all begin on 128 bytes: the gradients run with fewer workgroups to a unit where such rows are long."""
+    tl.test_logits_that_the_caches_do_not_hold(losses, dtype, rows, vocab)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,out", [(BF, BF), (F32, F32), (F32, BF), (BF, F32)])
+@pytest.mark.parametrize("vocab", [33000, 131072])
+def test_gradients_into_rows_that_begin_elsewhere(losses, dtype, out, vocab):  # noqa: F811
+    """Past the caches too: the logits begin on 128 bytes, the gradient's rows anywhere."""
+    rows = (288 << 20) // (vocab * (2 if dtype == BF else 4)) + 1
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    x = (torch.randn(rows, vocab, generator=gen, device="cuda") * 2).to(dtype)
+    ids = torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+    few = torch.randint(0, vocab, (rows, 9), generator=gen, device="cuda")
+    values = torch.log_softmax(torch.randn(rows, 10, generator=gen, device="cuda"), 1)[:, :9].contiguous()
+    g, gh = torch.randn(rows, generator=gen, device="cuda"), torch.randn(rows, generator=gen, device="cuda")
+    r, d = losses.token_logprobs(x, ids, entropy=True), losses.distill_top(x, few, values, rest=True)
+    wide = torch.empty(rows, vocab + 9, dtype=out, device="cuda")
+    for call in (lambda **k: losses.token_logprobs_grad(x, ids, r.stats, g, **k), lambda **k: losses.distill_top_grad(x, few, values, d.stats, g, **k),
+                 lambda **k: losses.token_logprobs_grad(x, ids, r.stats, g, grad_entropy=gh, entropy=r.entropy, **k)):
+        want = call(dtype=out)
+        for at in (1, 4):
+            wide.fill_(7.0)
+            call(out=wide[:, at:at + vocab])
+            assert torch.equal(wide[:, at:at + vocab], want)
+            assert bool((wide[:, :at] == 7).all()) and bool((wide[:, at + vocab:] == 7).all())
