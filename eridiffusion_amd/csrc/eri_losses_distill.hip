@@ -36,7 +36,8 @@ __device__ __forceinline__ int32_t entry_of(const DistillArgs &a, uint64_t row, 
 }
 
 /* One wave: `o` are the sums over the row, or with REST over what the teacher does not name.  fp64 where two numbers that may all but cancel are
- * made: an exponential and a logarithm more or less for each row count where rows are short (16384 x 1000 with the rest 33.5 us with seven of them). */
+ * made: an exponential and a logarithm more or less for each row count where rows are short (16384 x 1000 with the rest 33.5 us with seven of them).  What the named
+ * tokens hold and log1p of the two shares are single numbers, fp32: a unit or two in their last place. */
 template <typename T, bool REST> __device__ __forceinline__ void finish(const DistillArgs &a, uint64_t row, Sums o, int32_t id, float x, float teacher, uint32_t lane) {
     const bool used = id >= 0;
     // the student: sums over the whole row, and what the named tokens hold of it, each token once

@@ -230,7 +230,7 @@ template <typename T> bool by_waves(uint64_t vocab, uint64_t rows, uint32_t many
  *                                   8388 x 128000  756 694 (813 693)    2097 x 128000  183 182 (192 178)    1365 x 196608  176 188 (175 182)
  *     distillation, f32, 3          5041 x 106496  682 687 (728 706)    4369 x 122880  708 690 (743 703)    2097 x 128000  361 349 (395 357)
  *                                   4194 x 128000  739 692 (816 709)    1048 x 128000  179 180 (187 186)     819 x 163840  175 176 (175 181)
- * and nowhere gained: scores of f32, with 4 (53649 x 10007 692 819, 4194 x 128000 694 713); bf16 gradients of f32, 4194 x 128000, the scores' with 4 (538 686) and the
+ * Not asked for by scores of f32, with 4 (53649 x 10007 692 819, 4194 x 128000 694 713, 4369 x 122880 723 708); bf16 gradients of f32, 4194 x 128000, the scores' with 4 (538 686) and the
  * distillation's with 3 (521 582); distillation of bf16, with 3 (8388 x 128000 670 727); rows that begin anywhere (8192 x 128001 bf16 753 795).  Where the gradient's
  * rows begin does not matter: 8 elements off, 8388 x 128000 bf16 803 704. */
 constexpr uint32_t room_for(uint32_t groups, uint32_t used = 0) { return 160 * 1024 / (groups + 1) + 512 - used; }
