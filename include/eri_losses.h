@@ -59,8 +59,9 @@ int eri_token_logprobs(const EriTokenLogprobs *args, void *stream);
 
 /* The logits' gradient from grad = dL/dlogprob and grad_entropy = dL/dentropy:
  *     out[j] = (grad * ([j = id] - p[j]) - grad_entropy * p[j] * (ln p[j] + entropy)) / T
- * A row whose id names no token gets nothing from grad, and one that gets nothing from either is written with zeros and not read.  What p is 0 for gets
- * 0, as long as (grad + grad_entropy * entropy) / T and 256 grad_entropy / T are finite in F32; past that a row may hold infinities and NaN. */
+ * A row whose id names no token gets nothing from grad, and one that gets nothing from either is written with zeros and not read.  A token whose p
+ * is 0 gets nothing but grad / T where it is the named one, as long as (grad + grad_entropy * entropy) / T and 256 grad_entropy / T are finite in F32; past that
+ * a row may hold infinities and NaN. */
 typedef struct EriTokenLogprobsGrad {
     const void *logits;
     const void *ids;

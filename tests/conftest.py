@@ -29,8 +29,8 @@ def pytest_collection_modifyitems(config, items):
 def _a_device_without_the_last_modules_leftovers():
     """Device memory that the modules before still hold, in cycles or in torch's cache, goes back first.
 
-    Tests read how much is free, and the driver reports that in steps of 2 MiB: what an allocation takes off it depends on how far
-    into such a step the others reach."""
+    Tests read how much is free, which is reported in steps of 2 MiB: what an allocation takes off it depends on how far into such a
+    step the others reach."""
     import torch
 
     if torch.cuda.is_available():
